@@ -43,8 +43,10 @@ typedef enum tla_status {
   TLA_ERR_NO_DEVICE = -14,
   TLA_ERR_SHARED = -15,       /* operation not allowed on a layer that borrows another's cache */
   TLA_ERR_SCRATCH_LIMIT = -16, /* request exceeds the fixed scratch of tla_decode_noalloc */
-  TLA_ERR_BOUNDS = -17         /* device-reported, bounds-check builds only: an index outside its buffer
+  TLA_ERR_BOUNDS = -17,        /* device-reported, bounds-check builds only: an index outside its buffer
                                   (the access was skipped) */
+  TLA_ERR_PAGE = -18           /* device-reported: a page number outside the pool, or a page list out of order
+                                  (the page was left out) */
 } tla_status;
 
 /* RoPE scaling: RopeScalingConfig | YarnRoPEConfig (packages/three-llm/src/types.ts:245-256). */
@@ -70,7 +72,9 @@ enum {
   TLA_FLAG_OFFSET_RMS_NORM = 1u << 0, /* offsetRMSNorm: QK-norm scale is (1 + w) */
   TLA_FLAG_V_NORM = 1u << 1,          /* vNorm: weightless RMS norm of V before caching */
   TLA_FLAG_IO_FP32 = 1u << 2,         /* qkv, gate and out are float32 (default: fp16) */
-  TLA_FLAG_CACHE_FP32 = 1u << 3       /* K/V cache in float32 (default: fp16) */
+  TLA_FLAG_CACHE_FP32 = 1u << 3,      /* K/V cache in float32 (default: fp16) */
+  TLA_FLAG_IO_BF16 = 1u << 4,         /* paged layers: qkv, query, gate and out are bfloat16 */
+  TLA_FLAG_CACHE_BF16 = 1u << 5       /* paged layers: K/V pages in bfloat16 */
 };
 
 /* AttentionKernelOptions (packages/three-llm/src/types.ts:288-312) plus the
@@ -312,6 +316,99 @@ int tla_decode_noalloc(const tla_attn_config* config, void* key_cache, void* val
                        const float* q_norm_weight, const float* k_norm_weight, const void* qkv,
                        const int32_t* positions, const void* gate, void* out, int32_t* status, int32_t batch,
                        void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged key-value cache (no counterpart in the reference, whose cache is one
+ * contiguous block per sequence). The K/V of all sequences live in a pool of
+ * fixed-size pages that the caller owns and hands out; a page table lists
+ * each sequence's pages in order, so a sequence holds memory for the tokens
+ * it has, grows page by page, and may share its first pages with others.
+ *
+ * Page tables are device int32 [batch][table_width], row b for sequence b:
+ * token t of sequence b lives in slot t % page_size of page
+ * page_table[b][t / page_size]. Entries past the sequence's last page are not
+ * read. A page number outside [0, page_count) that is needed is reported
+ * (TLA_ERR_PAGE through tla_get_error) and left out: nothing is stored to it
+ * and its tokens take no part.
+ *
+ * positions are device int32 [batch]. A negative position marks a row without
+ * a sequence (a batch padded to a captured size): nothing is appended for it
+ * and its query, output and page-list rows are zeros, zeros and -1. A position
+ * at or past the capacity, min(max_tokens, table_width * page_size), is
+ * reported (TLA_ERR_POSITION) and its row treated the same way.
+ *
+ * The calls are stream-ordered, allocate nothing and hold no state between
+ * calls outside the caller's buffers: calls on one layer may run at the same
+ * time on several streams as long as no call writes what another reads (give
+ * each its own workspace), and all may be captured in CUDA graphs. */
+typedef struct tla_page_pool {
+  void* key;               /* device; element (page, kv_head, slot, d) at key + page*page_stride + */
+  void* value;             /* kv_head*head_stride + slot*slot_stride + d, strides in elements      */
+  void* bounds;            /* device [page_count][kv_head_count][2][head_dim] in the pages' type, 16-byte
+                              aligned, or NULL: per page the smallest and the largest key of every
+                              dimension over the slots appended so far */
+  int64_t page_stride, head_stride, slot_stride;
+  int32_t page_count;
+  int32_t page_size;       /* tokens per page: a power of two up to 1024 */
+} tla_page_pool;
+
+typedef struct tla_paged tla_paged;
+
+/* A layer over a page pool. config as for tla_layer_create, except that the
+ * cache is the caller's pool: max_tokens bounds the positions, max_batch the
+ * sequences of one call, kv_head_count must divide head_count, and the flags
+ * may name bfloat16. The I/O type is the pages' type, or float32 over any
+ * pages. No two elements of the pool may share an address. The pool is
+ * neither copied nor cleared; its memory must outlive the layer. */
+int tla_paged_create(tla_ctx* ctx, const tla_attn_config* config, const tla_page_pool* pool,
+                     const float* q_norm_weight, const float* k_norm_weight, tla_paged** out);
+int tla_paged_destroy(tla_paged* layer);
+
+/* Appends K/V: QK-norm, RoPE and vNorm as tla_decode forms them, then the rows'
+ * K and V into their slots and, when the pool has bounds, the keys as stored
+ * into their pages' bounds (slot 0 starts a page's bounds afresh).
+ *   qkv         device [rows][head_count + 2*kv_head_count][head_dim]
+ *   row_offsets NULL: rows == batch, and row b is sequence b's new token at positions[b];
+ *               else device int32 [batch + 1], ascending from 0 to at most rows: rows
+ *               row_offsets[b] .. row_offsets[b+1]-1 are sequence b's next tokens, at positions[b],
+ *               positions[b] + 1, ...; rows past row_offsets[batch] are left alone
+ *   query_out   device [rows][head_count][head_dim], the rotated queries in the I/O type, or NULL
+ * The sequences of one call may share no page that the call appends to. */
+int tla_paged_append(tla_paged* layer, const void* qkv, const int32_t* positions, const int32_t* row_offsets,
+                     const int32_t* page_table, int32_t table_width, int32_t batch, int32_t rows, void* query_out,
+                     void* stream);
+
+/* Device bytes of workspace that tla_paged_decode and tla_paged_select need for
+ * up to `batch` sequences and this table width (16-byte aligned; the contents
+ * need no preparation and mean nothing afterwards). */
+int tla_paged_workspace(const tla_paged* layer, int32_t batch, int32_t table_width, size_t* bytes);
+
+/* Attention of one new token per sequence over its pages, the new token's own
+ * K/V included (append first): over the tokens of [window start, positions[b]],
+ * or of those the tokens on the listed pages.
+ *   query device [batch][head_count][head_dim] in the I/O type (tla_paged_append's query_out)
+ *   pages NULL, or device int32 [batch][kv_head_count][page_count]: page indexes within the sequence
+ *         (t / page_size), rising (tla_paged_select's output). A list ends before its first negative
+ *         entry; it also ends, and TLA_ERR_PAGE is reported, before an entry that does not rise or
+ *         lies past the position
+ *   gate  device [batch][head_count][head_dim] or NULL; out device [batch][head_count][head_dim]
+ * A row with nothing to attend to is zeros. */
+int tla_paged_decode(tla_paged* layer, const void* query, const int32_t* positions, const int32_t* page_table,
+                     int32_t table_width, const int32_t* pages, int32_t page_count, const void* gate, void* out,
+                     int32_t batch, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The pages a decode step should read, per sequence and kv head: of the pages
+ * holding [window start, positions[b]] the first `first_pages`, the last
+ * `last_pages` and the best of the others, `page_count` in all (all of them
+ * when there are no more). A page's score is the sum over the kv head's query
+ * heads and over d of q_d * high_d where q_d > 0 and q_d * low_d where q_d < 0,
+ * low and high being its bounds: an upper bound on the summed dot products
+ * with any of its keys. It is summed in 64 bits and rounded to 32; ties go to
+ * the lower page. Needs a pool with bounds and a positive attn_scale.
+ *   pages_out device int32 [batch][kv_head_count][page_count], rising, then -1 */
+int tla_paged_select(tla_paged* layer, const void* query, const int32_t* positions, const int32_t* page_table,
+                     int32_t table_width, int32_t first_pages, int32_t last_pages, int32_t* pages_out,
+                     int32_t page_count, int32_t batch, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -19,12 +19,15 @@ STATUS = {
     -8: "TLA_ERR_ROTARY_DIM", -9: "TLA_ERR_UNSUPPORTED", -10: "TLA_ERR_CUDA", -11: "TLA_ERR_OUT_OF_MEMORY",
     -12: "TLA_ERR_POSITION", -13: "TLA_ERR_TIMEOUT", -14: "TLA_ERR_NO_DEVICE", -15: "TLA_ERR_SHARED",
     -16: "TLA_ERR_SCRATCH_LIMIT", -17: "TLA_ERR_BOUNDS",
+    -18: "TLA_ERR_PAGE",
 }
 ROPE_TYPES = {"default": 0, "none": 0, "linear": 1, "yarn": 2, "llama3": 3}
 FLAG_OFFSET_RMS_NORM = 1 << 0
 FLAG_V_NORM = 1 << 1
 FLAG_IO_FP32 = 1 << 2
 FLAG_CACHE_FP32 = 1 << 3
+FLAG_IO_BF16 = 1 << 4
+FLAG_CACHE_BF16 = 1 << 5
 
 EXPORTS = [
     "tla_status_string", "tla_create", "tla_destroy", "tla_get_error", "tla_rope_parameters", "tla_layer_create",
@@ -33,6 +36,8 @@ EXPORTS = [
     "tla_decode_noalloc", "tla_exchange_create", "tla_exchange_connect", "tla_exchange_combine",
     "tla_exchange_buffer", "tla_exchange_connect_buffers", "tla_exchange_destroy", "tla_decode_exchange",
     "tla_query", "tla_scores", "tla_qkv_decode", "tla_qkv_prefill", "tla_out_proj", "tla_out_proj_allreduce",
+    "tla_paged_create", "tla_paged_destroy", "tla_paged_append", "tla_paged_workspace", "tla_paged_decode",
+    "tla_paged_select",
 ]
 
 
@@ -88,6 +93,19 @@ class CacheView(ctypes.Structure):
     ]
 
 
+class PagePool(ctypes.Structure):
+    _fields_ = [
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("bounds", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64),
+        ("page_count", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -131,6 +149,13 @@ def lib():
         L.tla_exchange_destroy.argtypes = [P]
         L.tla_decode_exchange.argtypes = [P, P, P, P, i32, i32, i32, P, P, P, i32, P]
         L.tla_decode_noalloc.argtypes = [ctypes.POINTER(AttnConfig), P, P, P, P, P, P, P, P, P, i32, P]
+        size_t = ctypes.c_size_t
+        L.tla_paged_create.argtypes = [P, ctypes.POINTER(AttnConfig), ctypes.POINTER(PagePool), P, P, ctypes.POINTER(P)]
+        L.tla_paged_destroy.argtypes = [P]
+        L.tla_paged_append.argtypes = [P, P, P, P, P, i32, i32, i32, P, P]
+        L.tla_paged_workspace.argtypes = [P, i32, i32, ctypes.POINTER(size_t)]
+        L.tla_paged_decode.argtypes = [P, P, P, P, i32, P, i32, P, P, i32, P, size_t, P]
+        L.tla_paged_select.argtypes = [P, P, P, P, i32, i32, i32, P, i32, i32, P, size_t, P]
         for name in EXPORTS:
             if name != "tla_status_string":
                 getattr(L, name).restype = ctypes.c_int

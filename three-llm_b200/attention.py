@@ -63,6 +63,32 @@ def rope_parameters(dim, theta, scaling=None):
     return inv[: dim // 2], af.value
 
 
+def attn_config(o, head_count, kv_head_count, head_dim, max_tokens, max_batch):
+    """tla_attn_config of the AttentionKernelOptions keys (types.ts:288-312) in `o`; the norm flags are set."""
+    rotary = o["rotaryDim"] if o.get("rotaryDim") is not None else head_dim                    # TSLAttention.ts:81
+    scaling = o.get("ropeScaling") or o.get("yarn")
+    if scaling is not None and o.get("ropeScaling") is None and "type" not in scaling:
+        scaling = dict(scaling, type="yarn")
+    cfg = _abi.AttnConfig()
+    cfg.head_count = head_count
+    cfg.kv_head_count = kv_head_count
+    cfg.head_dim = head_dim
+    cfg.max_tokens = max_tokens
+    cfg.max_batch = max_batch
+    cfg.rotary_dim = rotary
+    cfg.rope_freq_dim = o.get("ropeFreqDim") or rotary                                         # :82
+    cfg.rope_pair_count = o["ropePairCount"] if o.get("ropePairCount") is not None else rotary // 2  # :83
+    cfg.rope_theta = float(o.get("ropeTheta") or 0)                                            # :80
+    cfg.rope_scaling = _abi.make_scaling(scaling)
+    cfg.sliding_window = o.get("slidingWindow") or 0                                           # :94
+    cfg.has_attn_scale = 1
+    cfg.attn_scale = float(o["attnScale"] if o.get("attnScale") is not None else 1 / math.sqrt(head_dim))
+    cfg.rms_epsilon = float(o.get("rmsEpsilon") or 1e-6)                                       # :96
+    cfg.flags = ((_abi.FLAG_OFFSET_RMS_NORM if o.get("offsetRMSNorm") is True else 0)
+                 | (_abi.FLAG_V_NORM if o.get("vNorm") is True else 0))
+    return cfg
+
+
 class CUDAAttention:
     """Drop-in for TSLAttention: `new TSLAttention(qkvNode, hiddenSize, headCount, maxTokens, options)`.
 
@@ -105,34 +131,13 @@ class CUDAAttention:
         self.dtype = dtype
         self.device = qkv_node.device if qkv_node is not None else torch.device("cuda", torch.cuda.current_device())
         self.context = context or Context.default(self.device.index or 0)
-        scaling = o.get("ropeScaling") or o.get("yarn")
-        if scaling is not None and o.get("ropeScaling") is None and "type" not in scaling:
-            scaling = dict(scaling, type="yarn")
-        cfg = _abi.AttnConfig()
-        cfg.head_count = self.headCount
-        cfg.kv_head_count = self.kvHeadCount
-        cfg.head_dim = self.headDim
-        cfg.max_tokens = max_tokens
-        cfg.max_batch = self.maxBatch
-        cfg.rotary_dim = self.rotaryDim
-        cfg.rope_freq_dim = self.ropeFreqDim
-        cfg.rope_pair_count = self.ropePairCount
-        cfg.rope_theta = float(self.ropeTheta)
-        cfg.rope_scaling = _abi.make_scaling(scaling)
-        cfg.sliding_window = self.slidingWindow
-        cfg.has_attn_scale = 1
-        cfg.attn_scale = float(self.attnScale)
-        cfg.rms_epsilon = float(self.rmsEpsilon)
+        cfg = attn_config(o, self.headCount, self.kvHeadCount, self.headDim, max_tokens, self.maxBatch)
         flags = 0
-        if self.offsetRMSNorm:
-            flags |= _abi.FLAG_OFFSET_RMS_NORM
-        if self.vNorm:
-            flags |= _abi.FLAG_V_NORM
         if dtype == torch.float32:
             flags |= _abi.FLAG_IO_FP32
         if o.get("cacheDtype", "float16") in ("float32", torch.float32):
             flags |= _abi.FLAG_CACHE_FP32
-        cfg.flags = flags
+        cfg.flags |= flags
         self._qn = None if o.get("qNormWeight") is None else np.ascontiguousarray(o["qNormWeight"], np.float32)
         self._kn = None if o.get("kNormWeight") is None else np.ascontiguousarray(o["kNormWeight"], np.float32)
         h = ctypes.c_void_p()

@@ -1439,6 +1439,7 @@ extern "C" int tla_decode_noalloc(const tla_attn_config* cfg, void* key_cache, v
       cfg->sliding_window < 0)
     return TLA_ERR_INVALID_ARG;
   // Only the shapes of the fast kernel: fp16 cache, head_dim 64/128, GQA group <= 16.
+  if (cfg->flags & (TLA_FLAG_IO_BF16 | TLA_FLAG_CACHE_BF16)) return TLA_ERR_UNSUPPORTED;  // paged layers only
   if ((cfg->flags & TLA_FLAG_CACHE_FP32) || (D != 64 && D != 128) || Hq % Hk != 0 || Hq / Hk > 16 ||
       cfg->max_batch > kMaxBatch)
     return TLA_ERR_UNSUPPORTED;

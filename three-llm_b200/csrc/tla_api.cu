@@ -11,6 +11,7 @@
 
 #include "tla_device.cuh"
 #include "exchange.cuh"
+#include "tla_host.h"
 #include "tla_internal.h"
 
 namespace tla {
@@ -115,25 +116,11 @@ cudaError_t cached_occupancy(const void* kernel, int threads, int smem, int* blo
 }
 }  // namespace tla
 
+using tla::DeviceGuard;
+using tla::dev_alloc;
+using tla::from_cuda;
+
 namespace {
-
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    if (prev >= 0) cudaSetDevice(prev);
-  }
-};
-
-int from_cuda(cudaError_t e) {
-  if (e == cudaSuccess) return TLA_OK;
-  if (getenv("TLA_DEBUG")) fprintf(stderr, "tla: CUDA error %d: %s\n", static_cast<int>(e), cudaGetErrorString(e));
-  if (e == cudaErrorMemoryAllocation) return TLA_ERR_OUT_OF_MEMORY;
-  return TLA_ERR_CUDA;
-}
 
 // ropeParameters, packages/three-llm/src/runtime/rope.ts:4-52: double
 // arithmetic, float32 table.
@@ -183,13 +170,6 @@ int rope_parameters(int32_t dim, double theta, const tla_rope_scaling* scaling, 
   return TLA_OK;
 }
 
-template <typename T>
-int dev_alloc(T** p, size_t count) {
-  *p = nullptr;
-  if (count == 0) return TLA_OK;
-  return from_cuda(cudaMalloc(reinterpret_cast<void**>(p), count * sizeof(T)));
-}
-
 int ensure_qscratch(tla_ctx* ctx, size_t bytes) {
   if (bytes <= ctx->qscratch_bytes) return TLA_OK;
   if (ctx->d_qscratch) cudaFree(ctx->d_qscratch);
@@ -204,6 +184,71 @@ int ensure_qscratch(tla_ctx* ctx, size_t bytes) {
 bool valid_layer(const tla_layer* L) { return L && L->ctx && L->k_cache && L->v_cache; }
 
 }  // namespace
+
+namespace tla {
+
+int layer_params(const tla_attn_config* cfg, tla_layer* L, std::vector<float>* inv_freq) {
+  const int Hq = cfg->head_count, D = cfg->head_dim;
+  const int Hk = cfg->kv_head_count > 0 ? cfg->kv_head_count : Hq;
+  if (Hq <= 0 || D <= 0 || Hk > Hq || cfg->max_tokens <= 0 || cfg->max_batch <= 0 || cfg->sliding_window < 0)
+    return TLA_ERR_INVALID_ARG;
+  if (D > 256) return TLA_ERR_UNSUPPORTED;
+  const int rotary = cfg->rotary_dim < 0 ? D : cfg->rotary_dim;
+  if (rotary % 2 != 0 || rotary > D) return TLA_ERR_ROTARY_DIM;  // load/DecoderRecipe.ts:409-415
+  const bool rope_on = cfg->rope_theta > 0 && rotary > 0;       // math.ts:217, TSLAttention.ts:84-87
+  const int freq_dim = cfg->rope_freq_dim > 0 ? cfg->rope_freq_dim : rotary;
+  const int pair_count = cfg->rope_pair_count >= 0 ? cfg->rope_pair_count : rotary / 2;
+  inv_freq->assign(static_cast<size_t>(freq_dim / 2) + 1, 0.f);
+  double af = 1;
+  if (rope_on) {
+    int rc = rope_parameters(freq_dim, cfg->rope_theta, &cfg->rope_scaling, inv_freq->data(), &af);
+    if (rc != TLA_OK) return rc;
+    // invFreq[k] past the table would be undefined (NaN) in the reference.
+    if (pair_count > freq_dim / 2) return TLA_ERR_INVALID_ARG;
+  }
+  L->cfg = *cfg;
+  L->Hq = Hq;
+  L->Hk = Hk;
+  L->D = D;
+  L->G = (Hq % Hk == 0) ? Hq / Hk : 0;
+  L->max_tokens = cfg->max_tokens;
+  L->max_batch = cfg->max_batch;
+  L->rotary = rope_on ? rotary : 0;
+  L->freq_half = rope_on ? freq_dim / 2 : 0;
+  L->pair_count = rope_on ? (pair_count < rotary / 2 ? pair_count : rotary / 2) : 0;
+  L->sliding = cfg->sliding_window;
+  L->attn_scale = static_cast<float>(cfg->has_attn_scale ? cfg->attn_scale : 1 / sqrt(static_cast<double>(D)));
+  L->attn_factor = static_cast<float>(af);
+  L->rms_eps = static_cast<float>(cfg->rms_epsilon > 0 ? cfg->rms_epsilon : 1e-6);
+  L->io_fp32 = (cfg->flags & TLA_FLAG_IO_FP32) != 0;
+  L->cache_fp32 = (cfg->flags & TLA_FLAG_CACHE_FP32) != 0;
+  L->v_norm = (cfg->flags & TLA_FLAG_V_NORM) != 0;
+  L->offset_rms = (cfg->flags & TLA_FLAG_OFFSET_RMS_NORM) != 0;
+  return TLA_OK;
+}
+
+int layer_tables(tla_layer* L, const std::vector<float>& inv_freq, const float* q_norm_weight,
+                 const float* k_norm_weight) {
+  int rc = dev_alloc(&L->d_inv_freq, inv_freq.size());
+  if (rc == TLA_OK)
+    rc = from_cuda(cudaMemcpy(L->d_inv_freq, inv_freq.data(), inv_freq.size() * sizeof(float),
+                              cudaMemcpyHostToDevice));
+  if (rc == TLA_OK && q_norm_weight) {
+    rc = dev_alloc(&L->d_qnorm, L->D);
+    if (rc == TLA_OK)
+      rc = from_cuda(cudaMemcpy(L->d_qnorm, q_norm_weight, L->D * sizeof(float), cudaMemcpyHostToDevice));
+  }
+  if (rc == TLA_OK && k_norm_weight) {
+    rc = dev_alloc(&L->d_knorm, L->D);
+    if (rc == TLA_OK)
+      rc = from_cuda(cudaMemcpy(L->d_knorm, k_norm_weight, L->D * sizeof(float), cudaMemcpyHostToDevice));
+  }
+  L->has_qnorm = q_norm_weight != nullptr;
+  L->has_knorm = k_norm_weight != nullptr;
+  return rc;
+}
+
+}  // namespace tla
 
 extern "C" {
 
@@ -227,6 +272,7 @@ const char* tla_status_string(int status) {
     case TLA_ERR_SHARED: return "layer borrows another layer's cache";
     case TLA_ERR_SCRATCH_LIMIT: return "request exceeds the fixed scratch of the allocation-free decode";
     case TLA_ERR_BOUNDS: return "index outside its buffer (bounds-check build)";
+    case TLA_ERR_PAGE: return "page outside the pool, or page list out of order";
     default: return "unknown status";
   }
 }
@@ -302,64 +348,22 @@ int tla_layer_create(tla_ctx* ctx, const tla_attn_config* cfg, const float* q_no
                      tla_layer** out) {
   if (!ctx || !cfg || !out) return TLA_ERR_INVALID_ARG;
   *out = nullptr;
-  const int Hq = cfg->head_count, D = cfg->head_dim;
-  const int Hk = cfg->kv_head_count > 0 ? cfg->kv_head_count : Hq;
-  if (Hq <= 0 || D <= 0 || Hk > Hq || cfg->max_tokens <= 0 || cfg->max_batch <= 0 || cfg->sliding_window < 0)
-    return TLA_ERR_INVALID_ARG;
-  if (D > 256) return TLA_ERR_UNSUPPORTED;
-  const int rotary = cfg->rotary_dim < 0 ? D : cfg->rotary_dim;
-  if (rotary % 2 != 0 || rotary > D) return TLA_ERR_ROTARY_DIM;  // load/DecoderRecipe.ts:409-415
-  const bool rope_on = cfg->rope_theta > 0 && rotary > 0;       // math.ts:217, TSLAttention.ts:84-87
-  const int freq_dim = cfg->rope_freq_dim > 0 ? cfg->rope_freq_dim : rotary;
-  const int pair_count = cfg->rope_pair_count >= 0 ? cfg->rope_pair_count : rotary / 2;
-  std::vector<float> inv(static_cast<size_t>(freq_dim / 2) + 1, 0.f);
-  double af = 1;
-  if (rope_on) {
-    int rc = rope_parameters(freq_dim, cfg->rope_theta, &cfg->rope_scaling, inv.data(), &af);
-    if (rc != TLA_OK) return rc;
-    // invFreq[k] past the table would be undefined (NaN) in the reference.
-    if (pair_count > freq_dim / 2) return TLA_ERR_INVALID_ARG;
-  }
+  if (cfg->flags & (TLA_FLAG_IO_BF16 | TLA_FLAG_CACHE_BF16)) return TLA_ERR_UNSUPPORTED;  // paged layers only
+  tla_layer params;
+  std::vector<float> inv;
+  int rc = tla::layer_params(cfg, &params, &inv);
+  if (rc != TLA_OK) return rc;
   DeviceGuard g(ctx->device);
-  tla_layer* L = new tla_layer();
+  tla_layer* L = new tla_layer(params);
   L->ctx = ctx;
-  L->cfg = *cfg;
-  L->Hq = Hq;
-  L->Hk = Hk;
-  L->D = D;
-  L->G = (Hq % Hk == 0) ? Hq / Hk : 0;
-  L->max_tokens = cfg->max_tokens;
-  L->max_batch = cfg->max_batch;
-  L->rotary = rope_on ? rotary : 0;
-  L->freq_half = rope_on ? freq_dim / 2 : 0;
-  L->pair_count = rope_on ? (pair_count < rotary / 2 ? pair_count : rotary / 2) : 0;
-  L->sliding = cfg->sliding_window;
-  L->attn_scale = static_cast<float>(cfg->has_attn_scale ? cfg->attn_scale : 1 / sqrt(static_cast<double>(D)));
-  L->attn_factor = static_cast<float>(af);
-  L->rms_eps = static_cast<float>(cfg->rms_epsilon > 0 ? cfg->rms_epsilon : 1e-6);
-  L->io_fp32 = (cfg->flags & TLA_FLAG_IO_FP32) != 0;
-  L->cache_fp32 = (cfg->flags & TLA_FLAG_CACHE_FP32) != 0;
-  L->v_norm = (cfg->flags & TLA_FLAG_V_NORM) != 0;
-  L->offset_rms = (cfg->flags & TLA_FLAG_OFFSET_RMS_NORM) != 0;
+  const int Hk = L->Hk, D = L->D;
   const size_t elems = static_cast<size_t>(L->max_batch) * Hk * L->max_tokens * D;
   const size_t ebytes = L->cache_fp32 ? 4 : 2;
-  int rc = from_cuda(cudaMalloc(&L->k_cache, elems * ebytes));
+  rc = from_cuda(cudaMalloc(&L->k_cache, elems * ebytes));
   if (rc == TLA_OK) rc = from_cuda(cudaMalloc(&L->v_cache, elems * ebytes));
   if (rc == TLA_OK) rc = from_cuda(cudaMemset(L->k_cache, 0, elems * ebytes));
   if (rc == TLA_OK) rc = from_cuda(cudaMemset(L->v_cache, 0, elems * ebytes));
-  if (rc == TLA_OK) rc = dev_alloc(&L->d_inv_freq, inv.size());
-  if (rc == TLA_OK)
-    rc = from_cuda(cudaMemcpy(L->d_inv_freq, inv.data(), inv.size() * sizeof(float), cudaMemcpyHostToDevice));
-  if (rc == TLA_OK && q_norm_weight) {
-    rc = dev_alloc(&L->d_qnorm, D);
-    if (rc == TLA_OK) rc = from_cuda(cudaMemcpy(L->d_qnorm, q_norm_weight, D * sizeof(float), cudaMemcpyHostToDevice));
-  }
-  if (rc == TLA_OK && k_norm_weight) {
-    rc = dev_alloc(&L->d_knorm, D);
-    if (rc == TLA_OK) rc = from_cuda(cudaMemcpy(L->d_knorm, k_norm_weight, D * sizeof(float), cudaMemcpyHostToDevice));
-  }
-  L->has_qnorm = q_norm_weight != nullptr;
-  L->has_knorm = k_norm_weight != nullptr;
+  if (rc == TLA_OK) rc = tla::layer_tables(L, inv, q_norm_weight, k_norm_weight);
   if (rc == TLA_OK && L->G > 0) rc = from_cuda(tla::decode_fast_configure(L));
   if (rc == TLA_OK && L->fast_decode) {
     const size_t need = tla::decode_fast_scratch_floats(L);

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -230,6 +231,10 @@ template <>
 __device__ __forceinline__ float to_f32<__half>(__half v) {
   return __half2float(v);
 }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
@@ -239,6 +244,11 @@ __device__ __forceinline__ float from_f32<float>(float v) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) {
   return __float2half_rn(v);
+}
+
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {

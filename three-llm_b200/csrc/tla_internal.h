@@ -57,7 +57,22 @@ struct tla_layer {
   CUtensorMap tmap_k128{}, tmap_v128{};  // 128-token boxes
 };
 
+// A layer over a caller's page pool. `base` carries the head shapes, RoPE and
+// norms; its cache pointers are the pool's.
+struct tla_paged {
+  tla_layer base;
+  tla_page_pool pool{};
+  int io = 0, kept = 0;     // tla::Type of the activations and of the pages
+  int page_shift = 0;       // log2(page_size)
+  // tensor-core decode path (16-bit pages, D in {64, 128}, page_size >= 16)
+  bool fast = false;
+  int fast_grid = 0;        // persistent CTAs per launch
+  CUtensorMap tmap_k{}, tmap_v{};
+};
+
 namespace tla {
+
+enum Type { kFp16 = 0, kBf16 = 1, kFp32 = 2 };
 
 // Launch with programmatic dependent launch allowed: the kernel may start
 // while the previous kernel in the stream finishes; it waits (griddep_wait)
@@ -176,5 +191,32 @@ cudaError_t launch_out_proj_allreduce(tla_ctx* ctx, const ExchangeDev& x, const 
 cudaError_t launch_out_proj(tla_ctx* ctx, const void* attn, const void* weight, const float* bias,
                             const void* residual, bool residual_f32, void* y, bool y_f32, int rows, int in_features,
                             int hidden, cudaStream_t stream);
+
+// ---------------------------------------------------------------- paged cache
+// What every kernel of a paged call gets: the layer, the pool and the table.
+struct PagedArgs {
+  LayerArgs a;
+  void* key;
+  void* value;
+  void* bounds;
+  int64_t page_stride, head_stride, slot_stride;  // elements
+  const int32_t* table;                           // [batch][width]
+  const int32_t* positions;                       // [batch]
+  int width, batch;
+  int page_count, page_shift;
+  int capacity;  // tokens a sequence can hold: min(max_tokens, width * page_size)
+};
+PagedArgs paged_args(const tla_paged* P, const int32_t* positions, const int32_t* table, int width, int batch);
+
+cudaError_t launch_paged_append(const tla_paged* P, const PagedArgs& p, const void* qkv, const int32_t* offsets,
+                                int rows, void* query_out, cudaStream_t stream);
+cudaError_t launch_paged_select(const tla_paged* P, const PagedArgs& p, const void* query, int first, int last,
+                                int32_t* pages_out, int count, void* workspace, cudaStream_t stream);
+size_t paged_select_workspace(const tla_paged* P, int batch, int width);
+// pages: null, or the listed pages [batch][Hk][count].
+cudaError_t launch_paged_decode_generic(const tla_paged* P, const PagedArgs& p, const void* query,
+                                        const int32_t* pages, int count, const void* gate, void* out, void* workspace,
+                                        cudaStream_t stream);
+size_t paged_decode_generic_workspace(const tla_paged* P, int batch);
 
 }  // namespace tla
