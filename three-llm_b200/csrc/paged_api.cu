@@ -63,7 +63,11 @@ bool rows_apart(const tla_page_pool& pool, int heads, int D) {
   return true;
 }
 
-size_t decode_workspace(const tla_paged* P, int batch) { return tla::paged_decode_generic_workspace(P, batch); }
+// Enough for either decode path: which one runs depends on the call.
+size_t decode_workspace(const tla_paged* P, int batch) {
+  const size_t a = tla::paged_decode_generic_workspace(P, batch), b = tla::paged_decode_workspace(P);
+  return a > b ? a : b;
+}
 
 }  // namespace
 
@@ -106,6 +110,7 @@ int tla_paged_create(tla_ctx* ctx, const tla_attn_config* cfg, const tla_page_po
   P->io = io;
   P->kept = kept;
   while ((1 << P->page_shift) < pool->page_size) ++P->page_shift;
+  tla::paged_decode_configure(P);
   rc = tla::layer_tables(&P->base, inv, q_norm_weight, k_norm_weight);
   if (rc != TLA_OK) {
     tla_paged_destroy(P);
@@ -162,6 +167,9 @@ int tla_paged_decode(tla_paged* P, const void* query, const int32_t* positions, 
   if (need > 0 && (!workspace || workspace_bytes < need)) return TLA_ERR_INVALID_ARG;
   DeviceGuard g(P->base.ctx->device);
   const tla::PagedArgs p = tla::paged_args(P, positions, page_table, table_width, batch);
+  if (tla::paged_decode_takes(P, p, page_count))
+    return from_cuda(tla::launch_paged_decode(P, p, query, pages, page_count, gate, out, workspace,
+                                              static_cast<cudaStream_t>(stream)));
   return from_cuda(tla::launch_paged_decode_generic(P, p, query, pages, page_count, gate, out, workspace,
                                                     static_cast<cudaStream_t>(stream)));
 }

@@ -66,7 +66,6 @@ struct tla_paged {
   int page_shift = 0;       // log2(page_size)
   // tensor-core decode path (16-bit pages, D in {64, 128}, page_size >= 16)
   bool fast = false;
-  int fast_grid = 0;        // persistent CTAs per launch
   CUtensorMap tmap_k{}, tmap_v{};
 };
 
@@ -218,5 +217,11 @@ cudaError_t launch_paged_decode_generic(const tla_paged* P, const PagedArgs& p, 
                                         const int32_t* pages, int count, const void* gate, void* out, void* workspace,
                                         cudaStream_t stream);
 size_t paged_decode_generic_workspace(const tla_paged* P, int batch);
+// Tensor-core path: set up at creation, and whether it takes a call (count: listed pages, 0 for all).
+void paged_decode_configure(tla_paged* P);
+bool paged_decode_takes(const tla_paged* P, const PagedArgs& p, int count);
+size_t paged_decode_workspace(const tla_paged* P);
+cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const void* query, const int32_t* pages,
+                                int count, const void* gate, void* out, void* workspace, cudaStream_t stream);
 
 }  // namespace tla
