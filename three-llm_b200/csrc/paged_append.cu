@@ -123,8 +123,278 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// Bounds of the pages that a chunk touched, from the keys as stored: the block
-// of a page's first new row walks the page's new slots.
+// Four neighbouring elements.
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const __half* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                     __uint_as_float(u.y & 0xffff0000u));
+}
+__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void store4(__half* p, float4 v) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+// A rounding to the pages' type, as a float.
+template <typename CT>
+__device__ __forceinline__ float4 as_stored(float4 v) {
+  return make_float4(to_f32(from_f32<CT>(v.x)), to_f32(from_f32<CT>(v.y)), to_f32(from_f32<CT>(v.z)),
+                     to_f32(from_f32<CT>(v.w)));
+}
+// (the comparison's order keeps what is there when either is NaN, as low_of and high_of do)
+__device__ __forceinline__ float4 low4(float4 a, float4 b) {
+  return make_float4(b.x < a.x ? b.x : a.x, b.y < a.y ? b.y : a.y, b.z < a.z ? b.z : a.z, b.w < a.w ? b.w : a.w);
+}
+__device__ __forceinline__ float4 high4(float4 a, float4 b) {
+  return make_float4(b.x > a.x ? b.x : a.x, b.y > a.y ? b.y : a.y, b.z > a.z ? b.z : a.z, b.w > a.w ? b.w : a.w);
+}
+
+// head_dim 64 or 128, rotary dimensions a multiple of 8: D / 8 lanes hold a
+// head, each the four rotation pairs 4 l .. 4 l + 3 (both elements, so that no
+// lane needs another's; dimensions past the rotary ones pair up among
+// themselves and stay). `parts` warps share a row's heads, so that few rows
+// still fill the GPU; a warp forms the row's cosines and sines once, one or
+// two per lane, and hands them out by shuffles. Rows of a long prompt are
+// bound by memory (about 60 instructions per lane and 16 bytes read).
+template <typename IO, typename CT, int D>
+__global__ void __launch_bounds__(kThreads)
+    paged_append_rows_kernel(PagedArgs p, const IO* __restrict__ qkv, const int32_t* __restrict__ offsets, int rows,
+                             IO* __restrict__ query_out, int parts, int part_heads) {
+  constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes per head, heads per warp-wide load
+  constexpr int kLoads = sizeof(IO) == 2 ? 4 : 2;    // warp-wide loads in flight
+  const unsigned full = 0xffffffffu;
+  const LayerArgs& a = p.a;
+  const int Hq = a.Hq, Hk = a.Hk, heads = Hq + 2 * Hk, half = a.rotary / 2;
+  const int lane = threadIdx.x & 31, group = lane / kLanes, i0 = 4 * (lane % kLanes);
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  const int row = static_cast<int>(unit / parts), part = static_cast<int>(unit % parts);
+  // the first elements of the lane's four pairs, and their partners
+  const int d0 = i0 < half ? i0 : a.rotary + i0 - half;
+  const int d1 = d0 + (i0 < half ? half : (D - a.rotary) / 2);
+  griddep_wait();
+  griddep_launch_dependents();
+  if (row >= rows) return;
+  const int h_begin = part * part_heads, h_end = min(heads, h_begin + part_heads);
+  const IO* src = qkv + static_cast<int64_t>(row) * heads * D;
+  const int b = sequence_of(offsets, p.batch, row);
+  if (b < 0) return;
+  const int start = p.positions[b];
+  const int pos = start < 0 || !offsets ? start
+                  : static_cast<int>(min(start + (static_cast<long long>(row) - offsets[b]), 0x7fffffffLL));
+  if (pos < 0 || pos >= p.capacity) {
+    if (pos >= 0 && lane == 0) report_error(a.error, TLA_ERR_POSITION);
+    if (query_out)
+      for (int h = h_begin + group; h < min(h_end, Hq); h += kPer) {
+        IO* q = query_out + (static_cast<int64_t>(row) * Hq + h) * D;
+        store4(q + d0, make_float4(0.f, 0.f, 0.f, 0.f));
+        store4(q + d1, make_float4(0.f, 0.f, 0.f, 0.f));
+      }
+    return;
+  }
+  const int slot = pos & ((1 << p.page_shift) - 1);
+  // (a part with queries only does not need the page)
+  const int page = h_end > Hq ? pool_page(p, b, pos >> p.page_shift) : -1;
+  float cos4[4], sin4[4];
+  if (h_begin < Hq + Hk) {
+    float c0 = 1.f, s0 = 0.f, c1 = 1.f, s1 = 0.f;
+    if (lane < min(a.pair_count, half)) rope_cos_sin(pos, a.inv_freq[lane], &c0, &s0);
+    if (D == 128 && lane + 32 < min(a.pair_count, half)) rope_cos_sin(pos, a.inv_freq[lane + 32], &c1, &s1);
+    const int turned = i0 < half ? min(a.pair_count, half) - i0 : 0;  // of this lane's pairs, those before this one
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int src_lane = (i0 + e) & 31;
+      float c = __shfl_sync(full, c0, src_lane), s = __shfl_sync(full, s0, src_lane);
+      if (D == 128) {
+        const float ch = __shfl_sync(full, c1, src_lane), sh = __shfl_sync(full, s1, src_lane);
+        if (i0 + e >= 32) {
+          c = ch;
+          s = sh;
+        }
+      }
+      cos4[e] = e < turned ? c * a.attn_factor : 1.f;
+      sin4[e] = e < turned ? s * a.attn_factor : 0.f;
+    }
+  }
+  const bool any_norm = a.q_norm != nullptr || a.k_norm != nullptr || a.v_norm != 0;
+  for (int h0 = h_begin; h0 < h_end; h0 += kLoads * kPer) {
+    float4 lo[kLoads], hi[kLoads];
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+      const int h = h0 + c * kPer + group;
+      if (h < h_end) {
+        lo[c] = load4(src + h * D + d0);
+        hi[c] = load4(src + h * D + d1);
+      } else {
+        lo[c] = hi[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+      if (h0 + c * kPer >= h_end) break;  // (the same for the whole warp)
+      const int h = h0 + c * kPer + group;
+      float x[4] = {lo[c].x, lo[c].y, lo[c].z, lo[c].w}, y[4] = {hi[c].x, hi[c].y, hi[c].z, hi[c].w};
+      if (any_norm) {  // math.ts:78-97
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ss += x[e] * x[e] + y[e] * y[e];
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(full, ss, o);
+        const float* w = h < Hq ? a.q_norm : h < Hq + Hk ? a.k_norm : nullptr;
+        if (h < Hq + Hk ? w != nullptr : a.v_norm != 0) {
+          const float inv_rms = 1.f / sqrtf(ss / static_cast<float>(D) + a.rms_eps);
+          const float add = a.offset_rms ? 1.f : 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = x[e] * inv_rms * (w == nullptr ? 1.f : add + w[d0 + e]);
+            y[e] = y[e] * inv_rms * (w == nullptr ? 1.f : add + w[d1 + e]);
+          }
+        }
+      }
+      if (h < Hq + Hk) {  // RoPE, math.ts:134-147
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float u = x[e] * cos4[e] - y[e] * sin4[e];
+          y[e] = y[e] * cos4[e] + x[e] * sin4[e];
+          x[e] = u;
+        }
+      }
+      if (h >= h_end) continue;
+      const float4 v0 = make_float4(x[0], x[1], x[2], x[3]), v1 = make_float4(y[0], y[1], y[2], y[3]);
+      if (h < Hq) {
+        if (query_out) {
+          IO* q = query_out + (static_cast<int64_t>(row) * Hq + h) * D;
+          store4(q + d0, v0);
+          store4(q + d1, v1);
+        }
+      } else if (page >= 0) {
+        const bool is_key = h < Hq + Hk;
+        const int kvh = h - Hq - (is_key ? 0 : Hk);
+        CT* at = static_cast<CT*>(is_key ? p.key : p.value) + pool_row(p, page, kvh, slot);
+        store4(at + d0, v0);
+        store4(at + d1, v1);
+        if (is_key && p.bounds && !offsets) {  // one new token: its page's bounds right here
+          CT* low = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D;
+          CT* high = low + D;
+          const float4 k0 = as_stored<CT>(v0), k1 = as_stored<CT>(v1);
+          store4(low + d0, slot == 0 ? k0 : low4(load4(low + d0), k0));
+          store4(low + d1, slot == 0 ? k1 : low4(load4(low + d1), k1));
+          store4(high + d0, slot == 0 ? k0 : high4(load4(high + d0), k0));
+          store4(high + d1, slot == 0 ? k1 : high4(load4(high + d1), k1));
+        }
+      }
+    }
+  }
+}
+
+// Pages that sequence b's chunk goes to (0: none), its rows cut off where the
+// positions or the rows end.
+struct Chunk {
+  int row, start, n;
+};
+__device__ __forceinline__ Chunk chunk_of(const PagedArgs& p, const int32_t* offsets, int rows, int b) {
+  const int start = p.positions[b], row = offsets[b];
+  const long long end = min(static_cast<long long>(offsets[b + 1]), static_cast<long long>(rows));
+  if (start < 0 || start >= p.capacity || row < 0 || end <= row) return {0, 0, 0};
+  return {row, start, static_cast<int>(min(end - row, static_cast<long long>(p.capacity) - start))};
+}
+__device__ __forceinline__ int pages_of(const PagedArgs& p, const Chunk& c) {
+  return c.n == 0 ? 0 : ((c.start + c.n - 1) >> p.page_shift) - (c.start >> p.page_shift) + 1;
+}
+
+// Bounds of the pages that the chunks went to, from the keys as stored, which
+// L2 still holds: a block per touched page and kv head, its threads over 16
+// bytes of a row each and over the rows. Block k finds the k-th touched page
+// by a scan of the sequences' page counts.
+constexpr int kBoundsThreads = 256;
+template <typename CT, int D>
+__global__ void __launch_bounds__(kBoundsThreads)
+    paged_bounds_rows_kernel(PagedArgs p, const int32_t* __restrict__ offsets, int rows) {
+  constexpr int kVec = 16 / sizeof(CT), kLanes = D / kVec, kRows = kBoundsThreads / kLanes;
+  __shared__ int sums[kBoundsThreads / 32];
+  __shared__ int found[2];
+  __shared__ __align__(16) CT low_s[kRows][D], high_s[kRows][D];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, Hk = p.a.Hk;
+  const int want = blockIdx.x / Hk, kvh = blockIdx.x - want * Hk;
+  int before = 0;
+  if (tid == 0) found[0] = -1;
+  for (int base = 0; base < p.batch; base += kBoundsThreads) {
+    const int b = base + tid;
+    const int n = b < p.batch ? pages_of(p, chunk_of(p, offsets, rows, b)) : 0;
+    int scan = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    if (lane == 31) sums[warp] = scan;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < kBoundsThreads / 32; ++w) {
+      if (w < warp) scan += sums[w];
+      all += sums[w];
+    }
+    scan += before;  // pages up to and with sequence b's
+    if (n > 0 && want < scan && want >= scan - n) {
+      found[0] = b;
+      found[1] = want - (scan - n);
+    }
+    before += all;
+    __syncthreads();
+    if (found[0] >= 0) break;
+  }
+  const int b = found[0];
+  if (b < 0) return;
+  const Chunk c = chunk_of(p, offsets, rows, b);
+  const int index = (c.start >> p.page_shift) + found[1], size = 1 << p.page_shift;
+  const int page = p.table[static_cast<int64_t>(b) * p.width + index];
+  if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.page_count)) return;  // reported by the append
+  const int begin = max(0, c.start - index * size), end = min(size, c.start + c.n - index * size);  // the page's new slots
+  const int d = (tid % kLanes) * kVec, r = tid / kLanes;
+  const CT* key = static_cast<const CT*>(p.key) + pool_row(p, page, kvh, 0) + d;
+  CT low[kVec], high[kVec];
+  bool any = false;
+  for (int s = begin + r; s < end; s += kRows) {
+    const uint4 u = *reinterpret_cast<const uint4*>(key + s * p.slot_stride);
+    const CT* v = reinterpret_cast<const CT*>(&u);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      low[e] = any ? low_of(low[e], v[e]) : v[e];
+      high[e] = any ? high_of(high[e], v[e]) : v[e];
+    }
+    any = true;
+  }
+  if (any)
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      low_s[r][d + e] = low[e];
+      high_s[r][d + e] = high[e];
+    }
+  __syncthreads();
+  const int held = min(kRows, end - begin);  // rows of the table that were filled
+  for (int i = tid; i < 2 * D; i += kBoundsThreads) {
+    const bool is_low = i < D;
+    const int e = is_low ? i : i - D;
+    CT* at = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D + i;
+    CT v = is_low ? low_s[0][e] : high_s[0][e];
+    for (int k = 1; k < held; ++k) v = is_low ? low_of(v, low_s[k][e]) : high_of(v, high_s[k][e]);
+    if (begin > 0) v = is_low ? low_of(at[0], v) : high_of(at[0], v);
+    at[0] = v;
+  }
+}
+
+// Bounds of the pages that a chunk touched, any shape: the block of a page's
+// first new row walks the page's new slots.
 template <typename CT>
 __global__ void __launch_bounds__(kThreads)
     paged_bounds_kernel(PagedArgs p, const int32_t* __restrict__ offsets, int rows) {
@@ -159,30 +429,56 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+template <typename CT>
+cudaError_t bounds_t(const PagedArgs& p, bool rows_ok, const int32_t* offsets, int rows, cudaStream_t stream) {
+  if (!rows_ok) return launch_pdl(paged_bounds_kernel<CT>, rows, kThreads, 0, stream, p, offsets, rows);
+  // a chunk of n rows touches at most (n - 1) / page_size + 2 pages, and no more than its rows
+  const long long pages = min(static_cast<long long>(rows), (static_cast<long long>(rows) >> p.page_shift) + 2LL * p.batch);
+  auto k = p.a.D == 64 ? paged_bounds_rows_kernel<CT, 64> : paged_bounds_rows_kernel<CT, 128>;
+  return launch_pdl(k, static_cast<unsigned>(pages * p.a.Hk), kBoundsThreads, 0, stream, p, offsets, rows);
+}
+
 template <typename IO, typename CT>
-cudaError_t append_t(const PagedArgs& p, const void* qkv, const int32_t* offsets, int rows, void* query_out,
-                     cudaStream_t stream) {
-  const size_t smem = sizeof(float) * (static_cast<size_t>(p.a.Hq + 2 * p.a.Hk) * p.a.D + p.a.rotary);
-  auto k = paged_append_kernel<IO, CT>;
-  if (smem > 48 * 1024) {
-    cudaError_t e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
+cudaError_t append_t(const tla_paged* P, const PagedArgs& p, const void* qkv, const int32_t* offsets, int rows,
+                     void* query_out, cudaStream_t stream) {
+  const int D = p.a.D, heads = p.a.Hq + 2 * p.a.Hk;
+  const bool rows_ok = P->wide && p.a.rotary % 8 == 0;
+  cudaError_t e;
+  if (rows_ok) {
+    // Warps per row: enough for 16 on every SM, at most one per warp-wide load
+    // (64 rows of 48 heads: 12 warps per row).
+    const int per = 256 / D, most = (heads + per - 1) / per;
+    long long parts = (16LL * P->base.ctx->sm_count + rows - 1) / rows;
+    parts = parts < 1 ? 1 : parts > most ? most : parts;
+    const int part_heads = (most + static_cast<int>(parts) - 1) / static_cast<int>(parts) * per;
+    parts = (heads + part_heads - 1) / part_heads;
+    const unsigned blocks = static_cast<unsigned>((rows * parts + 3) / 4);
+    auto k = D == 64 ? paged_append_rows_kernel<IO, CT, 64> : paged_append_rows_kernel<IO, CT, 128>;
+    e = launch_pdl(k, blocks, kThreads, 0, stream, p, static_cast<const IO*>(qkv), offsets, rows,
+                   static_cast<IO*>(query_out), static_cast<int>(parts), part_heads);
+  } else {
+    const size_t smem = sizeof(float) * (static_cast<size_t>(heads) * D + p.a.rotary);
+    auto k = paged_append_kernel<IO, CT>;
+    if (smem > 48 * 1024) {
+      e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem));
+      if (e != cudaSuccess) return e;
+    }
+    e = launch_pdl(k, rows, kThreads, smem, stream, p, static_cast<const IO*>(qkv), offsets, rows,
+                   static_cast<IO*>(query_out));
   }
-  cudaError_t e = launch_pdl(k, rows, kThreads, smem, stream, p, static_cast<const IO*>(qkv), offsets, rows,
-                             static_cast<IO*>(query_out));
   if (e != cudaSuccess || !p.bounds || !offsets) return e;
-  return launch_pdl(paged_bounds_kernel<CT>, rows, kThreads, 0, stream, p, offsets, rows);
+  return bounds_t<CT>(p, P->wide, offsets, rows, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_paged_append(const tla_paged* P, const PagedArgs& p, const void* qkv, const int32_t* offsets,
                                 int rows, void* query_out, cudaStream_t stream) {
-  if (P->io == kFp16) return append_t<__half, __half>(p, qkv, offsets, rows, query_out, stream);
-  if (P->io == kBf16) return append_t<__nv_bfloat16, __nv_bfloat16>(p, qkv, offsets, rows, query_out, stream);
-  if (P->kept == kFp16) return append_t<float, __half>(p, qkv, offsets, rows, query_out, stream);
-  if (P->kept == kBf16) return append_t<float, __nv_bfloat16>(p, qkv, offsets, rows, query_out, stream);
-  return append_t<float, float>(p, qkv, offsets, rows, query_out, stream);
+  if (P->io == kFp16) return append_t<__half, __half>(P, p, qkv, offsets, rows, query_out, stream);
+  if (P->io == kBf16) return append_t<__nv_bfloat16, __nv_bfloat16>(P, p, qkv, offsets, rows, query_out, stream);
+  if (P->kept == kFp16) return append_t<float, __half>(P, p, qkv, offsets, rows, query_out, stream);
+  if (P->kept == kBf16) return append_t<float, __nv_bfloat16>(P, p, qkv, offsets, rows, query_out, stream);
+  return append_t<float, float>(P, p, qkv, offsets, rows, query_out, stream);
 }
 
 }  // namespace tla

@@ -697,15 +697,13 @@ cudaError_t launch_t(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   using IO = typename std::conditional<SPLIT, float, CT>::type;
   auto kernel = paged_decode_kernel<D, CT, SPLIT, TWO>;
   const void* k = reinterpret_cast<const void*>(kernel);
-  // (batches rounded up: few different sizes to ask the occupancy of)
-  const int smem = smem_layout<D>(d.rows, (d.p.batch + 63) & ~63, SPLIT).total;
+  const int smem = smem_layout<D>(d.rows, d.p.batch, SPLIT).total;
   cudaError_t e = raise_smem_limit(k, smem);
   if (e != cudaSuccess) return e;
-  int blocks = 0;
-  e = cached_occupancy(k, kThreads, smem, &blocks);
-  if (e != cudaSuccess) return e;
-  if (blocks < 1) return cudaErrorInvalidConfiguration;
-  const int grid = (blocks < kCtasPerSm ? blocks : kCtasPerSm) * P->base.ctx->sm_count;
+  // two CTAs per SM by registers (the launch bounds), if shared memory holds
+  // two (228 KB, 1 KB of it reserved per CTA)
+  const int per_sm = kCtasPerSm * (smem + 1024) <= 228 * 1024 ? kCtasPerSm : 1;
+  const int grid = per_sm * P->base.ctx->sm_count;
   d.small_grid = P->base.ctx->sm_count;
   e = launch_pdl(kernel, grid, kThreads, smem, stream, d);
   if (e != cudaSuccess) return e;
@@ -757,15 +755,12 @@ int subgroup_rows(const tla_paged* P) {
 void paged_decode_configure(tla_paged* P) {
   const tla_page_pool& pool = P->pool;
   P->fast = false;
-  if (P->kept == kFp32 || (P->io == kFp32 && P->kept != kFp16) || (P->base.D != 64 && P->base.D != 128) ||
-      pool.page_size < 16 || P->base.ctx->encode_tiled == nullptr ||
+  if (!P->wide || P->kept == kFp32 || (P->io == kFp32 && P->kept != kFp16) || pool.page_size < 16 || P->base.ctx->encode_tiled == nullptr ||
       kCtasPerSm * P->base.ctx->sm_count > kMaxGrid)
     return;
-  // a dimension of one entry may carry any stride
   tla_paged q = *P;
   if (pool.page_count == 1) q.pool.page_stride = P->base.D;
   if (P->base.Hk == 1) q.pool.head_stride = P->base.D;
-  if (q.pool.page_stride % 8 || q.pool.head_stride % 8 || q.pool.slot_stride % 8) return;
   P->fast = make_pool_map(&q, pool.key, &P->tmap_k) && make_pool_map(&q, pool.value, &P->tmap_v);
 }
 

@@ -19,10 +19,18 @@ import torch
 
 from . import _abi
 from ._abi import check, lib
-from .attention import Context, _ptr, attn_config
+from .attention import Context, attn_config
 
 _IO_FLAGS = {torch.float16: 0, torch.bfloat16: _abi.FLAG_IO_BF16, torch.float32: _abi.FLAG_IO_FP32}
 _PAGE_FLAGS = {torch.float16: 0, torch.bfloat16: _abi.FLAG_CACHE_BF16, torch.float32: _abi.FLAG_CACHE_FP32}
+
+
+def _current_raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same handle without a Stream object around it, where this PyTorch offers it
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_raw_stream)
 
 
 class PagedAttention:
@@ -84,8 +92,10 @@ class PagedAttention:
             if tuple(key_bounds.shape) != (k.shape[0], self.kvHeadCount, 2, self.headDim):
                 raise ValueError("key_bounds must be [pages, kvHeadCount, 2, headDim]")
         self.keyPages, self.valuePages, self.keyBounds = k, v, key_bounds
-        self.context = context or Context.default(self.device.index or 0)
-        if self.context.device != (self.device.index or 0):
+        self._index = self.device.index
+        self._lib = lib()
+        self.context = context or Context.default(self._index)
+        if self.context.device != self._index:
             raise ValueError("the context and the pages are on different devices")
         cfg = attn_config(o, self.headCount, self.kvHeadCount, self.headDim, max_tokens, self.maxBatch)
         cfg.flags |= _IO_FLAGS[self.dtype] | _PAGE_FLAGS[k.dtype]
@@ -102,23 +112,23 @@ class PagedAttention:
             norms.append(w)
         self.qNormAttribute, self.kNormAttribute = norms
         h = ctypes.c_void_p()
-        check(lib().tla_paged_create(self.context.handle, ctypes.byref(cfg), ctypes.byref(pool),
+        check(self._lib.tla_paged_create(self.context.handle, ctypes.byref(cfg), ctypes.byref(pool),
                                      *(None if w is None else w.ctypes.data_as(ctypes.c_void_p) for w in norms),
                                      ctypes.byref(h)), "PagedAttention constructor")
         self.handle = h
         self._workspace_bytes = {}
 
-    # ---- argument checks
+    # ---- argument checks (a step makes several calls per layer: each check is a few attribute reads)
     def _rows(self, t, name, rows, width):
-        if t.dtype != self.dtype or t.device != self.device or not t.is_contiguous():
+        if t.dtype is not self.dtype or t.get_device() != self._index or not t.is_contiguous():
             raise TypeError(f"{name} must be a contiguous {self.dtype} tensor on {self.device}")
         if t.numel() != rows * width:
             raise ValueError(f"{name} must hold {rows} rows of {width} values, not shape {tuple(t.shape)}")
 
     def _ints(self, t, name, shape):
-        if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.get_device() != self._index or not t.is_contiguous():
             raise TypeError(f"{name} must be a contiguous int32 tensor on {self.device}")
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
 
     def _sequences(self, positions, page_table):
@@ -131,15 +141,16 @@ class PagedAttention:
         return batch, width
 
     def _on(self, stream):
-        """The stream of a call, and the context that makes tensors on it."""
+        """The raw stream of a call: the current one of the pages' device, or the given one."""
         if stream is None:
-            return torch.cuda.current_stream(self.device)
+            return _current_raw_stream(self._index)
         if stream.device != self.device:
             raise ValueError("the stream and the pages are on different devices")
-        return stream
+        return stream.cuda_stream
 
     def _new(self, shape, dtype, stream):
-        if stream == torch.cuda.current_stream(self.device):
+        """A tensor that belongs to the call's stream."""
+        if stream is None:
             return torch.empty(shape, dtype=dtype, device=self.device)
         with torch.cuda.stream(stream):
             return torch.empty(shape, dtype=dtype, device=self.device)
@@ -148,9 +159,9 @@ class PagedAttention:
         n = self._workspace_bytes.get((batch, width))
         if n is None:
             size = ctypes.c_size_t()
-            check(lib().tla_paged_workspace(self.handle, batch, width, ctypes.byref(size)), "workspace")
+            check(self._lib.tla_paged_workspace(self.handle, batch, width, ctypes.byref(size)), "workspace")
             n = self._workspace_bytes[batch, width] = size.value
-        return self._new((n,), torch.uint8, stream)
+        return self._new(n, torch.uint8, stream), n
 
     # ---- the operators
     def append(self, qkv, positions, page_table, row_offsets=None, query=None, stream=None):
@@ -159,67 +170,75 @@ class PagedAttention:
         qkv [rows, (headCount + 2*kvHeadCount) * headDim]. Without row_offsets, row b is
         sequence b's new token at positions[b]. With it (int32 [batch + 1]), rows
         row_offsets[b] .. row_offsets[b+1]-1 are sequence b's tokens from positions[b] on."""
-        s = self._on(stream)
+        on = self._on(stream)
         batch, width = self._sequences(positions, page_table)
         rows = qkv.shape[0]
         self._rows(qkv, "qkv", rows, self.rowSize)
-        if row_offsets is None:
-            if rows != batch:
-                raise ValueError(f"{rows} rows for {batch} sequences need row_offsets")
-        else:
+        offsets = None
+        if row_offsets is not None:
             self._ints(row_offsets, "row_offsets", (batch + 1,))
+            offsets = row_offsets.data_ptr()
+        elif rows != batch:
+            raise ValueError(f"{rows} rows for {batch} sequences need row_offsets")
         if query is None:
-            query = self._new((rows, self.qSize), self.dtype, s)
+            query = self._new((rows, self.qSize), self.dtype, stream)
         else:
             self._rows(query, "query", rows, self.qSize)
-        check(lib().tla_paged_append(self.handle, _ptr(qkv), _ptr(positions), _ptr(row_offsets), _ptr(page_table),
-                                     width, batch, rows, _ptr(query), ctypes.c_void_p(s.cuda_stream)), "append")
+        rc = self._lib.tla_paged_append(self.handle, qkv.data_ptr(), positions.data_ptr(), offsets,
+                                        page_table.data_ptr(), width, batch, rows, query.data_ptr(), on)
+        if rc:
+            check(rc, "append")
         return query
 
     def decode(self, query, positions, page_table, pages=None, gate=None, out=None, stream=None):
         """Attention of one new token per sequence: query [batch, headCount * headDim] as append
         returned it; pages None, or int32 [batch, kvHeadCount, count] as select returned them."""
-        s = self._on(stream)
+        on = self._on(stream)
         batch, width = self._sequences(positions, page_table)
         self._rows(query, "query", batch, self.qSize)
-        count = 0
+        listed, count = None, 0
         if pages is not None:
             count = pages.shape[-1]
             if count == 0:  # (an empty tensor's null address would read as no list)
                 raise _abi.TlaError(-1, "decode: pages lists nothing")
             self._ints(pages, "pages", (batch, self.kvHeadCount, count))
+            listed = pages.data_ptr()
         if gate is not None:
             self._rows(gate, "gate", batch, self.qSize)
+            gate = gate.data_ptr()
         if out is None:
-            out = self._new((batch, self.qSize), self.dtype, s)
+            out = self._new((batch, self.qSize), self.dtype, stream)
         else:
             self._rows(out, "out", batch, self.qSize)
-        work = self._workspace(batch, width, s)
-        check(lib().tla_paged_decode(self.handle, _ptr(query), _ptr(positions), _ptr(page_table), width, _ptr(pages),
-                                     count, _ptr(gate), _ptr(out), batch, _ptr(work), work.numel(),
-                                     ctypes.c_void_p(s.cuda_stream)), "decode")
+        work, size = self._workspace(batch, width, stream)
+        rc = self._lib.tla_paged_decode(self.handle, query.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
+                                        width, listed, count, gate, out.data_ptr(), batch, work.data_ptr(), size, on)
+        if rc:
+            check(rc, "decode")
         return out
 
     def select(self, query, positions, page_table, count, first=1, last=1, pages=None, stream=None):
         """The `count` pages per sequence and kv head that decode should read: the first `first`,
         the last `last` and the best scored of the others; int32 [batch, kvHeadCount, count]."""
-        s = self._on(stream)
+        on = self._on(stream)
         batch, width = self._sequences(positions, page_table)
         self._rows(query, "query", batch, self.qSize)
         count = int(count)
         if pages is None:
-            pages = self._new((batch, self.kvHeadCount, max(count, 0)), torch.int32, s)
+            pages = self._new((batch, self.kvHeadCount, max(count, 0)), torch.int32, stream)
         else:
             self._ints(pages, "pages", (batch, self.kvHeadCount, count))
-        work = self._workspace(batch, width, s)
-        check(lib().tla_paged_select(self.handle, _ptr(query), _ptr(positions), _ptr(page_table), width, int(first),
-                                     int(last), _ptr(pages), count, batch, _ptr(work), work.numel(),
-                                     ctypes.c_void_p(s.cuda_stream)), "select")
+        work, size = self._workspace(batch, width, stream)
+        rc = self._lib.tla_paged_select(self.handle, query.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
+                                        width, int(first), int(last), pages.data_ptr(), count, batch, work.data_ptr(),
+                                        size, on)
+        if rc:
+            check(rc, "select")
         return pages
 
     def close(self):
         if self.handle:
-            lib().tla_paged_destroy(self.handle)
+            self._lib.tla_paged_destroy(self.handle)
             self.handle = None
 
     def __del__(self):
