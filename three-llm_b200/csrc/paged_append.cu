@@ -9,6 +9,8 @@
 // K and V to their slots, K as stored into its page's bounds.
 #include <math.h>
 
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace tla {
@@ -31,6 +33,23 @@ __device__ __forceinline__ int sequence_of(const int32_t* offsets, int batch, in
       hi = mid;
   }
   return lo;
+}
+
+// The same by a whole warp, 32 offsets at a time: two rounds of loads for up to
+// 1024 sequences where the search above takes ten.
+__device__ __forceinline__ int sequence_of_warp(const int32_t* offsets, int batch, int row, int lane) {
+  if (!offsets) return row;
+  int lo = 0, n = batch + 1;  // the answer is the last of [lo, lo + n) that is <= row
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = lo + lane * step;
+    const unsigned low = __ballot_sync(0xffffffffu, at < lo + n && offsets[min(at, batch)] <= row);
+    if (low == 0) return -1;  // (only possible in the first round: row lies before offsets[0])
+    const int last = 31 - __clz(low);
+    n = min(step, lo + n - (lo + last * step));
+    lo += last * step;
+  }
+  // (offsets out of order may lead anywhere: what counts is that the row lies in the sequence found)
+  return lo < batch && offsets[lo] <= row && row < offsets[lo + 1] ? lo : -1;
 }
 
 template <typename CT>
@@ -185,7 +204,7 @@ __global__ void __launch_bounds__(kThreads)
   if (row >= rows) return;
   const int h_begin = part * part_heads, h_end = min(heads, h_begin + part_heads);
   const IO* src = qkv + static_cast<int64_t>(row) * heads * D;
-  const int b = sequence_of(offsets, p.batch, row);
+  const int b = sequence_of_warp(offsets, p.batch, row, lane);
   if (b < 0) return;
   const int start = p.positions[b];
   const int pos = start < 0 || !offsets ? start
@@ -224,75 +243,117 @@ __global__ void __launch_bounds__(kThreads)
       sin4[e] = e < turned ? s * a.attn_factor : 0.f;
     }
   }
-  const bool any_norm = a.q_norm != nullptr || a.k_norm != nullptr || a.v_norm != 0;
-  for (int h0 = h_begin; h0 < h_end; h0 += kLoads * kPer) {
-    float4 lo[kLoads], hi[kLoads];
+  // Heads [from, to) of one kind: 0 queries, 1 keys, 2 values.
+  auto heads_of = [&](auto kind, int from, int to, const float* w, bool norm) {
+    constexpr int kKind = decltype(kind)::value;
+    if (from >= to) return;
+    if (kKind == 0 ? query_out == nullptr : page < 0) return;
+    float wx[4], wy[4];  // the norm's weights of this lane's elements
+    if (norm) {
+      const float add = a.offset_rms ? 1.f : 0.f;
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c) {
-      const int h = h0 + c * kPer + group;
-      if (h < h_end) {
-        lo[c] = load4(src + h * D + d0);
-        hi[c] = load4(src + h * D + d1);
-      } else {
-        lo[c] = hi[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int e = 0; e < 4; ++e) {
+        wx[e] = w == nullptr ? 1.f : add + w[d0 + e];
+        wy[e] = w == nullptr ? 1.f : add + w[d1 + e];
       }
     }
+    const IO* in = src + (from + group) * D;
+    for (int h0 = from; h0 < to; h0 += kLoads * kPer, in += kLoads * kPer * D) {
+      float4 lo[kLoads], hi[kLoads];
 #pragma unroll
-    for (int c = 0; c < kLoads; ++c) {
-      if (h0 + c * kPer >= h_end) break;  // (the same for the whole warp)
-      const int h = h0 + c * kPer + group;
-      float x[4] = {lo[c].x, lo[c].y, lo[c].z, lo[c].w}, y[4] = {hi[c].x, hi[c].y, hi[c].z, hi[c].w};
-      if (any_norm) {  // math.ts:78-97
-        float ss = 0.f;
+      for (int c = 0; c < kLoads; ++c) {
+        lo[c] = hi[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (h0 + c * kPer + group < to) {
+          lo[c] = load4(in + c * kPer * D + d0);
+          hi[c] = load4(in + c * kPer * D + d1);
+        }
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ss += x[e] * x[e] + y[e] * y[e];
+      for (int c = 0; c < kLoads; ++c) {
+        if (h0 + c * kPer >= to) break;  // (the same for the whole warp)
+        const int h = h0 + c * kPer + group;
+        float x[4] = {lo[c].x, lo[c].y, lo[c].z, lo[c].w}, y[4] = {hi[c].x, hi[c].y, hi[c].z, hi[c].w};
+        if (norm) {  // math.ts:78-97
+          float ss = 0.f;
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(full, ss, o);
-        const float* w = h < Hq ? a.q_norm : h < Hq + Hk ? a.k_norm : nullptr;
-        if (h < Hq + Hk ? w != nullptr : a.v_norm != 0) {
-          const float inv_rms = 1.f / sqrtf(ss / static_cast<float>(D) + a.rms_eps);
-          const float add = a.offset_rms ? 1.f : 0.f;
+          for (int e = 0; e < 4; ++e) ss += x[e] * x[e] + y[e] * y[e];
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(full, ss, o);
+          const float inv_rms = rsqrtf(ss * (1.f / D) + a.rms_eps);  // (2 ulp)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[e] = x[e] * inv_rms * (w == nullptr ? 1.f : add + w[d0 + e]);
-            y[e] = y[e] * inv_rms * (w == nullptr ? 1.f : add + w[d1 + e]);
+            x[e] *= inv_rms * wx[e];
+            y[e] *= inv_rms * wy[e];
           }
         }
-      }
-      if (h < Hq + Hk) {  // RoPE, math.ts:134-147
+        if (kKind < 2) {  // RoPE, math.ts:134-147
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float u = x[e] * cos4[e] - y[e] * sin4[e];
-          y[e] = y[e] * cos4[e] + x[e] * sin4[e];
-          x[e] = u;
+          for (int e = 0; e < 4; ++e) {
+            const float u = x[e] * cos4[e] - y[e] * sin4[e];
+            y[e] = y[e] * cos4[e] + x[e] * sin4[e];
+            x[e] = u;
+          }
         }
-      }
-      if (h >= h_end) continue;
-      const float4 v0 = make_float4(x[0], x[1], x[2], x[3]), v1 = make_float4(y[0], y[1], y[2], y[3]);
-      if (h < Hq) {
-        if (query_out) {
+        if (h >= to) continue;
+        const float4 v0 = make_float4(x[0], x[1], x[2], x[3]), v1 = make_float4(y[0], y[1], y[2], y[3]);
+        if (kKind == 0) {
           IO* q = query_out + (static_cast<int64_t>(row) * Hq + h) * D;
           store4(q + d0, v0);
           store4(q + d1, v1);
-        }
-      } else if (page >= 0) {
-        const bool is_key = h < Hq + Hk;
-        const int kvh = h - Hq - (is_key ? 0 : Hk);
-        CT* at = static_cast<CT*>(is_key ? p.key : p.value) + pool_row(p, page, kvh, slot);
-        store4(at + d0, v0);
-        store4(at + d1, v1);
-        if (is_key && p.bounds && !offsets) {  // one new token: its page's bounds right here
-          CT* low = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D;
-          CT* high = low + D;
-          const float4 k0 = as_stored<CT>(v0), k1 = as_stored<CT>(v1);
-          store4(low + d0, slot == 0 ? k0 : low4(load4(low + d0), k0));
-          store4(low + d1, slot == 0 ? k1 : low4(load4(low + d1), k1));
-          store4(high + d0, slot == 0 ? k0 : high4(load4(high + d0), k0));
-          store4(high + d1, slot == 0 ? k1 : high4(load4(high + d1), k1));
+        } else {
+          const int kvh = h - Hq - (kKind == 1 ? 0 : Hk);
+          CT* at = static_cast<CT*>(kKind == 1 ? p.key : p.value) + pool_row(p, page, kvh, slot);
+          store4(at + d0, v0);
+          store4(at + d1, v1);
+          if (kKind == 1 && p.bounds && !offsets) {  // one new token: its page's bounds right here
+            CT* low = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D;
+            CT* high = low + D;
+            const float4 k0 = as_stored<CT>(v0), k1 = as_stored<CT>(v1);
+            store4(low + d0, slot == 0 ? k0 : low4(load4(low + d0), k0));
+            store4(low + d1, slot == 0 ? k1 : low4(load4(low + d1), k1));
+            store4(high + d0, slot == 0 ? k0 : high4(load4(high + d0), k0));
+            store4(high + d1, slot == 0 ? k1 : high4(load4(high + d1), k1));
+          }
         }
       }
     }
-  }
+  };
+  heads_of(std::integral_constant<int, 0>(), h_begin, min(h_end, Hq), a.q_norm, a.q_norm != nullptr);
+  heads_of(std::integral_constant<int, 1>(), max(h_begin, Hq), min(h_end, Hq + Hk), a.k_norm, a.k_norm != nullptr);
+  heads_of(std::integral_constant<int, 2>(), max(h_begin, Hq + Hk), h_end, nullptr, a.v_norm != 0);
+}
+
+// Smaller and larger elements of 16 bytes.
+__device__ __forceinline__ uint32_t low_pair(uint32_t a, uint32_t b, __half) {
+  const __half2 v = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t high_pair(uint32_t a, uint32_t b, __half) {
+  const __half2 v = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t low_pair(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t high_pair(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t low_pair(uint32_t a, uint32_t b, float) {
+  return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b)));
+}
+__device__ __forceinline__ uint32_t high_pair(uint32_t a, uint32_t b, float) {
+  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+}
+template <typename CT>
+__device__ __forceinline__ uint4 low_vec(uint4 a, uint4 b) {
+  return make_uint4(low_pair(a.x, b.x, CT()), low_pair(a.y, b.y, CT()), low_pair(a.z, b.z, CT()), low_pair(a.w, b.w, CT()));
+}
+template <typename CT>
+__device__ __forceinline__ uint4 high_vec(uint4 a, uint4 b) {
+  return make_uint4(high_pair(a.x, b.x, CT()), high_pair(a.y, b.y, CT()), high_pair(a.z, b.z, CT()),
+                    high_pair(a.w, b.w, CT()));
 }
 
 // Pages that sequence b's chunk goes to (0: none), its rows cut off where the
@@ -362,24 +423,17 @@ __global__ void __launch_bounds__(kBoundsThreads)
   const int begin = max(0, c.start - index * size), end = min(size, c.start + c.n - index * size);  // the page's new slots
   const int d = (tid % kLanes) * kVec, r = tid / kLanes;
   const CT* key = static_cast<const CT*>(p.key) + pool_row(p, page, kvh, 0) + d;
-  CT low[kVec], high[kVec];
-  bool any = false;
-  for (int s = begin + r; s < end; s += kRows) {
-    const uint4 u = *reinterpret_cast<const uint4*>(key + s * p.slot_stride);
-    const CT* v = reinterpret_cast<const CT*>(&u);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      low[e] = any ? low_of(low[e], v[e]) : v[e];
-      high[e] = any ? high_of(high[e], v[e]) : v[e];
+  if (begin + r < end) {
+    uint4 low = *reinterpret_cast<const uint4*>(key + (begin + r) * p.slot_stride), high = low;
+#pragma unroll 4
+    for (int s = begin + r + kRows; s < end; s += kRows) {
+      const uint4 u = *reinterpret_cast<const uint4*>(key + s * p.slot_stride);
+      low = low_vec<CT>(low, u);
+      high = high_vec<CT>(high, u);
     }
-    any = true;
+    *reinterpret_cast<uint4*>(&low_s[r][d]) = low;
+    *reinterpret_cast<uint4*>(&high_s[r][d]) = high;
   }
-  if (any)
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) {
-      low_s[r][d + e] = low[e];
-      high_s[r][d + e] = high[e];
-    }
   __syncthreads();
   const int held = min(kRows, end - begin);  // rows of the table that were filled
   for (int i = tid; i < 2 * D; i += kBoundsThreads) {
