@@ -142,18 +142,34 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// Four neighbouring elements.
-__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 load4(const __half* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
+// Four neighbouring elements, as loaded and as floats.
+template <typename T>
+struct Raw4 {
+  uint2 u;
+};
+template <>
+struct Raw4<float> {
+  float4 u;
+};
+template <typename T>
+__device__ __forceinline__ Raw4<T> raw4(const T* p) {
+  return *reinterpret_cast<const Raw4<T>*>(p);
+}
+__device__ __forceinline__ float4 floats(const Raw4<float>& r) { return r.u; }
+__device__ __forceinline__ float4 floats(const Raw4<__half>& r) {
+  const uint2 u = r.u;
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
   const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
   return make_float4(a.x, a.y, b.x, b.y);
 }
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
+__device__ __forceinline__ float4 floats(const Raw4<__nv_bfloat16>& r) {
+  const uint2 u = r.u;
   return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
                      __uint_as_float(u.y & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  return floats(raw4(p));
 }
 __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ void store4(__half* p, float4 v) {
@@ -185,7 +201,7 @@ __device__ __forceinline__ float4 high4(float4 a, float4 b) {
 // two per lane, and hands them out by shuffles. Rows of a long prompt are
 // bound by memory (about 60 instructions per lane and 16 bytes read).
 template <typename IO, typename CT, int D>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 5)
     paged_append_rows_kernel(PagedArgs p, const IO* __restrict__ qkv, const int32_t* __restrict__ offsets, int rows,
                              IO* __restrict__ query_out, int parts, int part_heads) {
   constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes per head, heads per warp-wide load
@@ -248,67 +264,71 @@ __global__ void __launch_bounds__(kThreads)
     constexpr int kKind = decltype(kind)::value;
     if (from >= to) return;
     if (kKind == 0 ? query_out == nullptr : page < 0) return;
-    float wx[4], wy[4];  // the norm's weights of this lane's elements
-    if (norm) {
-      const float add = a.offset_rms ? 1.f : 0.f;
+    // The norm's weights folded into the rotation: (x, y) of a pair becomes
+    // r (x xc - y ys, y yc + x xs), r = 1 / rms.
+    float xc[4], xs[4], yc[4], ys[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        wx[e] = w == nullptr ? 1.f : add + w[d0 + e];
-        wy[e] = w == nullptr ? 1.f : add + w[d1 + e];
-      }
+    for (int e = 0; e < 4; ++e) {
+      const float add = a.offset_rms ? 1.f : 0.f;
+      const float wx = w == nullptr ? 1.f : add + w[d0 + e], wy = w == nullptr ? 1.f : add + w[d1 + e];
+      xc[e] = kKind == 2 ? 1.f : wx * cos4[e];
+      xs[e] = kKind == 2 ? 0.f : wx * sin4[e];
+      yc[e] = kKind == 2 ? 1.f : wy * cos4[e];
+      ys[e] = kKind == 2 ? 0.f : wy * sin4[e];
     }
     const IO* in = src + (from + group) * D;
-    for (int h0 = from; h0 < to; h0 += kLoads * kPer, in += kLoads * kPer * D) {
-      float4 lo[kLoads], hi[kLoads];
+    IO* q = kKind == 0 ? query_out + (static_cast<int64_t>(row) * Hq + from + group) * D : nullptr;
+    CT* kv = kKind == 0 ? nullptr : static_cast<CT*>(kKind == 1 ? p.key : p.value) + pool_row(p, page, 0, slot);
+    for (int h0 = from + group; h0 - group < to; h0 += kLoads * kPer, in += kLoads * kPer * D, q += kLoads * kPer * D) {
+      Raw4<IO> lo[kLoads], hi[kLoads];
 #pragma unroll
       for (int c = 0; c < kLoads; ++c) {
-        lo[c] = hi[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (h0 + c * kPer + group < to) {
-          lo[c] = load4(in + c * kPer * D + d0);
-          hi[c] = load4(in + c * kPer * D + d1);
+        const bool on = h0 + c * kPer < to;
+        lo[c] = on ? raw4(in + c * kPer * D + d0) : Raw4<IO>{};
+        hi[c] = on ? raw4(in + c * kPer * D + d1) : Raw4<IO>{};
+      }
+      float r[kLoads];
+      if (norm) {  // math.ts:78-97; the loads' sums go through the shuffles side by side
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) {
+          const float4 x = floats(lo[c]), y = floats(hi[c]);
+          r[c] = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
         }
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+          for (int c = 0; c < kLoads; ++c) r[c] += __shfl_xor_sync(full, r[c], o);
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) r[c] = rsqrtf(r[c] * (1.f / D) + a.rms_eps);  // (2 ulp)
       }
 #pragma unroll
       for (int c = 0; c < kLoads; ++c) {
-        if (h0 + c * kPer >= to) break;  // (the same for the whole warp)
-        const int h = h0 + c * kPer + group;
-        float x[4] = {lo[c].x, lo[c].y, lo[c].z, lo[c].w}, y[4] = {hi[c].x, hi[c].y, hi[c].z, hi[c].w};
-        if (norm) {  // math.ts:78-97
-          float ss = 0.f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) ss += x[e] * x[e] + y[e] * y[e];
-#pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(full, ss, o);
-          const float inv_rms = rsqrtf(ss * (1.f / D) + a.rms_eps);  // (2 ulp)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] *= inv_rms * wx[e];
-            y[e] *= inv_rms * wy[e];
-          }
+        float4 x = floats(lo[c]), y = floats(hi[c]);
+        if (norm) {
+          x = make_float4(x.x * r[c], x.y * r[c], x.z * r[c], x.w * r[c]);
+          y = make_float4(y.x * r[c], y.y * r[c], y.z * r[c], y.w * r[c]);
         }
         if (kKind < 2) {  // RoPE, math.ts:134-147
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float u = x[e] * cos4[e] - y[e] * sin4[e];
-            y[e] = y[e] * cos4[e] + x[e] * sin4[e];
-            x[e] = u;
-          }
+          const float4 u = x;
+          x = make_float4(u.x * xc[0] - y.x * ys[0], u.y * xc[1] - y.y * ys[1], u.z * xc[2] - y.z * ys[2],
+                          u.w * xc[3] - y.w * ys[3]);
+          y = make_float4(y.x * yc[0] + u.x * xs[0], y.y * yc[1] + u.y * xs[1], y.z * yc[2] + u.z * xs[2],
+                          y.w * yc[3] + u.w * xs[3]);
         }
+        const int h = h0 + c * kPer;
         if (h >= to) continue;
-        const float4 v0 = make_float4(x[0], x[1], x[2], x[3]), v1 = make_float4(y[0], y[1], y[2], y[3]);
         if (kKind == 0) {
-          IO* q = query_out + (static_cast<int64_t>(row) * Hq + h) * D;
-          store4(q + d0, v0);
-          store4(q + d1, v1);
+          store4(q + c * kPer * D + d0, x);
+          store4(q + c * kPer * D + d1, y);
         } else {
           const int kvh = h - Hq - (kKind == 1 ? 0 : Hk);
-          CT* at = static_cast<CT*>(kKind == 1 ? p.key : p.value) + pool_row(p, page, kvh, slot);
-          store4(at + d0, v0);
-          store4(at + d1, v1);
+          CT* at = kv + kvh * p.head_stride;
+          store4(at + d0, x);
+          store4(at + d1, y);
           if (kKind == 1 && p.bounds && !offsets) {  // one new token: its page's bounds right here
             CT* low = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D;
             CT* high = low + D;
-            const float4 k0 = as_stored<CT>(v0), k1 = as_stored<CT>(v1);
+            const float4 k0 = as_stored<CT>(x), k1 = as_stored<CT>(y);
             store4(low + d0, slot == 0 ? k0 : low4(load4(low + d0), k0));
             store4(low + d1, slot == 0 ? k1 : low4(load4(low + d1), k1));
             store4(high + d0, slot == 0 ? k0 : high4(load4(high + d0), k0));
@@ -372,38 +392,43 @@ __device__ __forceinline__ int pages_of(const PagedArgs& p, const Chunk& c) {
 }
 
 // Bounds of the pages that the chunks went to, from the keys as stored, which
-// L2 still holds: a block per touched page and kv head, its threads over 16
-// bytes of a row each and over the rows. Block k finds the k-th touched page
-// by a scan of the sequences' page counts.
-constexpr int kBoundsThreads = 256;
+// L2 still holds: a block per touched page and two kv heads, four warps per
+// head, their lanes over 16 bytes of a row each and over the rows: a 64-token
+// page's reads are all in flight at once, since latency is what this pass
+// costs. Block k finds the k-th touched page by a scan of the sequences' page
+// counts.
+constexpr int kBoundsHeads = 2, kBoundsWarps = 4;
 template <typename CT, int D>
-__global__ void __launch_bounds__(kBoundsThreads)
+__global__ void __launch_bounds__(kBoundsHeads * kBoundsWarps * 32)
     paged_bounds_rows_kernel(PagedArgs p, const int32_t* __restrict__ offsets, int rows) {
-  constexpr int kVec = 16 / sizeof(CT), kLanes = D / kVec, kRows = kBoundsThreads / kLanes;
-  __shared__ int sums[kBoundsThreads / 32];
+  constexpr int kVec = 16 / sizeof(CT), kLanes = D / kVec, kRows = 32 / kLanes;
+  const unsigned full = 0xffffffffu;
+  __shared__ int sums[kBoundsHeads * kBoundsWarps];
   __shared__ int found[2];
-  __shared__ __align__(16) CT low_s[kRows][D], high_s[kRows][D];
+  __shared__ uint4 part_s[kBoundsHeads][kBoundsWarps][2][kLanes];
   griddep_wait();
   griddep_launch_dependents();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, Hk = p.a.Hk;
-  const int want = blockIdx.x / Hk, kvh = blockIdx.x - want * Hk;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, Hk = p.a.Hk, threads = blockDim.x;
+  const int groups = (Hk + kBoundsHeads - 1) / kBoundsHeads;
+  const int want = blockIdx.x / groups, head = warp / kBoundsWarps, w = warp % kBoundsWarps;
+  const int kvh = (blockIdx.x - want * groups) * kBoundsHeads + head;
   int before = 0;
   if (tid == 0) found[0] = -1;
-  for (int base = 0; base < p.batch; base += kBoundsThreads) {
+  for (int base = 0; base < p.batch; base += threads) {
     const int b = base + tid;
     const int n = b < p.batch ? pages_of(p, chunk_of(p, offsets, rows, b)) : 0;
     int scan = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, scan, o);
+      const int v = __shfl_up_sync(full, scan, o);
       if (lane >= o) scan += v;
     }
     if (lane == 31) sums[warp] = scan;
     __syncthreads();
     int all = 0;
-    for (int w = 0; w < kBoundsThreads / 32; ++w) {
-      if (w < warp) scan += sums[w];
-      all += sums[w];
+    for (int i = 0; i < threads / 32; ++i) {
+      if (i < warp) scan += sums[i];
+      all += sums[i];
     }
     scan += before;  // pages up to and with sequence b's
     if (n > 0 && want < scan && want >= scan - n) {
@@ -420,30 +445,53 @@ __global__ void __launch_bounds__(kBoundsThreads)
   const int index = (c.start >> p.page_shift) + found[1], size = 1 << p.page_shift;
   const int page = p.table[static_cast<int64_t>(b) * p.width + index];
   if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.page_count)) return;  // reported by the append
-  const int begin = max(0, c.start - index * size), end = min(size, c.start + c.n - index * size);  // the page's new slots
-  const int d = (tid % kLanes) * kVec, r = tid / kLanes;
-  const CT* key = static_cast<const CT*>(p.key) + pool_row(p, page, kvh, 0) + d;
-  if (begin + r < end) {
-    uint4 low = *reinterpret_cast<const uint4*>(key + (begin + r) * p.slot_stride), high = low;
-#pragma unroll 4
-    for (int s = begin + r + kRows; s < end; s += kRows) {
+  // the page's new slots
+  const int64_t from = static_cast<int64_t>(index) << p.page_shift;
+  const int begin = static_cast<int>(max(static_cast<int64_t>(0), c.start - from));
+  const int end = static_cast<int>(min(static_cast<int64_t>(size), c.start + static_cast<int64_t>(c.n) - from));
+  const int d = (lane % kLanes) * kVec, r = w * kRows + lane / kLanes;
+  if (kvh < Hk) {
+    const CT* key = static_cast<const CT*>(p.key) + pool_row(p, page, kvh, 0) + d;
+    // rows past the end repeat the last one: the smallest and largest stay
+    uint4 low = *reinterpret_cast<const uint4*>(key + min(begin + r, end - 1) * p.slot_stride), high = low;
+#pragma unroll 8
+    for (int s = begin + r + kBoundsWarps * kRows; s < end; s += kBoundsWarps * kRows) {
       const uint4 u = *reinterpret_cast<const uint4*>(key + s * p.slot_stride);
       low = low_vec<CT>(low, u);
       high = high_vec<CT>(high, u);
     }
-    *reinterpret_cast<uint4*>(&low_s[r][d]) = low;
-    *reinterpret_cast<uint4*>(&high_s[r][d]) = high;
+#pragma unroll
+    for (int o = kLanes; o < 32; o <<= 1) {
+      const uint4 a = make_uint4(__shfl_xor_sync(full, low.x, o), __shfl_xor_sync(full, low.y, o),
+                                 __shfl_xor_sync(full, low.z, o), __shfl_xor_sync(full, low.w, o));
+      const uint4 h = make_uint4(__shfl_xor_sync(full, high.x, o), __shfl_xor_sync(full, high.y, o),
+                                 __shfl_xor_sync(full, high.z, o), __shfl_xor_sync(full, high.w, o));
+      low = low_vec<CT>(low, a);
+      high = high_vec<CT>(high, h);
+    }
+    if (lane < kLanes) {
+      part_s[head][w][0][lane] = low;
+      part_s[head][w][1][lane] = high;
+    }
   }
   __syncthreads();
-  const int held = min(kRows, end - begin);  // rows of the table that were filled
-  for (int i = tid; i < 2 * D; i += kBoundsThreads) {
-    const bool is_low = i < D;
-    const int e = is_low ? i : i - D;
-    CT* at = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D + i;
-    CT v = is_low ? low_s[0][e] : high_s[0][e];
-    for (int k = 1; k < held; ++k) v = is_low ? low_of(v, low_s[k][e]) : high_of(v, high_s[k][e]);
-    if (begin > 0) v = is_low ? low_of(at[0], v) : high_of(at[0], v);
-    at[0] = v;
+  if (kvh >= Hk || w != 0) return;
+  // the first lanes join the lows, the next the highs
+  for (int i = lane; i < 2 * kLanes; i += 32) {
+    const bool is_low = i < kLanes;
+    const int at = is_low ? i : i - kLanes;
+    uint4 v = part_s[head][0][is_low ? 0 : 1][at];
+#pragma unroll
+    for (int k = 1; k < kBoundsWarps; ++k) {
+      const uint4 u = part_s[head][k][is_low ? 0 : 1][at];
+      v = is_low ? low_vec<CT>(v, u) : high_vec<CT>(v, u);
+    }
+    CT* out = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D + (is_low ? 0 : D) + at * kVec;
+    if (begin > 0) {
+      const uint4 u = *reinterpret_cast<const uint4*>(out);
+      v = is_low ? low_vec<CT>(v, u) : high_vec<CT>(v, u);
+    }
+    *reinterpret_cast<uint4*>(out) = v;
   }
 }
 
@@ -489,7 +537,9 @@ cudaError_t bounds_t(const PagedArgs& p, bool rows_ok, const int32_t* offsets, i
   // a chunk of n rows touches at most (n - 1) / page_size + 2 pages, and no more than its rows
   const long long pages = min(static_cast<long long>(rows), (static_cast<long long>(rows) >> p.page_shift) + 2LL * p.batch);
   auto k = p.a.D == 64 ? paged_bounds_rows_kernel<CT, 64> : paged_bounds_rows_kernel<CT, 128>;
-  return launch_pdl(k, static_cast<unsigned>(pages * p.a.Hk), kBoundsThreads, 0, stream, p, offsets, rows);
+  const int heads = p.a.Hk < kBoundsHeads ? p.a.Hk : kBoundsHeads;
+  return launch_pdl(k, static_cast<unsigned>(pages * ((p.a.Hk + kBoundsHeads - 1) / kBoundsHeads)),
+                    heads * kBoundsWarps * 32, 0, stream, p, offsets, rows);
 }
 
 template <typename IO, typename CT>
