@@ -379,9 +379,11 @@ int tla_paged_append(tla_paged* layer, const void* qkv, const int32_t* positions
                      void* stream);
 
 /* Device bytes of workspace that tla_paged_decode and tla_paged_select need for
- * up to `batch` sequences and this table width (16-byte aligned; the contents
- * need no preparation and mean nothing afterwards). */
-int tla_paged_workspace(const tla_paged* layer, int32_t batch, int32_t table_width, size_t* bytes);
+ * `batch` sequences, this table width and page_count listed pages (0: no list);
+ * 0 where none is needed. 16-byte aligned; the contents need no preparation and
+ * mean nothing afterwards. Either output may be NULL. */
+int tla_paged_workspace(const tla_paged* layer, int32_t batch, int32_t table_width, int32_t page_count,
+                        size_t* decode_bytes, size_t* select_bytes);
 
 /* Attention of one new token per sequence over its pages, the new token's own
  * K/V included (append first): over the tokens of [window start, positions[b]],

@@ -73,7 +73,7 @@ def test_create_refuses(pkg, args, code):
 def test_calls_refuse_a_missing_layer(pkg):
     lib = pkg.lib()
     size = ctypes.c_size_t()
-    assert lib.tla_paged_workspace(None, 1, 1, ctypes.byref(size)) == INVALID
+    assert lib.tla_paged_workspace(None, 1, 1, 0, ctypes.byref(size), ctypes.byref(size)) == INVALID
     assert lib.tla_paged_append(None, 16, 16, None, 16, 1, 1, 1, 16, None) == INVALID
     assert lib.tla_paged_decode(None, 16, 16, 16, 1, None, 0, None, 16, 1, 16, 16, None) == INVALID
     assert lib.tla_paged_select(None, 16, 16, 16, 1, 0, 0, 16, 1, 1, 16, 16, None) == INVALID

@@ -3,6 +3,8 @@
 sequence is NaN, and the tables' unused entries name no page, so a read of
 either shows. Error bounds come with the reference's outputs; they count each
 rounding, and are derived there."""
+import ctypes
+
 import pytest
 import torch
 
@@ -544,8 +546,15 @@ def test_python_refuses(pkg, cuda):
     a.close()
     with pytest.raises(pkg.TlaError):
         a.decode(q, pos, table)
-    assert pkg.lib().tla_paged_decode(layer().handle, q.data_ptr(), pos.data_ptr(), table.data_ptr(), 1, None, 0, None,
-                                      q.data_ptr(), 2, None, 0, None) == -1  # no workspace
+    # a long table's call needs a workspace, and refuses none or a small one
+    long = pkg.PagedAttention(512, 8, 1 << 16, k, v, {"headDim": 64, "kvHeadCount": 2})
+    wide = torch.zeros(2, 4096, dtype=torch.int32, device=cuda)
+    need = ctypes.c_size_t()
+    assert pkg.lib().tla_paged_workspace(long.handle, 2, 4096, 0, ctypes.byref(need), None) == 0 and need.value > 0
+    work = torch.empty(need.value + 16, dtype=torch.uint8, device=cuda)
+    for at, size in ((None, 0), (work.data_ptr(), need.value - 1), (work.data_ptr() + 8, need.value)):
+        assert pkg.lib().tla_paged_decode(long.handle, q.data_ptr(), pos.data_ptr(), wide.data_ptr(), 4096, None, 0,
+                                          None, q.data_ptr(), 2, at, size, None) == -1
 
 
 def test_empty_calls(pkg, cuda):

@@ -153,7 +153,7 @@ def lib():
         L.tla_paged_create.argtypes = [P, ctypes.POINTER(AttnConfig), ctypes.POINTER(PagePool), P, P, ctypes.POINTER(P)]
         L.tla_paged_destroy.argtypes = [P]
         L.tla_paged_append.argtypes = [P, P, P, P, P, i32, i32, i32, P, P]
-        L.tla_paged_workspace.argtypes = [P, i32, i32, ctypes.POINTER(size_t)]
+        L.tla_paged_workspace.argtypes = [P, i32, i32, i32, ctypes.POINTER(size_t), ctypes.POINTER(size_t)]
         L.tla_paged_decode.argtypes = [P, P, P, P, i32, P, i32, P, P, i32, P, size_t, P]
         L.tla_paged_select.argtypes = [P, P, P, P, i32, i32, i32, P, i32, i32, P, size_t, P]
         for name in EXPORTS:

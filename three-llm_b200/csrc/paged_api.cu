@@ -63,10 +63,9 @@ bool rows_apart(const tla_page_pool& pool, int heads, int D) {
   return true;
 }
 
-// Enough for either decode path: which one runs depends on the call.
-size_t decode_workspace(const tla_paged* P, int batch) {
-  const size_t a = tla::paged_decode_generic_workspace(P, batch), b = tla::paged_decode_workspace(P);
-  return a > b ? a : b;
+size_t decode_workspace(const tla_paged* P, const tla::PagedArgs& p, int count) {
+  return tla::paged_decode_takes(P, p, count) ? tla::paged_decode_workspace(P, p, count)
+                                              : tla::paged_decode_generic_workspace(P, p.batch);
 }
 
 }  // namespace
@@ -152,10 +151,12 @@ int tla_paged_append(tla_paged* P, const void* qkv, const int32_t* positions, co
                                             row_offsets, rows, query_out, static_cast<cudaStream_t>(stream)));
 }
 
-int tla_paged_workspace(const tla_paged* P, int32_t batch, int32_t table_width, size_t* bytes) {
-  if (!P || !bytes || batch < 0 || batch > P->base.max_batch || table_width <= 0) return TLA_ERR_INVALID_ARG;
-  const size_t d = decode_workspace(P, batch), s = tla::paged_select_workspace(P, batch, table_width);
-  *bytes = ((d > s ? d : s) + 15) & ~size_t(15);
+int tla_paged_workspace(const tla_paged* P, int32_t batch, int32_t table_width, int32_t page_count,
+                        size_t* decode_bytes, size_t* select_bytes) {
+  if (!P || batch < 0 || batch > P->base.max_batch || table_width <= 0 || page_count < 0) return TLA_ERR_INVALID_ARG;
+  const tla::PagedArgs p = tla::paged_args(P, nullptr, nullptr, table_width, batch);
+  if (decode_bytes) *decode_bytes = batch > 0 ? decode_workspace(P, p, page_count) : 0;
+  if (select_bytes) *select_bytes = tla::paged_select_workspace(P, batch, table_width);
   return TLA_OK;
 }
 
@@ -168,10 +169,10 @@ int tla_paged_decode(tla_paged* P, const void* query, const int32_t* positions, 
   if (batch == 0) return TLA_OK;
   if (!query || !out || !aligned16(query) || !aligned16(out) || !aligned16(gate) || !aligned16(workspace))
     return TLA_ERR_INVALID_ARG;
-  const size_t need = decode_workspace(P, batch);
+  const tla::PagedArgs p = tla::paged_args(P, positions, page_table, table_width, batch);
+  const size_t need = decode_workspace(P, p, page_count);
   if (need > 0 && (!workspace || workspace_bytes < need)) return TLA_ERR_INVALID_ARG;
   DeviceGuard g(P->base.ctx->device);
-  const tla::PagedArgs p = tla::paged_args(P, positions, page_table, table_width, batch);
   if (tla::paged_decode_takes(P, p, page_count))
     return from_cuda(tla::launch_paged_decode(P, p, query, pages, page_count, gate, out, workspace,
                                               static_cast<cudaStream_t>(stream)));

@@ -70,6 +70,7 @@ struct DecodeParams {
   int subs;        // groups of up to 16 query heads per kv head
   int rows;        // query heads per such group, the last one's may be fewer
   int small_grid;
+  int whole;       // every pair goes to one CTA: nothing is joined
 };
 
 struct SmemLayout {
@@ -177,6 +178,23 @@ __device__ __forceinline__ Seg seg_at(const int* prefix, int b, int pairs, int g
   return s;
 }
 
+// The first pair that starts at or after unit g.
+__device__ __forceinline__ int next_pair(const int* prefix, int batch, int pairs, int g) {
+  if (g >= prefix[batch]) return prefix[batch];
+  int b = 0, n = batch;  // prefix[b] <= g < prefix[b + n]
+  while (n > 1) {
+    const int half = n / 2;
+    if (prefix[b + half] <= g) {
+      b += half;
+      n -= half;
+    } else {
+      n = half;
+    }
+  }
+  const int per = (prefix[b + 1] - prefix[b]) / pairs;
+  return prefix[b] + (g - prefix[b] + per - 1) / per * per;
+}
+
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int slot, int head,
                                             int page) {
   asm volatile(
@@ -267,7 +285,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         static_cast<IO*>(d.out)[static_cast<int64_t>(b) * Hq * D + i] = from_f32<IO>(0.f);
   const int grid = effective_grid(total, gridDim.x, d.small_grid);
   if (total == 0 || cta >= grid) return;
-  const int tb = cta_begin(cta, total, grid), te = cta_begin(cta + 1, total, grid);
+  int tb = cta_begin(cta, total, grid), te = cta_begin(cta + 1, total, grid);
+  if (d.whole) {
+    tb = next_pair(prefix, p.batch, pairs, tb);
+    te = next_pair(prefix, p.batch, pairs, te);
+  }
   if (tb >= te) return;
   const int shift = p.page_shift, mask = (1 << shift) - 1;
 
@@ -706,7 +728,7 @@ cudaError_t launch_t(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   const int grid = per_sm * P->base.ctx->sm_count;
   d.small_grid = P->base.ctx->sm_count;
   e = launch_pdl(kernel, grid, kThreads, smem, stream, d);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || d.whole) return e;
   return launch_pdl(paged_decode_join_kernel<D, IO>, static_cast<unsigned>(d.p.batch) * P->base.Hq, kJoinWarps * 32, 0,
                     stream, d, grid);
 }
@@ -764,22 +786,33 @@ void paged_decode_configure(tla_paged* P) {
   P->fast = make_pool_map(&q, pool.key, &P->tmap_k) && make_pool_map(&q, pool.value, &P->tmap_v);
 }
 
+// The most tiles that a pair of this call can have.
+long long most_tiles(const PagedArgs& p, int count) {
+  long long tokens = p.capacity, tiles = (tokens + kTile - 1) / kTile;
+  if (count > 0) {
+    const long long listed = ((static_cast<long long>(count) << p.page_shift) + kTile - 1) / kTile;
+    tiles = listed < tiles ? listed : tiles;
+  } else if (p.a.sliding > 0) {
+    const long long seen = (p.a.sliding - 2LL) / kTile + 2;
+    tiles = seen < tiles ? seen : tiles;
+  }
+  return tiles;
+}
+
+#ifndef WHOLE
+#define WHOLE 20
+#endif
+bool whole_pairs(const PagedArgs& p, int count) { return most_tiles(p, count) <= WHOLE; }
+
 // Whether a call's shares can be cut: the batch's table fits shared memory and
 // its tiles are counted in 32 bits.
 bool paged_decode_takes(const tla_paged* P, const PagedArgs& p, int count) {
-  if (!P->fast || p.batch > kMaxBatch) return false;
-  long long tokens = p.capacity;
-  if (count > 0) {
-    const long long listed = static_cast<long long>(count) << p.page_shift;
-    tokens = tokens < listed ? tokens : listed;
-  } else if (p.a.sliding > 0 && p.a.sliding + 2LL * kTile < tokens) {
-    tokens = p.a.sliding + 2LL * kTile;
-  }
-  return (tokens / kTile + 16) * p.a.Hk * subgroups(P) * p.batch < (1LL << 31);
+  return P->fast && p.batch <= kMaxBatch &&
+         (most_tiles(p, count) + 16) * p.a.Hk * subgroups(P) * p.batch < (1LL << 31);
 }
 
-size_t paged_decode_workspace(const tla_paged* P) {
-  if (!P->fast) return 0;
+size_t paged_decode_workspace(const tla_paged* P, const PagedArgs& p, int count) {
+  if (whole_pairs(p, count)) return 0;
   return static_cast<size_t>(kCtasPerSm) * P->base.ctx->sm_count * 2 * subgroup_rows(P) * (P->base.D + 2) *
          sizeof(float);
 }
@@ -799,6 +832,7 @@ cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const vo
   d.subs = subgroups(P);
   d.rows = subgroup_rows(P);
   d.small_grid = 0;
+  d.whole = whole_pairs(p, count) ? 1 : 0;
   return P->base.D == 64 ? launch_d<64>(P, d, stream) : launch_d<128>(P, d, stream);
 }
 

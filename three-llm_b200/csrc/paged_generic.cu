@@ -199,10 +199,8 @@ cudaError_t launch_t(const tla_paged* P, const PagedArgs& p, const void* query, 
 }  // namespace
 
 size_t paged_decode_generic_workspace(const tla_paged* P, int batch) {
-  // batch * shares_of(batch) is at most batch plus the blocks that fill the GPU
-  const int units = P->base.Hk * head_chunks(P);
-  const size_t rows = static_cast<size_t>(batch) + (4 * P->base.ctx->sm_count + units - 1) / units;
-  return rows * P->base.Hq * (P->base.D + 2) * sizeof(float);
+  const int shares = shares_of(P, batch);
+  return shares > 1 ? static_cast<size_t>(batch) * P->base.Hq * shares * (P->base.D + 2) * sizeof(float) : 0;
 }
 
 cudaError_t launch_paged_decode_generic(const tla_paged* P, const PagedArgs& p, const void* query,

@@ -8,17 +8,22 @@
 // in 64 bits: the choice is a whole number that a rounding next to the border
 // would change, and after rounding the sum once to 32 bits two ways of adding
 // it up agree.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include "paged.cuh"
 
 namespace tla {
 
+namespace cg = cooperative_groups;
+
 namespace {
 
-constexpr int kScoreThreads = 256;
-constexpr int kScorePages = 64;  // pages per block
-constexpr int kPickThreads = 256;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kMaxHeld = 48 * 1024;  // ranks that one block's shared memory holds
+constexpr int kScorePages = 256;     // pages per block of the scoring kernel for longer sequences
 
 // Larger scores have larger keys, and every score a key above 0.
 __device__ __forceinline__ uint32_t rank_of(float s) {
@@ -36,166 +41,314 @@ __device__ __forceinline__ PageRange page_range(const PagedArgs& p, int pos) {
   return {lo >> p.page_shift, (hi >> p.page_shift) - (lo >> p.page_shift) + 1};
 }
 
-// ranks[b][kvh][i]: page begin + i; the pages that always take part get the
-// highest ranks. A warp per page.
-template <typename IO, typename CT>
-__global__ void __launch_bounds__(kScoreThreads)
-    paged_score_kernel(PagedArgs p, const IO* __restrict__ query, int first, int last, int count,
-                       uint32_t* __restrict__ ranks) {
-  extern __shared__ double vec[];  // [2][D]: N, then P, as the bounds' order
-  griddep_wait();
-  griddep_launch_dependents();
-  const int D = p.a.D, G = p.a.G, Hk = p.a.Hk;
-  const int kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int b = blockIdx.z; b < p.batch; b += gridDim.z) {
-    const PageRange r = page_range(p, p.positions[b]);
-    if (r.n <= count) continue;  // all of them are taken
-    const int from = blockIdx.x * kScorePages, to = min(r.n, from + kScorePages);
-    if (from >= to) continue;
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += kScoreThreads) {
-      double neg = 0, pos = 0;
-      for (int g = 0; g < G; ++g) {
-        const float q = to_f32(query[(static_cast<int64_t>(b) * p.a.Hq + kvh * G + g) * D + d]);
-        neg += fminf(q, 0.f);
-        pos += fmaxf(q, 0.f);
-      }
-      vec[d] = neg;
-      vec[D + d] = pos;
+// The score's vector (N, then P, as the bounds' order), formed by a block.
+template <typename IO>
+__device__ __forceinline__ void form_vector(const PagedArgs& p, const IO* query, int b, int kvh, double* vec) {
+  const int D = p.a.D, G = p.a.G;
+  for (int d = threadIdx.x; d < D; d += kThreads) {
+    double neg = 0, pos = 0;
+    for (int g = 0; g < G; ++g) {
+      const float q = to_f32(query[(static_cast<int64_t>(b) * p.a.Hq + kvh * G + g) * D + d]);
+      neg += fminf(q, 0.f);
+      pos += fmaxf(q, 0.f);
     }
-    __syncthreads();
-    uint32_t* out = ranks + (static_cast<int64_t>(b) * Hk + kvh) * p.width;
-    for (int i = from + warp; i < to; i += kScoreThreads / 32) {
-      if (i < first || i >= r.n - last) {
-        if (lane == 0) out[i] = 0xffffffffu;
-        continue;
-      }
-      const int page = pool_page(p, b, r.begin + i);
-      if (page < 0) {
-        if (lane == 0) out[i] = 0u;
-        continue;
-      }
-      const CT* at = static_cast<const CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D;
-      double s = 0;
-      for (int d = lane; d < 2 * D; d += 32) s = fma(vec[d], static_cast<double>(to_f32(at[d])), s);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) out[i] = min(rank_of(static_cast<float>(s)), 0xfffffffeu);
-    }
+    vec[d] = neg;
+    vec[D + d] = pos;
   }
 }
 
-// The `count` highest ranks, ties to the lower page, in page order: a block
-// per (sequence, kv head). Four 8-bit passes find the lowest rank that is
-// taken and how many pages of exactly that rank are; one more writes the list.
-__global__ void __launch_bounds__(kPickThreads)
-    paged_pick_kernel(PagedArgs p, const uint32_t* __restrict__ ranks, int count, int32_t* __restrict__ pages_out) {
-  __shared__ int bins[256];
-  __shared__ int warp_sum_s[2][kPickThreads / 32];
-  __shared__ uint32_t prefix_s;
-  __shared__ int want_s;
-  griddep_wait();
-  griddep_launch_dependents();
-  const int Hk = p.a.Hk, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int b = blockIdx.x / Hk;
-  const int pos = p.positions[b];
-  const PageRange r = page_range(p, pos);
-  int32_t* out = pages_out + static_cast<int64_t>(blockIdx.x) * count;
-  if (r.n == 0 && pos >= 0 && tid == 0) report_error(p.a.error, TLA_ERR_POSITION);
-  if (r.n <= count) {
-    for (int i = tid; i < count; i += kPickThreads) out[i] = i < r.n ? r.begin + i : -1;
-    return;
+// Ranks of pages [from, to) of a pair, handed to `put(i, rank)` by one lane
+// each. A warp takes 32 pages at a time: its lanes look up their pages, then
+// each page's bounds are read across the warp, kAhead pages in flight.
+template <typename CT, typename Put>
+__device__ __forceinline__ void score_pages(const PagedArgs& p, const double* vec, int b, int kvh, PageRange r,
+                                            int first, int last, int from, int to, const Put& put) {
+  const unsigned full = 0xffffffffu;
+  const int D = p.a.D, Hk = p.a.Hk, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int base = from + warp * 32; base < to; base += kThreads) {
+    const int mine = base + lane;
+    const bool always = mine < first || mine >= r.n - last;
+    const int page = mine < to && !always ? pool_page(p, b, r.begin + mine) : -1;
+    uint32_t rank = always ? 0xffffffffu : 0u;  // (a page outside the pool ranks last)
+    const int n = min(32, to - base);
+    auto add = [&](int k, double s) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(full, s, o);
+      if (lane == k && page >= 0) rank = min(rank_of(static_cast<float>(s)), 0xfffffffeu);
+    };
+    const CT* bounds = static_cast<const CT*>(p.bounds) + static_cast<int64_t>(kvh) * 2 * D;
+    const int64_t stride = static_cast<int64_t>(Hk) * 2 * D;
+    if (sizeof(CT) == 2 && D == 128) {  // 8 elements of a page's 256 per lane
+      constexpr int kAhead = 4;
+      double v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = vec[lane * 8 + e];
+      for (int k = 0; k < n; k += kAhead) {
+        uint4 u[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int at = __shfl_sync(full, page, k + a);
+          u[a] = at < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(bounds + at * stride + lane * 8);
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const CT* x = reinterpret_cast<const CT*>(&u[a]);
+          double s0 = 0, s1 = 0;
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            s0 = fma(v[e], static_cast<double>(to_f32(x[e])), s0);
+            s1 = fma(v[e + 1], static_cast<double>(to_f32(x[e + 1])), s1);
+          }
+          add(k + a, s0 + s1);
+        }
+      }
+    } else {
+      for (int k = 0; k < n; ++k) {
+        const int at = __shfl_sync(full, page, k);
+        double s = 0;
+        if (at >= 0)
+          for (int d = lane; d < 2 * D; d += 32) s = fma(vec[d], static_cast<double>(to_f32(bounds[at * stride + d])), s);
+        add(k, s);
+      }
+    }
+    if (mine < to) put(mine, rank);
   }
-  const uint32_t* rank = ranks + static_cast<int64_t>(blockIdx.x) * p.width;
+}
+
+// Writes the `count` pages of the highest ranks, ties to the lower page, in
+// page order, by one block. The lowest rank that is taken is found two bits at
+// a time from the top: each round counts how many ranks share the bits found
+// so far and have at least 1, 2, 3 in the next two, by votes and sums across
+// the warps (ranks of like pages agree in most high bits, which a table of
+// counters would serialise on), and it ends early when every rank that shares
+// the bits is taken.
+struct PickSmem {
+  int counts[2][kWarps][4];
+  int taken[kWarps], same[kWarps];
+};
+__device__ __forceinline__ void pick_pages(const uint32_t* rank, PageRange r, int count, int32_t* out, PickSmem* sm) {
+  const unsigned full = 0xffffffffu;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t prefix = 0;
-  int want = count;  // pages still to take among those that share the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kPickThreads) bins[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < r.n; i += kPickThreads) {
-      const uint32_t v = rank[i];
-      if (shift == 24 || v >> (shift + 8) == prefix) atomicAdd(&bins[(v >> shift) & 255], 1);
+  int want = count;  // pages still to take among those that share the bits found
+  int shift = 30;
+  for (;; shift -= 2) {
+    int c1 = 0, c2 = 0, c3 = 0;
+    for (int i = tid; i < r.n; i += kThreads) {
+      const uint32_t v = rank[i] >> shift;
+      if (shift < 30 && (v >> 2) != prefix >> (shift + 2)) continue;
+      const int digit = v & 3;
+      c1 += digit >= 1;
+      c2 += digit >= 2;
+      c3 += digit >= 3;
+    }
+    c1 = __reduce_add_sync(full, c1);
+    c2 = __reduce_add_sync(full, c2);
+    c3 = __reduce_add_sync(full, c3);
+    int* mine = sm->counts[(shift >> 1) & 1][warp];
+    if (lane == 0) {
+      mine[0] = c1;
+      mine[1] = c2;
+      mine[2] = c3;
     }
     __syncthreads();
-    if (tid == 0) {
-      int bin = 255;
-      while (bin > 0 && bins[bin] < want) want -= bins[bin--];
-      prefix_s = prefix << 8 | static_cast<uint32_t>(bin);
-      want_s = want;
+    const int* all = sm->counts[(shift >> 1) & 1][lane % kWarps];
+    c1 = __reduce_add_sync(full, lane < kWarps ? all[0] : 0);
+    c2 = __reduce_add_sync(full, lane < kWarps ? all[1] : 0);
+    c3 = __reduce_add_sync(full, lane < kWarps ? all[2] : 0);
+    uint32_t digit = 0;
+    int here = -1;  // ranks with exactly this digit, where that says that all are taken
+    if (want <= c3) {
+      digit = 3;
+      here = c3;
+    } else if (want <= c2) {
+      digit = 2;
+      want -= c3;
+      here = c2 - c3;
+    } else if (want <= c1) {
+      digit = 1;
+      want -= c2;
+      here = c1 - c2;
+    } else {
+      want -= c1;
     }
-    __syncthreads();
-    prefix = prefix_s;
-    want = want_s;
+    prefix |= digit << shift;
+    if (shift == 0 || here == want) break;
   }
+  // taken: ranks whose bits from `shift` up are above the prefix's, and the first `want` that equal it
+  const uint32_t border = prefix >> shift;
   int taken = 0, equal = 0;  // before this round of pages
-  for (int base = 0; base < r.n; base += kPickThreads) {
+  for (int base = 0; base < r.n; base += kThreads) {
     const int i = base + tid;
-    const uint32_t v = i < r.n ? rank[i] : 0u;
-    const bool above = i < r.n && v > prefix, same = i < r.n && v == prefix;
-    const unsigned same_mask = __ballot_sync(0xffffffffu, same);
-    if (lane == 0) warp_sum_s[0][warp] = __popc(same_mask);
+    const uint32_t v = i < r.n ? rank[i] >> shift : 0u;
+    const bool above = i < r.n && v > border, same = i < r.n && v == border;
+    const unsigned same_mask = __ballot_sync(full, same);
     __syncthreads();
-    int eq = equal + __popc(same_mask & ((1u << lane) - 1));
-    int eq_all = 0;
-    for (int w = 0; w < kPickThreads / 32; ++w) {
-      if (w < warp) eq += warp_sum_s[0][w];
-      eq_all += warp_sum_s[0][w];
+    if (lane == 0) sm->same[warp] = __popc(same_mask);
+    __syncthreads();
+    int eq = equal + __popc(same_mask & ((1u << lane) - 1)), all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) eq += sm->same[w];
+      all += sm->same[w];
     }
+    equal += all;
     const bool take = above || (same && eq < want);
-    const unsigned take_mask = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) warp_sum_s[1][warp] = __popc(take_mask);
+    const unsigned take_mask = __ballot_sync(full, take);
+    if (lane == 0) sm->taken[warp] = __popc(take_mask);
     __syncthreads();
     int at = taken + __popc(take_mask & ((1u << lane) - 1));
-    int all = 0;
-    for (int w = 0; w < kPickThreads / 32; ++w) {
-      if (w < warp) at += warp_sum_s[1][w];
-      all += warp_sum_s[1][w];
+    all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) at += sm->taken[w];
+      all += sm->taken[w];
     }
     if (take) out[at] = r.begin + i;
     taken += all;
-    equal += eq_all;
-    __syncthreads();
   }
 }
 
+// All of a pair's pages, when there are no more than `count`.
+__device__ __forceinline__ void list_all(const PagedArgs& p, int pos, PageRange r, int count, int32_t* out) {
+  if (r.n == 0 && pos >= 0 && threadIdx.x == 0) report_error(p.a.error, TLA_ERR_POSITION);
+  for (int i = threadIdx.x; i < count; i += kThreads) out[i] = i < r.n ? r.begin + i : -1;
+}
+
+// A cluster per (sequence, kv head): its blocks score a share of the pages
+// each and leave the ranks in the first block's shared memory, which picks.
+// One launch: what a step waits for here is latency, not the bounds' bytes.
 template <typename IO, typename CT>
-cudaError_t select_t(const PagedArgs& p, const void* query, int first, int last, int32_t* pages_out, int count,
-                     uint32_t* ranks, cudaStream_t stream) {
-  const int most = min(p.width, (p.capacity + (1 << p.page_shift) - 1) >> p.page_shift);
-  if (most > count) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((most + kScorePages - 1) / kScorePages, p.a.Hk, min(p.batch, 65535));
-    cfg.blockDim = dim3(kScoreThreads);
-    cfg.dynamicSmemBytes = 2 * p.a.D * sizeof(double);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_score_kernel<IO, CT>, p, static_cast<const IO*>(query), first,
-                                             last, count, ranks);
-    if (e != cudaSuccess) return e;
+__global__ void __launch_bounds__(kThreads)
+    paged_select_kernel(PagedArgs p, const IO* __restrict__ query, int first, int last, int count,
+                        int32_t* __restrict__ pages_out) {
+  extern __shared__ __align__(16) double vec[];  // [2][D], then the ranks
+  __shared__ PickSmem pick_s;
+  uint32_t* ranks = reinterpret_cast<uint32_t*>(vec + 2 * p.a.D);
+  griddep_wait();
+  griddep_launch_dependents();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int share = cluster.block_rank(), shares = cluster.num_blocks();
+  const int pair = blockIdx.x / shares, b = pair / p.a.Hk, kvh = pair - b * p.a.Hk;
+  const int pos = p.positions[b];
+  const PageRange r = page_range(p, pos);
+  int32_t* out = pages_out + static_cast<int64_t>(pair) * count;
+  if (r.n <= count) {  // (the same for the whole cluster)
+    if (share == 0) list_all(p, pos, r, count, out);
+    return;
   }
-  return launch_pdl(paged_pick_kernel, static_cast<unsigned>(p.batch) * p.a.Hk, kPickThreads, 0, stream, p,
+  // every block of the cluster runs before one writes into another's memory
+  if (shares > 1) cluster.sync();
+  form_vector(p, query, b, kvh, vec);
+  __syncthreads();
+  uint32_t* held = shares > 1 ? cluster.map_shared_rank(ranks, 0) : ranks;
+  const int per = (r.n + shares - 1) / shares, from = share * per;
+  score_pages<CT>(p, vec, b, kvh, r, first, last, from, min(r.n, from + per),
+                  [&](int i, uint32_t rank) { held[i] = rank; });
+  if (shares > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  if (share == 0) pick_pages(ranks, r, count, out, &pick_s);
+}
+
+// The same in two launches, the ranks in the workspace, for sequences of more
+// pages than shared memory holds ranks.
+template <typename IO, typename CT>
+__global__ void __launch_bounds__(kThreads)
+    paged_score_kernel(PagedArgs p, const IO* __restrict__ query, int first, int last, int count,
+                       uint32_t* __restrict__ ranks) {
+  extern __shared__ __align__(16) double vec[];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int kvh = blockIdx.y;
+  for (int b = blockIdx.z; b < p.batch; b += gridDim.z) {
+    const PageRange r = page_range(p, p.positions[b]);
+    const int from = blockIdx.x * kScorePages, to = min(r.n, from + kScorePages);
+    if (r.n <= count || from >= to) continue;
+    __syncthreads();
+    form_vector(p, query, b, kvh, vec);
+    __syncthreads();
+    uint32_t* held = ranks + (static_cast<int64_t>(b) * p.a.Hk + kvh) * p.width;
+    score_pages<CT>(p, vec, b, kvh, r, first, last, from, to, [&](int i, uint32_t rank) { held[i] = rank; });
+  }
+}
+__global__ void __launch_bounds__(kThreads)
+    paged_pick_kernel(PagedArgs p, const uint32_t* __restrict__ ranks, int count, int32_t* __restrict__ pages_out) {
+  __shared__ PickSmem pick_s;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int pos = p.positions[blockIdx.x / p.a.Hk];
+  const PageRange r = page_range(p, pos);
+  int32_t* out = pages_out + static_cast<int64_t>(blockIdx.x) * count;
+  if (r.n <= count)
+    list_all(p, pos, r, count, out);
+  else
+    pick_pages(ranks + static_cast<int64_t>(blockIdx.x) * p.width, r, count, out, &pick_s);
+}
+
+// Pages that a sequence can have in this call.
+int most_pages(int width, int shift, int capacity) {
+  const long long n = (static_cast<long long>(capacity) + (1 << shift) - 1) >> shift;
+  return static_cast<int>(n < width ? n : width);
+}
+
+template <typename IO, typename CT>
+cudaError_t select_t(const tla_paged* P, const PagedArgs& p, const void* query, int first, int last,
+                     int32_t* pages_out, int count, uint32_t* ranks, cudaStream_t stream) {
+  const int most = most_pages(p.width, p.page_shift, p.capacity);
+  const long long pairs = static_cast<long long>(p.batch) * p.a.Hk;
+  const size_t vec = 2 * p.a.D * sizeof(double);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (most <= kMaxHeld) {
+    // Blocks per pair: as many as leave every SM one block, at least 64 pages each.
+    int shares = 1;
+    while (shares < kMaxCluster && pairs * shares * 2 <= P->base.ctx->sm_count && most > 64 * shares) shares *= 2;
+    auto k = paged_select_kernel<IO, CT>;
+    const size_t smem = vec + (most > count ? most * sizeof(uint32_t) : 0);
+    if (smem > 48 * 1024) {
+      const cudaError_t e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem));
+      if (e != cudaSuccess) return e;
+    }
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = shares;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(pairs * shares));
+    cfg.dynamicSmemBytes = smem;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, k, p, static_cast<const IO*>(query), first, last, count, pages_out);
+  }
+  cfg.gridDim = dim3((most + kScorePages - 1) / kScorePages, p.a.Hk, p.batch < 65535 ? p.batch : 65535);
+  cfg.dynamicSmemBytes = vec;
+  const cudaError_t e =
+      cudaLaunchKernelEx(&cfg, paged_score_kernel<IO, CT>, p, static_cast<const IO*>(query), first, last, count, ranks);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(paged_pick_kernel, static_cast<unsigned>(pairs), kThreads, 0, stream, p,
                     static_cast<const uint32_t*>(ranks), count, pages_out);
 }
 
 }  // namespace
 
 size_t paged_select_workspace(const tla_paged* P, int batch, int width) {
-  return P->pool.bounds ? static_cast<size_t>(batch) * P->base.Hk * width * sizeof(uint32_t) : 0;
+  const PagedArgs p = paged_args(P, nullptr, nullptr, width, batch);
+  if (!P->pool.bounds || most_pages(width, P->page_shift, p.capacity) <= kMaxHeld) return 0;
+  return static_cast<size_t>(batch) * P->base.Hk * width * sizeof(uint32_t);
 }
 
 cudaError_t launch_paged_select(const tla_paged* P, const PagedArgs& p, const void* query, int first, int last,
                                 int32_t* pages_out, int count, void* workspace, cudaStream_t stream) {
   uint32_t* ranks = static_cast<uint32_t*>(workspace);
-  if (P->io == kFp16) return select_t<__half, __half>(p, query, first, last, pages_out, count, ranks, stream);
+  if (P->io == kFp16) return select_t<__half, __half>(P, p, query, first, last, pages_out, count, ranks, stream);
   if (P->io == kBf16)
-    return select_t<__nv_bfloat16, __nv_bfloat16>(p, query, first, last, pages_out, count, ranks, stream);
-  if (P->kept == kFp16) return select_t<float, __half>(p, query, first, last, pages_out, count, ranks, stream);
-  if (P->kept == kBf16) return select_t<float, __nv_bfloat16>(p, query, first, last, pages_out, count, ranks, stream);
-  return select_t<float, float>(p, query, first, last, pages_out, count, ranks, stream);
+    return select_t<__nv_bfloat16, __nv_bfloat16>(P, p, query, first, last, pages_out, count, ranks, stream);
+  if (P->kept == kFp16) return select_t<float, __half>(P, p, query, first, last, pages_out, count, ranks, stream);
+  if (P->kept == kBf16) return select_t<float, __nv_bfloat16>(P, p, query, first, last, pages_out, count, ranks, stream);
+  return select_t<float, float>(P, p, query, first, last, pages_out, count, ranks, stream);
 }
 
 }  // namespace tla

@@ -221,7 +221,7 @@ size_t paged_decode_generic_workspace(const tla_paged* P, int batch);
 // Tensor-core path: set up at creation, and whether it takes a call (count: listed pages, 0 for all).
 void paged_decode_configure(tla_paged* P);
 bool paged_decode_takes(const tla_paged* P, const PagedArgs& p, int count);
-size_t paged_decode_workspace(const tla_paged* P);
+size_t paged_decode_workspace(const tla_paged* P, const PagedArgs& p, int count);
 cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const void* query, const int32_t* pages,
                                 int count, const void* gate, void* out, void* workspace, cudaStream_t stream);
 

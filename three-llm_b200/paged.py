@@ -155,13 +155,19 @@ class PagedAttention:
         with torch.cuda.stream(stream):
             return torch.empty(shape, dtype=dtype, device=self.device)
 
-    def _workspace(self, batch, width, stream):
-        n = self._workspace_bytes.get((batch, width))
-        if n is None:
-            size = ctypes.c_size_t()
-            check(self._lib.tla_paged_workspace(self.handle, batch, width, ctypes.byref(size)), "workspace")
-            n = self._workspace_bytes[batch, width] = size.value
-        return self._new(n, torch.uint8, stream), n
+    def _workspace(self, batch, width, count, which, stream):
+        """(the tensor that keeps it, its address, its size) of a call's workspace; which: 0 decode, 1 select."""
+        sizes = self._workspace_bytes.get((batch, width, count))
+        if sizes is None:
+            d, s = ctypes.c_size_t(), ctypes.c_size_t()
+            check(self._lib.tla_paged_workspace(self.handle, batch, width, count, ctypes.byref(d), ctypes.byref(s)),
+                  "workspace")
+            sizes = self._workspace_bytes[batch, width, count] = (d.value, s.value)
+        size = sizes[which]
+        if size == 0:
+            return None, None, 0
+        work = self._new(size, torch.uint8, stream)
+        return work, work.data_ptr(), size
 
     # ---- the operators
     def append(self, qkv, positions, page_table, row_offsets=None, query=None, stream=None):
@@ -210,9 +216,9 @@ class PagedAttention:
             out = self._new((batch, self.qSize), self.dtype, stream)
         else:
             self._rows(out, "out", batch, self.qSize)
-        work, size = self._workspace(batch, width, stream)
+        work, at, size = self._workspace(batch, width, count, 0, stream)
         rc = self._lib.tla_paged_decode(self.handle, query.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
-                                        width, listed, count, gate, out.data_ptr(), batch, work.data_ptr(), size, on)
+                                        width, listed, count, gate, out.data_ptr(), batch, at, size, on)
         if rc:
             check(rc, "decode")
         return out
@@ -228,10 +234,9 @@ class PagedAttention:
             pages = self._new((batch, self.kvHeadCount, max(count, 0)), torch.int32, stream)
         else:
             self._ints(pages, "pages", (batch, self.kvHeadCount, count))
-        work, size = self._workspace(batch, width, stream)
+        work, at, size = self._workspace(batch, width, 0, 1, stream)
         rc = self._lib.tla_paged_select(self.handle, query.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
-                                        width, int(first), int(last), pages.data_ptr(), count, batch, work.data_ptr(),
-                                        size, on)
+                                        width, int(first), int(last), pages.data_ptr(), count, batch, at, size, on)
         if rc:
             check(rc, "select")
         return pages
