@@ -5,18 +5,26 @@
 //
 // Each K and V element is read once and used by the group's query heads, about
 // 2 G operations per byte: memory bounds it, so the kernel's shape follows the
-// reads. A (sequence, kv head) pair's tokens are cut into 64-token tiles, and
-// the tiles of all pairs into equal contiguous shares, one per resident CTA,
-// whatever the sequences' lengths; a share may begin and end inside a pair. A
-// producer warp walks the share's pages: its lanes look up 32 table entries at
-// a time, one window ahead, and start one TMA box per page piece of a tile
-// (five-dimensional tensor maps: any order and padding of pages, heads and
-// slots, as long as the strides are multiples of 16 bytes) into a ring of
-// stages. Four consumer warps own 16 tokens of a tile each: 16 tokens always
-// lie in one page, so a page's end inside a tile, a page that is not in the
-// pool and the window's edges are decided per warp from the 16 tokens' first
-// position, which the producer leaves beside the stage. S = Q K^T and
-// O += P V run as m16n8k16 tensor-core tiles with the group's heads as rows.
+// reads. A (sequence, kv head) pair's tokens are cut into tiles (64 tokens at
+// head_dim 64, 32 at 128: 16 KB of K and V), and the tiles of all pairs into
+// equal contiguous shares, one per resident CTA, whatever the sequences'
+// lengths; a share may begin and end inside a pair. A producer warp walks the
+// share's pages: its lanes look up 32 table entries at a time, one window
+// ahead, and start one TMA box per page piece of a tile (five-dimensional
+// tensor maps: any order and padding of pages, heads and slots, as long as the
+// strides are multiples of 16 bytes) into a ring of stages. Four consumer warps
+// take the tiles in turn, each a whole tile by itself, so that a tile's chain
+// of products, maximum, exponentials and products again is four deep in flight
+// per CTA and needs no barrier between warps. 16 tokens always lie in one
+// page: a page's end inside a tile, a page that is not in the pool and the
+// window's edges are decided per 16 tokens from their first position, which
+// the producer leaves beside the stage.
+//
+// S^T = K Q^T and O^T += V^T P^T run as m16n8k16 tensor-core tiles: the tokens
+// (then the dimensions) are the 16 rows and the group's query heads the 8
+// columns (two column tiles for groups over 8), so that groups of 8 and fewer
+// waste no half of a tile, and P^T moves from accumulators to an operand by
+// one 8 x 8 transposition per 8 tokens.
 //
 // Pairs that several CTAs share leave (m, l, o) triples in the caller's
 // workspace, which a second kernel joins: no counters, so nothing has to be
@@ -36,7 +44,6 @@ namespace tla {
 
 namespace {
 
-constexpr int kTile = 64;
 constexpr int kConsumerWarps = 4;
 constexpr int kThreads = (kConsumerWarps + 1) * 32;
 constexpr int kMaxBatch = 1024;  // prefix table in shared memory
@@ -45,16 +52,33 @@ constexpr int kMaxGrid = 1024;   // segment table of the joining kernel
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNowhere = -(1 << 30);  // first position of 16 tokens that take no part
 
+#ifndef STG
+#define STG 4
+#endif
+#ifndef TILE64
+#define TILE64 64
+#endif
+#ifndef TILE128
+#define TILE128 32
+#endif
+#ifndef SETUP64
+#define SETUP64 4
+#endif
+#ifndef SETUP128
+#define SETUP128 4
+#endif
 template <int D>
 struct Cfg {
-  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kTile = D == 64 ? TILE64 : TILE128;
+  static constexpr int kGroups = kTile / 16;
+  static constexpr int kStages = STG;      // a multiple of the consumer warps: a stage is always the same warp's
   static constexpr int kHalves = D / 64;  // 128-byte rows per cache row
   static constexpr int kTileBytes = kTile * kHalves * 128;
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kQPitch = D * 2 + 16;
   // A pair costs its query set-up and its epilogue besides its tiles: counted
   // as this many tiles when the shares are cut.
-  static constexpr int kSetup = D == 64 ? 6 : 3;
+  static constexpr int kSetup = D == 64 ? SETUP64 : SETUP128;
 };
 
 struct DecodeParams {
@@ -106,7 +130,9 @@ __host__ __device__ inline SmemLayout smem_layout(int rows, int batch, bool spli
 struct Walk {
   int lo, hi, first, tiles;
 };
+template <int D>
 __device__ __forceinline__ Walk walk_of(const DecodeParams& d, int pos) {
+  constexpr int kTile = Cfg<D>::kTile;
   Walk w;
   if (!paged_range(d.p, pos, &w.lo, &w.hi)) return {0, -1, 0, 0};
   if (d.pages) {
@@ -122,7 +148,7 @@ __device__ __forceinline__ Walk walk_of(const DecodeParams& d, int pos) {
 
 template <int D>
 __device__ __forceinline__ int units_of(const DecodeParams& d, int pos) {
-  const int tiles = walk_of(d, pos).tiles;
+  const int tiles = walk_of<D>(d, pos).tiles;
   return tiles > 0 ? (tiles + Cfg<D>::kSetup) * d.p.a.Hk * d.subs : 0;
 }
 
@@ -231,6 +257,13 @@ __device__ __forceinline__ uint32_t pack_rest(uint32_t packed, float lo, float h
   return pack_half2(lo - f.x, hi - f.y);
 }
 
+// An 8 x 8 matrix of 16-bit values, a row pair of which each lane holds, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 template <typename IO>
 __device__ __forceinline__ void store_out(const DecodeParams& d, int64_t i, float v) {
   if (d.gate) v = v * (1.f / (1.f + expf(-to_f32(static_cast<const IO*>(d.gate)[i]))));  // math.ts:271-273
@@ -250,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   uint8_t* stages = smem + L.stages;
   int* prefix = reinterpret_cast<int*>(smem + L.prefix);
   int* spos = prefix + p.batch + 1;
-  int* meta = reinterpret_cast<int*>(smem + L.meta);  // [stage][4]: first position of each 16 tokens
+  int* meta = reinterpret_cast<int*>(smem + L.meta);  // [stage][4]: first position of each 16 tokens of its tile
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);
   uint64_t* empty = full + C::kStages;
   volatile int* flags = reinterpret_cast<volatile int*>(smem + L.flags);  // [0] a wait gave up
@@ -259,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     flags[0] = 0;
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kConsumerWarps);
+      mbar_init(&empty[s], 1);
     }
     fence_mbar_init();
     prefix[0] = 0;
@@ -295,7 +328,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
 
   if (warp == kConsumerWarps) {
     // ================================================================ producer
-    const int boxes = shift >= 6 ? 1 : kTile >> shift;  // per tile, K or V
+    constexpr int kTile = C::kTile;
+    const int boxes = max(1, kTile >> shift);  // per tile, K or V
     const int box_rows = kTile / boxes, box_bytes = C::kTileBytes / boxes;
     uint32_t it = 0;
     int b = 0;
@@ -305,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       g = sg.next;
       if (sg.n == 0) continue;
       const int kvh = sg.pair / d.subs;
-      const Walk w = walk_of(d, spos[b]);
+      const Walk w = walk_of<D>(d, spos[b]);
       const int32_t* list = d.pages ? d.pages + (static_cast<int64_t>(b) * p.a.Hk + kvh) * d.count : nullptr;
       const int last_page = w.hi >> shift;
       // entries of the table (or the list) that this share walks
@@ -336,16 +370,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         }
         const int piece = lane % boxes;  // lanes 0..boxes-1 load K, the next V
         const int my_page = __shfl_sync(0xffffffffu, page, e - base + piece);
-        const int group_piece = lane * 16 / box_rows;  // lanes 0..3: the 16-token groups
-        const int g_index = __shfl_sync(0xffffffffu, index, e - base + (lane < 4 ? group_piece : 0));
-        const int g_page = __shfl_sync(0xffffffffu, page, e - base + (lane < 4 ? group_piece : 0));
+        const int group_piece = lane * 16 / box_rows;  // first lanes: the tile's groups of 16 tokens
+        const int g_index = __shfl_sync(0xffffffffu, index, e - base + (lane < C::kGroups ? group_piece : 0));
+        const int g_page = __shfl_sync(0xffffffffu, page, e - base + (lane < C::kGroups ? group_piece : 0));
         const int loaded = __popc(__ballot_sync(0xffffffffu, lane < boxes && my_page >= 0));
         const bool go = !flags[0] && mbar_wait(&empty[s], ph ^ 1u, p.a.error);
         if (__any_sync(0xffffffffu, !go)) {
           flags[0] = 1;
           continue;
         }
-        if (lane < 4)
+        if (lane < C::kGroups)
           meta[s * 4 + lane] = g_page < 0 ? kNowhere : (g_index << shift) + offset + lane * 16 - group_piece * box_rows;
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&full[s], 2 * loaded * box_bytes);
@@ -365,8 +399,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   // ================================================================== consumers
   CT* q_s = reinterpret_cast<CT*>(smem + L.q);
   float* red = reinterpret_cast<float*>(smem + L.red);
-  const int g_row = lane >> 2, t4 = lane & 3;
-  uint32_t it = 0;
+  constexpr int kNt = TWO ? 2 : 1;  // column tiles of 8 query heads
+  constexpr int kGroups = C::kGroups;
+  const int g8 = lane >> 2, t4 = lane & 3;
+  const int frag_row = (lane & 7) + ((lane >> 3) & 1) * 8;   // K as the left operand: token rows, then dimensions
+  const int vfrag_row = (lane & 7) + (lane >> 4) * 8;        // V transposed: its tokens are the columns
+  uint32_t it0 = 0;  // the share's tiles before this segment
   int b = 0;
   for (int g = tb; g < te;) {
     while (prefix[b + 1] <= g) ++b;
@@ -377,12 +415,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     }
     const int kvh = sg.pair / d.subs, sub = sg.pair - kvh * d.subs;
     const int h0 = kvh * G + sub * rows, heads = min(rows, (kvh + 1) * G - h0);
-    const Walk w = walk_of(d, spos[b]);
+    const Walk w = walk_of<D>(d, spos[b]);
     const IO* q = static_cast<const IO*>(d.query) + (static_cast<int64_t>(b) * Hq + h0) * D;
     // ---- the group's queries, 8 elements per thread and trip; rows past the group are zeros
-    float up0 = 1.f, up1 = 1.f;  // SPLIT: the power of two that this thread's two rows were divided by
     if constexpr (SPLIT) {
-      for (int r = warp; r < 16; r += kConsumerWarps) {
+      for (int r = warp; r < 8 * kNt; r += kConsumerWarps) {
         float x[D / 32], top = 0.f;
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) {
@@ -406,145 +443,159 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
           *reinterpret_cast<float*>(q_s + r * (C::kQPitch / 2) + D) = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
       }
     } else {
-      for (int i = tid; i < 16 * D / 8; i += 128) {
+      for (int i = tid; i < 8 * kNt * D / 8; i += 128) {
         const int r = i / (D / 8), c = i - r * (D / 8);
         const uint4 v = r < heads ? reinterpret_cast<const uint4*>(q)[i] : make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(q_s + r * (C::kQPitch / 2) + c * 8) = v;
       }
     }
     named_barrier_sync(1, 128);
-    uint32_t qa[D / 16][4];
-    uint32_t ql[SPLIT ? D / 16 : 1][4];
+    uint32_t qb[kNt][D / 16][2];
+    uint32_t ql[kNt][SPLIT ? D / 16 : 1][2];
+    float scale[kNt][2];
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      const int r = (lane & 7) + ((lane >> 3) & 1) * 8;
-      const int ch = 2 * kk + (lane >> 4);
-      ldsm_x4(smem_u32(q_s) + r * C::kQPitch + ch * 16, qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3]);
-      if constexpr (SPLIT)
-        ldsm_x4(smem_u32(q_s) + (16 + r) * C::kQPitch + ch * 16, ql[kk][0], ql[kk][1], ql[kk][2], ql[kk][3]);
-    }
-    if constexpr (SPLIT) {
-      up0 = *reinterpret_cast<const float*>(q_s + g_row * (C::kQPitch / 2) + D);
-      up1 = *reinterpret_cast<const float*>(q_s + (g_row + 8) * (C::kQPitch / 2) + D);
-    }
-    const float scale0 = p.a.attn_scale * kLog2e * up0, scale1 = p.a.attn_scale * kLog2e * up1;
-
-    float o[D / 8][4];
+    for (int nt = 0; nt < kNt; ++nt) {
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      for (int kk = 0; kk < D / 16; kk += 2) {  // 8 heads x 32 dimensions
+        const uint32_t at = smem_u32(q_s) + (nt * 8 + (lane & 7)) * C::kQPitch + (2 * kk + (lane >> 3)) * 16;
+        ldsm_x4(at, qb[nt][kk][0], qb[nt][kk][1], qb[nt][kk + 1][0], qb[nt][kk + 1][1]);
+        if constexpr (SPLIT)
+          ldsm_x4(at + 16 * C::kQPitch, ql[nt][kk][0], ql[nt][kk][1], ql[nt][kk + 1][0], ql[nt][kk + 1][1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        scale[nt][e] = p.a.attn_scale * kLog2e;
+        if constexpr (SPLIT)
+          scale[nt][e] *= *reinterpret_cast<const float*>(q_s + (nt * 8 + 2 * t4 + e) * (C::kQPitch / 2) + D);
+      }
+    }
 
-    // ---- stream the segment's tiles
-    for (int j = 0; j < sg.n; ++j, ++it) {
+    // this thread's columns: heads nt * 8 + 2 * t4 + e
+    float o[kNt][D / 16][4], m[kNt][2], l[kNt][2];
+#pragma unroll
+    for (int nt = 0; nt < kNt; ++nt) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+
+    // ---- this warp's tiles of the segment
+    const uint32_t it1 = it0 + sg.n;
+    for (uint32_t it = it0 + ((warp - it0) & (kConsumerWarps - 1)); it < it1; it += kConsumerWarps) {
       const int s = it % C::kStages;
       const uint32_t ph = (it / C::kStages) & 1u;
       if (!flags[0] && !mbar_wait(&full[s], ph, p.a.error)) flags[0] = 1;
       __syncwarp();
-      const int at = meta[s * 4 + warp];  // the position of this warp's first token
-      if (at <= w.hi && at + 15 >= w.lo && !flags[0]) {
-        uint8_t* kst = stages + s * C::kStageBytes;
-        uint8_t* vst = kst + C::kTileBytes;
-        const int tok0 = warp * 16;
-        const bool whole = at >= w.lo && at + 15 <= w.hi;
+      uint8_t* kst = stages + s * C::kStageBytes;
+      uint8_t* vst = kst + C::kTileBytes;
+      int at[kGroups];
+      bool whole = !flags[0], any = false;
+#pragma unroll
+      for (int u = 0; u < kGroups; ++u) {
+        at[u] = meta[s * 4 + u];
+        whole = whole && at[u] >= w.lo && at[u] + 15 <= w.hi;
+        any = any || (at[u] <= w.hi && at[u] + 15 >= w.lo);
+      }
+      whole = __all_sync(0xffffffffu, whole);
+      if (__all_sync(0xffffffffu, any && !flags[0])) {
         if (!whole) {
-          // Slots outside the range may hold anything: their weights are 0,
-          // and their values must be finite for 0 v to be 0.
-          for (int i = lane; i < 16 * C::kHalves * 8; i += 32) {
-            const int r = i / (C::kHalves * 8);
-            if (at + r < w.lo || at + r > w.hi)
-              *reinterpret_cast<uint4*>(vst + (tok0 * C::kHalves) * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+          // Slots outside the range, and pieces that were not loaded, may hold
+          // anything: their weights are 0, and their values must be finite for
+          // 0 v to be 0.
+          for (int i = lane; i < C::kTile * C::kHalves * 8; i += 32) {
+            const int r = i / (C::kHalves * 8), tok = meta[s * 4 + r / 16] + r % 16;
+            if (tok < w.lo || tok > w.hi) *reinterpret_cast<uint4*>(vst + i * 16) = make_uint4(0, 0, 0, 0);
           }
           __syncwarp();
         }
-        // S = Q K^T over this warp's 16 tokens
-        float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        // S^T = K Q^T: tokens g8 and g8 + 8 of each group, columns 2 t4 and 2 t4 + 1
+        float x[kGroups][kNt][4];
         const uint32_t kbase = smem_u32(kst);
 #pragma unroll
+        for (int u = 0; u < kGroups; ++u) {
+#pragma unroll
+          for (int nt = 0; nt < kNt; ++nt) x[u][nt][0] = x[u][nt][1] = x[u][nt][2] = x[u][nt][3] = 0.f;
+        }
+#pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const int tok = tok0 + (lane & 7) + ((lane >> 4) << 3);
-          const int chunk = 2 * kk + ((lane >> 3) & 1);
-          uint32_t r0, r1, r2, r3;
-          ldsm_x4(kbase + sw128(tok * C::kHalves + (chunk >> 3), chunk & 7), r0, r1, r2, r3);
-          mma_t<CT>(acc[0], qa[kk], r0, r1);
-          mma_t<CT>(acc[1], qa[kk], r2, r3);
-          if constexpr (SPLIT) {
-            mma_t<CT>(acc[0], ql[kk], r0, r1);
-            mma_t<CT>(acc[1], ql[kk], r2, r3);
+          const int chunk = 2 * kk + (lane >> 4);
+#pragma unroll
+          for (int u = 0; u < kGroups; ++u) {
+            const int tok = u * 16 + frag_row;
+            uint32_t a[4];
+            ldsm_x4(kbase + sw128(tok * C::kHalves + (chunk >> 3), chunk & 7), a[0], a[1], a[2], a[3]);
+#pragma unroll
+            for (int nt = 0; nt < kNt; ++nt) {
+              mma_t<CT>(x[u][nt], a, qb[nt][kk][0], qb[nt][kk][1]);
+              if constexpr (SPLIT) mma_t<CT>(x[u][nt], a, ql[nt][kk][0], ql[nt][kk][1]);
+            }
           }
         }
         // mask + online softmax (log2 domain)
-        float x[2][4];
+        uint32_t pb[kGroups][kNt][2], pl[SPLIT ? kGroups : 1][kNt][2];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int nt = 0; nt < kNt; ++nt) {
+          float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int tok = at + nt * 8 + 2 * t4 + (e & 1);
-            const float v = acc[nt][e] * (e < 2 ? scale0 : scale1);
-            x[nt][e] = whole || (tok >= w.lo && tok <= w.hi) ? v : -INFINITY;
+          for (int u = 0; u < kGroups; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int tok = at[u] + g8 + (e >> 1) * 8;
+              const float v = x[u][nt][e] * scale[nt][e & 1];
+              x[u][nt][e] = whole || (tok >= w.lo && tok <= w.hi) ? v : -INFINITY;
+              top[e & 1] = fmaxf(top[e & 1], x[u][nt][e]);
+            }
+          float base[2], keep[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
+            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
+            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
+            top[e] = fmaxf(top[e], m[nt][e]);
+            base[e] = top[e] == -INFINITY ? 0.f : top[e];
+            keep[e] = ex2(m[nt][e] - base[e]);
+            m[nt][e] = top[e];
+            l[nt][e] *= keep[e];
           }
-        float mt0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-        mt0 = fmaxf(mt0, __shfl_xor_sync(0xffffffffu, mt0, 1));
-        mt0 = fmaxf(mt0, __shfl_xor_sync(0xffffffffu, mt0, 2));
-        const float mn0 = fmaxf(m0, mt0);
-        const float mu0 = mn0 == -INFINITY ? 0.f : mn0;
-        const float al0 = ex2(m0 - mu0);
-        m0 = mn0;
-        float pr[2][4];
-        pr[0][0] = ex2(x[0][0] - mu0);
-        pr[0][1] = ex2(x[0][1] - mu0);
-        pr[1][0] = ex2(x[1][0] - mu0);
-        pr[1][1] = ex2(x[1][1] - mu0);
-        l0 = l0 * al0 + (pr[0][0] + pr[0][1]) + (pr[1][0] + pr[1][1]);
-        float al1 = 1.f;
-        if (TWO) {
-          float mt1 = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
-          mt1 = fmaxf(mt1, __shfl_xor_sync(0xffffffffu, mt1, 1));
-          mt1 = fmaxf(mt1, __shfl_xor_sync(0xffffffffu, mt1, 2));
-          const float mn1 = fmaxf(m1, mt1);
-          const float mu1 = mn1 == -INFINITY ? 0.f : mn1;
-          al1 = ex2(m1 - mu1);
-          m1 = mn1;
-          pr[0][2] = ex2(x[0][2] - mu1);
-          pr[0][3] = ex2(x[0][3] - mu1);
-          pr[1][2] = ex2(x[1][2] - mu1);
-          pr[1][3] = ex2(x[1][3] - mu1);
-          l1 = l1 * al1 + (pr[0][2] + pr[0][3]) + (pr[1][2] + pr[1][3]);
-        }
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          o[i][0] *= al0;
-          o[i][1] *= al0;
-          if (TWO) {
-            o[i][2] *= al1;
-            o[i][3] *= al1;
+          for (int u = 0; u < kGroups; ++u) {
+            float pr[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              pr[e] = ex2(x[u][nt][e] - base[e & 1]);
+              l[nt][e & 1] += pr[e];
+            }
+            // P rounded to the pages' type: its products with V then run on
+            // the tensor cores (SPLIT keeps the rest as a second operand)
+            const uint32_t p0 = pack2<CT>(pr[0], pr[1]), p1 = pack2<CT>(pr[2], pr[3]);
+            pb[u][nt][0] = transpose8(p0);
+            pb[u][nt][1] = transpose8(p1);
+            if constexpr (SPLIT) {
+              pl[u][nt][0] = transpose8(pack_rest(p0, pr[0], pr[1]));
+              pl[u][nt][1] = transpose8(pack_rest(p1, pr[2], pr[3]));
+            }
           }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nt][i][e] *= keep[e & 1];
         }
-        // P rounded to the pages' type: its products with V then run on the
-        // tensor cores (SPLIT keeps the rest as a second operand)
-        uint32_t pa[4], pl[4];
-        pa[0] = pack2<CT>(pr[0][0], pr[0][1]);
-        pa[1] = TWO ? pack2<CT>(pr[0][2], pr[0][3]) : 0u;
-        pa[2] = pack2<CT>(pr[1][0], pr[1][1]);
-        pa[3] = TWO ? pack2<CT>(pr[1][2], pr[1][3]) : 0u;
-        if constexpr (SPLIT) {
-          pl[0] = pack_rest(pa[0], pr[0][0], pr[0][1]);
-          pl[1] = TWO ? pack_rest(pa[1], pr[0][2], pr[0][3]) : 0u;
-          pl[2] = pack_rest(pa[2], pr[1][0], pr[1][1]);
-          pl[3] = TWO ? pack_rest(pa[3], pr[1][2], pr[1][3]) : 0u;
-        }
-        // O += P V
+        // O^T += V^T P^T: dimensions g8 and g8 + 8 of each 16
         const uint32_t vbase = smem_u32(vst);
 #pragma unroll
-        for (int dd = 0; dd < D / 16; ++dd) {
-          const int tok = tok0 + (lane & 7) + (((lane >> 3) & 1) << 3);
-          const int chunk = 2 * dd + (lane >> 4);
-          uint32_t r0, r1, r2, r3;
-          ldsm_x4_t(vbase + sw128(tok * C::kHalves + (chunk >> 3), chunk & 7), r0, r1, r2, r3);
-          mma_t<CT>(o[2 * dd], pa, r0, r1);
-          mma_t<CT>(o[2 * dd + 1], pa, r2, r3);
-          if constexpr (SPLIT) {
-            mma_t<CT>(o[2 * dd], pl, r0, r1);
-            mma_t<CT>(o[2 * dd + 1], pl, r2, r3);
+        for (int u = 0; u < kGroups; ++u) {
+          const int tok = u * 16 + vfrag_row;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            const int chunk = 2 * i + ((lane >> 3) & 1);
+            uint32_t a[4];
+            ldsm_x4_t(vbase + sw128(tok * C::kHalves + (chunk >> 3), chunk & 7), a[0], a[1], a[2], a[3]);
+#pragma unroll
+            for (int nt = 0; nt < kNt; ++nt) {
+              mma_t<CT>(o[nt][i], a, pb[u][nt][0], pb[u][nt][1]);
+              if constexpr (SPLIT) mma_t<CT>(o[nt][i], a, pl[u][nt][0], pl[u][nt][1]);
+            }
           }
         }
         if (!whole) fence_proxy_async_smem();  // the zeros before the next TMA into this stage
@@ -552,35 +603,32 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
     }
+    it0 = it1;
 
     // ---- join the 4 warps' (m, l, O)
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    if (TWO) {
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    }
     float* rw = red + warp * rows * (D + 2);
-    if (g_row < heads) {
-      float* rr = rw + g_row * (D + 2);
-      if (t4 == 0) {
-        rr[0] = m0;
-        rr[1] = l0;
-      }
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-        *reinterpret_cast<float2*>(rr + 2 + i * 8 + 2 * t4) = make_float2(o[i][0], o[i][1]);
-    }
-    if (TWO && g_row + 8 < heads) {
-      float* rr = rw + (g_row + 8) * (D + 2);
-      if (t4 == 0) {
-        rr[0] = m1;
-        rr[1] = l1;
-      }
+    for (int nt = 0; nt < kNt; ++nt)
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-        *reinterpret_cast<float2*>(rr + 2 + i * 8 + 2 * t4) = make_float2(o[i][2], o[i][3]);
-    }
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nt][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int r = nt * 8 + 2 * t4 + e;
+        if (r < heads) {
+          float* rr = rw + r * (D + 2);
+          if (g8 == 0) {
+            rr[0] = m[nt][e];
+            rr[1] = sum;
+          }
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            rr[2 + i * 16 + g8] = o[nt][i][e];
+            rr[2 + i * 16 + 8 + g8] = o[nt][i][2 + e];
+          }
+        }
+      }
     named_barrier_sync(1, 128);
     const bool whole = sg.lt == 0 && sg.n == sg.tiles;
     float* mine = d.scratch + (static_cast<size_t>(cta) * 2 + (g == tb ? 0 : 1)) * rows * (D + 2);
@@ -747,7 +795,8 @@ cudaError_t launch_d(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
 bool make_pool_map(const tla_paged* P, void* base, CUtensorMap* map) {
   const tla_page_pool& pool = P->pool;
   const cuuint64_t halves = static_cast<cuuint64_t>(P->base.D / 64);
-  const cuuint32_t box_slots = pool.page_size < kTile ? pool.page_size : kTile;
+  const int tile = P->base.D == 64 ? Cfg<64>::kTile : Cfg<128>::kTile;
+  const cuuint32_t box_slots = pool.page_size < tile ? pool.page_size : tile;
   const cuuint64_t dims[5] = {64, halves, static_cast<cuuint64_t>(pool.page_size), static_cast<cuuint64_t>(P->base.Hk),
                               static_cast<cuuint64_t>(pool.page_count)};
   const cuuint64_t strides[4] = {128, static_cast<cuuint64_t>(pool.slot_stride) * 2,
@@ -788,6 +837,7 @@ void paged_decode_configure(tla_paged* P) {
 
 // The most tiles that a pair of this call can have.
 long long most_tiles(const PagedArgs& p, int count) {
+  const int kTile = p.a.D == 64 ? Cfg<64>::kTile : Cfg<128>::kTile;
   long long tokens = p.capacity, tiles = (tokens + kTile - 1) / kTile;
   if (count > 0) {
     const long long listed = ((static_cast<long long>(count) << p.page_shift) + kTile - 1) / kTile;
