@@ -5,20 +5,23 @@
 //
 // Each K and V element is read once and used by the group's query heads, about
 // 2 G operations per byte: memory bounds it, so the kernel's shape follows the
-// reads. A (sequence, kv head) pair's tokens are cut into tiles (64 tokens at
-// head_dim 64, 32 at 128: 16 KB of K and V), and the tiles of all pairs into
+// reads. A (sequence, kv head) pair's tokens are cut into tiles (8 KB of K and
+// V: 32 tokens at head_dim 64, 16 at 128), and the tiles of all pairs into
 // equal contiguous shares, one per resident CTA, whatever the sequences'
-// lengths; a share may begin and end inside a pair. A producer warp walks the
-// share's pages: its lanes look up 32 table entries at a time, one window
-// ahead, and start one TMA box per page piece of a tile (five-dimensional
-// tensor maps: any order and padding of pages, heads and slots, as long as the
-// strides are multiples of 16 bytes) into a ring of stages. Four consumer warps
-// take the tiles in turn, each a whole tile by itself, so that a tile's chain
-// of products, maximum, exponentials and products again is four deep in flight
-// per CTA and needs no barrier between warps. 16 tokens always lie in one
-// page: a page's end inside a tile, a page that is not in the pool and the
-// window's edges are decided per 16 tokens from their first position, which
-// the producer leaves beside the stage.
+// lengths; a share may begin and end inside a pair. Four warps take a share's
+// tiles in turn, each by itself: a warp keeps a ring of tiles of its own, which
+// its lanes fill by asynchronous 16-byte copies (any order, padding and stride
+// of pages, heads and slots), so that no barrier, no producer and no other
+// warp's tile stands between its reads. Its page table entries are looked up
+// 32 at a time, one window ahead, and its copies run ahead of its products
+// across the ends of sequences. 16 tokens always lie in one page: a page's end
+// inside a tile, a page that is not in the pool and the window's edges are
+// decided when a row is copied, as zeros in place of it.
+//
+// (A version with a producer warp and one TMA box per page piece moved the
+// same bytes per second when every SM streams, but a tile took one CTA 0.43 us
+// at 64-token pages and 0.7 us at 16: the issue of up to 8 boxes per tile and
+// the round trip of a stage bound it.)
 //
 // S^T = K Q^T and O^T += V^T P^T run as m16n8k16 tensor-core tiles: the tokens
 // (then the dimensions) are the 16 rows and the group's query heads the 8
@@ -40,38 +43,44 @@
 
 #include "paged.cuh"
 
+#ifndef CTAS
+#define CTAS 2
+#endif
+#ifndef TILE64
+#define TILE64 32
+#endif
+#ifndef TILE128
+#define TILE128 16
+#endif
+#ifndef STG64
+#define STG64 3
+#endif
+#ifndef STG128
+#define STG128 3
+#endif
+#ifndef SETUP64
+#define SETUP64 8
+#endif
+#ifndef SETUP128
+#define SETUP128 8
+#endif
 namespace tla {
 
 namespace {
 
-constexpr int kConsumerWarps = 4;
-constexpr int kThreads = (kConsumerWarps + 1) * 32;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
 constexpr int kMaxBatch = 1024;  // prefix table in shared memory
-constexpr int kCtasPerSm = 2;
+constexpr int kCtasPerSm = CTAS;
 constexpr int kMaxGrid = 1024;   // segment table of the joining kernel
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNowhere = -(1 << 30);  // first position of 16 tokens that take no part
 
-#ifndef STG
-#define STG 4
-#endif
-#ifndef TILE64
-#define TILE64 64
-#endif
-#ifndef TILE128
-#define TILE128 32
-#endif
-#ifndef SETUP64
-#define SETUP64 4
-#endif
-#ifndef SETUP128
-#define SETUP128 4
-#endif
 template <int D>
 struct Cfg {
   static constexpr int kTile = D == 64 ? TILE64 : TILE128;
   static constexpr int kGroups = kTile / 16;
-  static constexpr int kStages = STG;      // a multiple of the consumer warps: a stage is always the same warp's
+  static constexpr int kStages = D == 64 ? STG64 : STG128;
   static constexpr int kHalves = D / 64;  // 128-byte rows per cache row
   static constexpr int kTileBytes = kTile * kHalves * 128;
   static constexpr int kStageBytes = 2 * kTileBytes;
@@ -82,8 +91,6 @@ struct Cfg {
 };
 
 struct DecodeParams {
-  CUtensorMap tmap_k;
-  CUtensorMap tmap_v;
   PagedArgs p;
   const void* query;
   const int32_t* pages;  // null, or [batch][Hk][count]
@@ -98,7 +105,7 @@ struct DecodeParams {
 };
 
 struct SmemLayout {
-  int stages, q, red, meta, prefix, bars, flags, total;
+  int stages, q, red, meta, prefix, total;
 };
 template <int D>
 __host__ __device__ inline SmemLayout smem_layout(int rows, int batch, bool split) {
@@ -106,21 +113,16 @@ __host__ __device__ inline SmemLayout smem_layout(int rows, int batch, bool spli
   SmemLayout s;
   int off = 0;
   s.stages = off;
-  off += C::kStages * C::kStageBytes;
+  off += kWarps * C::kStages * C::kStageBytes;
   s.q = off;
   off += (split ? 2 : 1) * 16 * C::kQPitch;
   s.red = off;
-  off += kConsumerWarps * rows * (D + 2) * 4;
+  off += kWarps * rows * (D + 2) * 4;
   off = (off + 15) & ~15;
   s.meta = off;
-  off += C::kStages * 16;
+  off += kWarps * C::kStages * C::kGroups * 4;
   s.prefix = off;
   off += (2 * batch + 2) * 4;  // unit prefix, then positions
-  off = (off + 7) & ~7;
-  s.bars = off;
-  off += 2 * C::kStages * 8;
-  s.flags = off;
-  off += 16;
   s.total = off + 1024;  // alignment slack
   return s;
 }
@@ -221,13 +223,14 @@ __device__ __forceinline__ int next_pair(const int* prefix, int batch, int pairs
   return prefix[b] + (g - prefix[b] + per - 1) / per * per;
 }
 
-__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int slot, int head,
-                                            int page) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %3, %4, %5}], "
-      "[%6];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
-      : "memory");
+// 16 bytes to shared memory, zeros instead when `bytes` is 0.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 template <typename T>
@@ -280,25 +283,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   const PagedArgs& p = d.p;
   const int Hq = p.a.Hq, G = p.a.G, pairs = p.a.Hk * d.subs, rows = d.rows;
   const SmemLayout L = smem_layout<D>(rows, p.batch, SPLIT);
-  uint8_t* stages = smem + L.stages;
   int* prefix = reinterpret_cast<int*>(smem + L.prefix);
   int* spos = prefix + p.batch + 1;
-  int* meta = reinterpret_cast<int*>(smem + L.meta);  // [stage][4]: first position of each 16 tokens of its tile
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);
-  uint64_t* empty = full + C::kStages;
-  volatile int* flags = reinterpret_cast<volatile int*>(smem + L.flags);  // [0] a wait gave up
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
-  if (tid == 0) {
-    flags[0] = 0;
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    fence_mbar_init();
-    prefix[0] = 0;
-    tma_prefetch(&d.tmap_k);
-    tma_prefetch(&d.tmap_v);
-  }
+  const uint32_t ring = smem_u32(smem + L.stages) + warp * C::kStages * C::kStageBytes;
+  int* meta = reinterpret_cast<int*>(smem + L.meta) + warp * C::kStages * C::kGroups;  // first position of each 16 tokens
+  if (tid == 0) prefix[0] = 0;
   griddep_wait();
   griddep_launch_dependents();
   for (int b = tid; b < p.batch; b += kThreads) {
@@ -326,77 +316,97 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   if (tb >= te) return;
   const int shift = p.page_shift, mask = (1 << shift) - 1;
 
-  if (warp == kConsumerWarps) {
-    // ================================================================ producer
-    constexpr int kTile = C::kTile;
-    const int boxes = max(1, kTile >> shift);  // per tile, K or V
-    const int box_rows = kTile / boxes, box_bytes = C::kTileBytes / boxes;
-    uint32_t it = 0;
-    int b = 0;
-    for (int g = tb; g < te;) {
-      while (prefix[b + 1] <= g) ++b;
-      const Seg sg = seg_at<D>(prefix, b, pairs, g, te);
-      g = sg.next;
-      if (sg.n == 0) continue;
-      const int kvh = sg.pair / d.subs;
-      const Walk w = walk_of<D>(d, spos[b]);
-      const int32_t* list = d.pages ? d.pages + (static_cast<int64_t>(b) * p.a.Hk + kvh) * d.count : nullptr;
-      const int last_page = w.hi >> shift;
-      // entries of the table (or the list) that this share walks
-      const int t_begin = w.first + sg.lt, t_end = t_begin + sg.n;
-      const int e_begin = static_cast<int>((static_cast<int64_t>(t_begin) * kTile) >> shift);
-      int e_end = static_cast<int>((static_cast<int64_t>(t_end) * kTile - 1) >> shift) + 1;
-      e_end = min(e_end, list ? list_length(p, list, min(d.count, last_page + 1), last_page, lane) : last_page + 1);
-      const int e_first = list ? 0 : w.lo >> shift;
-      // a lane's entry of a window of 32: the page's index in the sequence and its place in the pool
-      auto look = [&](int e, int* index, int* page) {
-        const bool in = e >= e_first && e < e_end;
-        *index = !in ? 0 : list ? list[e] : e;
-        *page = in ? pool_page(p, b, *index) : -1;
-      };
-      int base = e_begin, index, page, index_next, page_next;
-      look(base + lane, &index, &page);
-      look(base + 32 + lane, &index_next, &page_next);
-      for (int t = t_begin; t < t_end; ++t, ++it) {
-        const int s = it % C::kStages;
-        const uint32_t ph = (it / C::kStages) & 1u;
-        const int64_t token = static_cast<int64_t>(t) * kTile;
-        const int e = static_cast<int>(token >> shift), offset = static_cast<int>(token) & mask;
-        if (e - base >= 32) {
-          base += 32;
-          index = index_next;
-          page = page_next;
-          look(base + 32 + lane, &index_next, &page_next);
+  // ================================================================== copies
+  // The warp's copies: tiles ld.it = warp, warp + 4, ... of the share, counted
+  // over its segments, each into the ring's next stage.
+  struct {
+    int g, b, it, begin, end;          // the share's tiles [begin, end) are the current segment's
+    int first, lo, hi, e_first, e_end;  // its first tile, range, and table (or list) entries
+    int base, index, page, index_next, page_next;  // windows of 32 entries: a lane's page in the sequence and the pool
+    const int32_t* list;
+    int64_t head;  // the kv head's first element of a page
+  } ld;
+  ld.g = tb;
+  ld.b = 0;
+  ld.it = warp;
+  ld.begin = ld.end = 0;
+  ld.base = 0;
+  ld.list = nullptr;
+  // (entries are only looked at when they are used, so that a window's loads are not waited for)
+  auto look = [&](int e, int* index, int* page) {
+    const bool in = e >= ld.e_first && e < ld.e_end;
+    *index = !in ? 0 : ld.list ? ld.list[e] : e;
+    *page = in ? p.table[static_cast<int64_t>(ld.b) * p.width + *index] : kNowhere;
+  };
+  auto load_next = [&](int stage) {
+    while (ld.it >= ld.end && ld.g < te) {  // on to the segment that holds the tile
+      while (prefix[ld.b + 1] <= ld.g) ++ld.b;
+      const Seg sg = seg_at<D>(prefix, ld.b, pairs, ld.g, te);
+      ld.g = sg.next;
+      ld.begin = ld.end;
+      ld.end += sg.n;
+      if (ld.it >= ld.end) continue;
+      const Walk w = walk_of<D>(d, spos[ld.b]);
+      const int kvh = sg.pair / d.subs, last_page = w.hi >> shift;
+      ld.list = d.pages ? d.pages + (static_cast<int64_t>(ld.b) * p.a.Hk + kvh) * d.count : nullptr;
+      ld.head = kvh * p.head_stride;
+      ld.lo = w.lo;
+      ld.hi = w.hi;
+      ld.first = w.first + sg.lt;
+      ld.e_first = ld.list ? 0 : w.lo >> shift;
+      ld.e_end = min(static_cast<int>((static_cast<int64_t>(ld.first + sg.n) * C::kTile - 1) >> shift) + 1,
+                     ld.list ? list_length(p, ld.list, min(d.count, last_page + 1), last_page, lane) : last_page + 1);
+      ld.base = static_cast<int>((static_cast<int64_t>(ld.first + ld.it - ld.begin) * C::kTile) >> shift);
+      look(ld.base + lane, &ld.index, &ld.page);
+      look(ld.base + 32 + lane, &ld.index_next, &ld.page_next);
+    }
+    if (ld.it < ld.end) {
+      const int64_t token = static_cast<int64_t>(ld.first + ld.it - ld.begin) * C::kTile;
+      const int e = static_cast<int>(token >> shift), offset = static_cast<int>(token) & mask;
+      if (e - ld.base >= 32) {
+        ld.base += 32;
+        ld.index = ld.index_next;
+        ld.page = ld.page_next;
+        look(ld.base + 32 + lane, &ld.index_next, &ld.page_next);
+      }
+      const uint32_t kst = ring + stage * C::kStageBytes;
+      constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes per row, rows per copy
+      const int r0 = lane / kLanes, chunk = lane % kLanes;
+#pragma unroll
+      for (int u = 0; u < C::kGroups; ++u) {
+        const int piece = (offset + u * 16) >> shift;  // pages of under a tile: the group's page within the tile
+        const int index = __shfl_sync(0xffffffffu, ld.index, e - ld.base + piece);
+        int page = __shfl_sync(0xffffffffu, ld.page, e - ld.base + piece);
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.page_count)) {
+          if (page != kNowhere) report_error(p.a.error, TLA_ERR_PAGE);
+          page = -1;
         }
-        const int piece = lane % boxes;  // lanes 0..boxes-1 load K, the next V
-        const int my_page = __shfl_sync(0xffffffffu, page, e - base + piece);
-        const int group_piece = lane * 16 / box_rows;  // first lanes: the tile's groups of 16 tokens
-        const int g_index = __shfl_sync(0xffffffffu, index, e - base + (lane < C::kGroups ? group_piece : 0));
-        const int g_page = __shfl_sync(0xffffffffu, page, e - base + (lane < C::kGroups ? group_piece : 0));
-        const int loaded = __popc(__ballot_sync(0xffffffffu, lane < boxes && my_page >= 0));
-        const bool go = !flags[0] && mbar_wait(&empty[s], ph ^ 1u, p.a.error);
-        if (__any_sync(0xffffffffu, !go)) {
-          flags[0] = 1;
-          continue;
+        const int slot = (offset + u * 16) & mask;
+        const int at = page < 0 ? kNowhere : (index << shift) + slot;
+        if (lane == 0) meta[stage * C::kGroups + u] = at;
+        const int64_t from = page < 0 ? 0 : page * p.page_stride + ld.head + (slot + r0) * p.slot_stride + chunk * 8;
+        const CT* k = static_cast<const CT*>(p.key) + from;
+        const CT* v = static_cast<const CT*>(p.value) + from;
+        const int64_t step = page < 0 ? 0 : kRows * p.slot_stride;
+#pragma unroll
+        for (int i = 0; i < 16 / kRows; ++i) {
+          const int r = r0 + i * kRows;
+          const int bytes = at + r >= ld.lo && at + r <= ld.hi ? 16 : 0;
+          const uint32_t dst = kst + sw128((u * 16 + r) * C::kHalves + (chunk >> 3), chunk & 7);
+          copy16(dst, k, bytes);
+          copy16(dst + C::kTileBytes, v, bytes);
+          k += step;
+          v += step;
         }
-        if (lane < C::kGroups)
-          meta[s * 4 + lane] = g_page < 0 ? kNowhere : (g_index << shift) + offset + lane * 16 - group_piece * box_rows;
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], 2 * loaded * box_bytes);
-        __syncwarp();
-        if (lane < 2 * boxes && my_page >= 0)
-          tma_load_5d(stages + s * C::kStageBytes + (lane < boxes ? 0 : C::kTileBytes) + piece * box_bytes,
-                      lane < boxes ? &d.tmap_k : &d.tmap_v, &full[s], offset, kvh, my_page);
       }
     }
-    // Do not leave the CTA with copies in flight.
-    const uint32_t first = it > static_cast<uint32_t>(C::kStages) ? it - C::kStages : 0u;
-    for (uint32_t i = first; i < it; ++i)
-      if (!flags[0]) mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1u, p.a.error);
-    return;
-  }
+    copies_commit();
+    ld.it += kWarps;
+  };
+#pragma unroll
+  for (int s = 0; s < C::kStages; ++s) load_next(s);
 
-  // ================================================================== consumers
+  // ================================================================== products
   CT* q_s = reinterpret_cast<CT*>(smem + L.q);
   float* red = reinterpret_cast<float*>(smem + L.red);
   constexpr int kNt = TWO ? 2 : 1;  // column tiles of 8 query heads
@@ -404,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   const int g8 = lane >> 2, t4 = lane & 3;
   const int frag_row = (lane & 7) + ((lane >> 3) & 1) * 8;   // K as the left operand: token rows, then dimensions
   const int vfrag_row = (lane & 7) + (lane >> 4) * 8;        // V transposed: its tokens are the columns
-  uint32_t it0 = 0;  // the share's tiles before this segment
+  int it0 = 0, stage = 0;  // the share's tiles before this segment; the ring's oldest tile
   int b = 0;
   for (int g = tb; g < te;) {
     while (prefix[b + 1] <= g) ++b;
@@ -419,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     const IO* q = static_cast<const IO*>(d.query) + (static_cast<int64_t>(b) * Hq + h0) * D;
     // ---- the group's queries, 8 elements per thread and trip; rows past the group are zeros
     if constexpr (SPLIT) {
-      for (int r = warp; r < 8 * kNt; r += kConsumerWarps) {
+      for (int r = warp; r < 8 * kNt; r += kWarps) {
         float x[D / 32], top = 0.f;
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) {
@@ -449,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         *reinterpret_cast<uint4*>(q_s + r * (C::kQPitch / 2) + c * 8) = v;
       }
     }
-    named_barrier_sync(1, 128);
+    __syncthreads();
     uint32_t qb[kNt][D / 16][2];
     uint32_t ql[kNt][SPLIT ? D / 16 : 1][2];
     float scale[kNt][2];
@@ -481,37 +491,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     }
 
     // ---- this warp's tiles of the segment
-    const uint32_t it1 = it0 + sg.n;
-    for (uint32_t it = it0 + ((warp - it0) & (kConsumerWarps - 1)); it < it1; it += kConsumerWarps) {
-      const int s = it % C::kStages;
-      const uint32_t ph = (it / C::kStages) & 1u;
-      if (!flags[0] && !mbar_wait(&full[s], ph, p.a.error)) flags[0] = 1;
+    const int it1 = it0 + sg.n;
+    for (int it = it0 + ((warp - it0) & (kWarps - 1)); it < it1; it += kWarps) {
+      copies_wait<C::kStages - 1>();
       __syncwarp();
-      uint8_t* kst = stages + s * C::kStageBytes;
-      uint8_t* vst = kst + C::kTileBytes;
       int at[kGroups];
-      bool whole = !flags[0], any = false;
+      bool whole = true, any = false;
 #pragma unroll
       for (int u = 0; u < kGroups; ++u) {
-        at[u] = meta[s * 4 + u];
+        at[u] = meta[stage * kGroups + u];
         whole = whole && at[u] >= w.lo && at[u] + 15 <= w.hi;
         any = any || (at[u] <= w.hi && at[u] + 15 >= w.lo);
       }
-      whole = __all_sync(0xffffffffu, whole);
-      if (__all_sync(0xffffffffu, any && !flags[0])) {
-        if (!whole) {
-          // Slots outside the range, and pieces that were not loaded, may hold
-          // anything: their weights are 0, and their values must be finite for
-          // 0 v to be 0.
-          for (int i = lane; i < C::kTile * C::kHalves * 8; i += 32) {
-            const int r = i / (C::kHalves * 8), tok = meta[s * 4 + r / 16] + r % 16;
-            if (tok < w.lo || tok > w.hi) *reinterpret_cast<uint4*>(vst + i * 16) = make_uint4(0, 0, 0, 0);
-          }
-          __syncwarp();
-        }
+      if (any) {  // (the same for the whole warp)
         // S^T = K Q^T: tokens g8 and g8 + 8 of each group, columns 2 t4 and 2 t4 + 1
         float x[kGroups][kNt][4];
-        const uint32_t kbase = smem_u32(kst);
+        const uint32_t kbase = ring + stage * C::kStageBytes;
 #pragma unroll
         for (int u = 0; u < kGroups; ++u) {
 #pragma unroll
@@ -582,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
             for (int e = 0; e < 4; ++e) o[nt][i][e] *= keep[e & 1];
         }
         // O^T += V^T P^T: dimensions g8 and g8 + 8 of each 16
-        const uint32_t vbase = smem_u32(vst);
+        const uint32_t vbase = kbase + C::kTileBytes;
 #pragma unroll
         for (int u = 0; u < kGroups; ++u) {
           const int tok = u * 16 + vfrag_row;
@@ -598,10 +593,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
             }
           }
         }
-        if (!whole) fence_proxy_async_smem();  // the zeros before the next TMA into this stage
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
+      load_next(stage);
+      stage = stage + 1 == C::kStages ? 0 : stage + 1;
     }
     it0 = it1;
 
@@ -629,17 +624,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
           }
         }
       }
-    named_barrier_sync(1, 128);
+    __syncthreads();
     const bool whole = sg.lt == 0 && sg.n == sg.tiles;
     float* mine = d.scratch + (static_cast<size_t>(cta) * 2 + (g == tb ? 0 : 1)) * rows * (D + 2);
     for (int i = tid; i < heads * D; i += 128) {
       const int r = i / D, c = i - r * D;
       float top = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll
-      for (int k = 0; k < kConsumerWarps; ++k) top = fmaxf(top, red[(k * rows + r) * (D + 2)]);
+      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, red[(k * rows + r) * (D + 2)]);
       if (top != -INFINITY) {
 #pragma unroll
-        for (int k = 0; k < kConsumerWarps; ++k) {
+        for (int k = 0; k < kWarps; ++k) {
           const float* rr = red + (k * rows + r) * (D + 2);
           const float f = ex2(rr[0] - top);
           sum += rr[1] * f;
@@ -656,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         }
       }
     }
-    named_barrier_sync(1, 128);  // red and q_s are free for the next segment
+    __syncthreads();  // red and q_s are free for the next segment
     g = sg.next;
   }
 }
@@ -772,7 +767,8 @@ cudaError_t launch_t(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   // two CTAs per SM by registers (the launch bounds), if shared memory holds
   // two (228 KB, 1 KB of it reserved per CTA)
-  const int per_sm = kCtasPerSm * (smem + 1024) <= 228 * 1024 ? kCtasPerSm : 1;
+  int per_sm = 228 * 1024 / (smem + 1024);
+  per_sm = per_sm < kCtasPerSm ? per_sm : kCtasPerSm;
   const int grid = per_sm * P->base.ctx->sm_count;
   d.small_grid = P->base.ctx->sm_count;
   e = launch_pdl(kernel, grid, kThreads, smem, stream, d);
@@ -792,25 +788,6 @@ cudaError_t launch_d(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   return two ? launch_t<D, __half, false, true>(P, d, stream) : launch_t<D, __half, false, false>(P, d, stream);
 }
 
-bool make_pool_map(const tla_paged* P, void* base, CUtensorMap* map) {
-  const tla_page_pool& pool = P->pool;
-  const cuuint64_t halves = static_cast<cuuint64_t>(P->base.D / 64);
-  const int tile = P->base.D == 64 ? Cfg<64>::kTile : Cfg<128>::kTile;
-  const cuuint32_t box_slots = pool.page_size < tile ? pool.page_size : tile;
-  const cuuint64_t dims[5] = {64, halves, static_cast<cuuint64_t>(pool.page_size), static_cast<cuuint64_t>(P->base.Hk),
-                              static_cast<cuuint64_t>(pool.page_count)};
-  const cuuint64_t strides[4] = {128, static_cast<cuuint64_t>(pool.slot_stride) * 2,
-                                 static_cast<cuuint64_t>(pool.head_stride) * 2,
-                                 static_cast<cuuint64_t>(pool.page_stride) * 2};
-  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(halves), box_slots, 1, 1};
-  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  return P->base.ctx->encode_tiled(map,
-                                   P->kept == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                                   5, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 int subgroups(const tla_paged* P) { return (P->base.G + 15) / 16; }
 int subgroup_rows(const tla_paged* P) {
   const int s = subgroups(P);
@@ -819,20 +796,13 @@ int subgroup_rows(const tla_paged* P) {
 
 }  // namespace
 
-// The tensor-core path takes 16-bit pages of 16 tokens and up (a warp's 16
-// tokens lie in one page), head_dim 64 or 128 and pools that a tensor map can
-// describe; float32 activations only over float16 pages (two bfloat16 parts
-// would carry 16 bits).
+// The tensor-core path takes 16-bit pages of 16 tokens and up (16 tokens lie in
+// one page), head_dim 64 or 128 and pools with rows on 16-byte boundaries;
+// float32 activations only over float16 pages (two bfloat16 parts would carry
+// 16 bits).
 void paged_decode_configure(tla_paged* P) {
-  const tla_page_pool& pool = P->pool;
-  P->fast = false;
-  if (!P->wide || P->kept == kFp32 || (P->io == kFp32 && P->kept != kFp16) || pool.page_size < 16 || P->base.ctx->encode_tiled == nullptr ||
-      kCtasPerSm * P->base.ctx->sm_count > kMaxGrid)
-    return;
-  tla_paged q = *P;
-  if (pool.page_count == 1) q.pool.page_stride = P->base.D;
-  if (P->base.Hk == 1) q.pool.head_stride = P->base.D;
-  P->fast = make_pool_map(&q, pool.key, &P->tmap_k) && make_pool_map(&q, pool.value, &P->tmap_v);
+  P->fast = P->wide && P->kept != kFp32 && (P->io != kFp32 || P->kept == kFp16) && P->pool.page_size >= 16 &&
+            kCtasPerSm * P->base.ctx->sm_count <= kMaxGrid;
 }
 
 // The most tiles that a pair of this call can have.
@@ -870,8 +840,6 @@ size_t paged_decode_workspace(const tla_paged* P, const PagedArgs& p, int count)
 cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const void* query, const int32_t* pages,
                                 int count, const void* gate, void* out, void* workspace, cudaStream_t stream) {
   DecodeParams d;
-  d.tmap_k = P->tmap_k;
-  d.tmap_v = P->tmap_v;
   d.p = p;
   d.query = query;
   d.pages = pages;

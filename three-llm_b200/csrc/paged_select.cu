@@ -23,7 +23,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxHeld = 48 * 1024;  // ranks that one block's shared memory holds
-constexpr int kScorePages = 256;     // pages per block of the scoring kernel for longer sequences
+constexpr int kScorePages = 32 * kWarps;  // pages per block of the scoring kernel for longer sequences
 
 // Larger scores have larger keys, and every score a key above 0.
 __device__ __forceinline__ uint32_t rank_of(float s) {
@@ -45,74 +45,123 @@ __device__ __forceinline__ PageRange page_range(const PagedArgs& p, int pos) {
 template <typename IO>
 __device__ __forceinline__ void form_vector(const PagedArgs& p, const IO* query, int b, int kvh, double* vec) {
   const int D = p.a.D, G = p.a.G;
+  const IO* q = query + (static_cast<int64_t>(b) * p.a.Hq + kvh * G) * D;
   for (int d = threadIdx.x; d < D; d += kThreads) {
     double neg = 0, pos = 0;
+#pragma unroll 4
     for (int g = 0; g < G; ++g) {
-      const float q = to_f32(query[(static_cast<int64_t>(b) * p.a.Hq + kvh * G + g) * D + d]);
-      neg += fminf(q, 0.f);
-      pos += fmaxf(q, 0.f);
+      const float x = to_f32(q[g * D + d]);
+      neg += fminf(x, 0.f);
+      pos += fmaxf(x, 0.f);
     }
     vec[d] = neg;
     vec[D + d] = pos;
   }
 }
 
-// Ranks of pages [from, to) of a pair, handed to `put(i, rank)` by one lane
-// each. A warp takes 32 pages at a time: its lanes look up their pages, then
-// each page's bounds are read across the warp, kAhead pages in flight.
-template <typename CT, typename Put>
-__device__ __forceinline__ void score_pages(const PagedArgs& p, const double* vec, int b, int kvh, PageRange r,
-                                            int first, int last, int from, int to, const Put& put) {
+// 16 bytes of bounds times their part of the vector.
+template <typename CT>
+__device__ __forceinline__ double dot16(uint4 u, const double* v) {
+  constexpr int kVec = 16 / sizeof(CT);
+  const CT* x = reinterpret_cast<const CT*>(&u);
+  double s0 = 0, s1 = 0;
+#pragma unroll
+  for (int e = 0; e < kVec; e += 2) {
+    s0 = fma(v[e], static_cast<double>(to_f32(x[e])), s0);
+    s1 = fma(v[e + 1], static_cast<double>(to_f32(x[e + 1])), s1);
+  }
+  return s0 + s1;
+}
+
+// A lane's page of a warp that takes pages first, first + step, ... of a
+// sequence: the lane-th of them. Their table entries may be looked up before
+// the range is known (`index` below the table's width).
+__device__ __forceinline__ int raw_page(const PagedArgs& p, int b, int64_t index) {
+  return index < p.width ? p.table[static_cast<int64_t>(b) * p.width + index] : -1;
+}
+
+// Ranks of 32 pages of a pair (i = from + step * lane, raw: their table
+// entries), handed to `put(i, rank)` by their lanes. Each page's bounds are
+// read across the lanes, kAhead reads in flight; kD is head_dim, or 0 for any.
+template <typename CT, int kD, typename Put>
+__device__ __forceinline__ void score_32(const PagedArgs& p, const double* vec, int kvh, PageRange r, int first,
+                                         int last, int from, int step, int raw, const Put& put) {
   const unsigned full = 0xffffffffu;
-  const int D = p.a.D, Hk = p.a.Hk, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int base = from + warp * 32; base < to; base += kThreads) {
-    const int mine = base + lane;
-    const bool always = mine < first || mine >= r.n - last;
-    const int page = mine < to && !always ? pool_page(p, b, r.begin + mine) : -1;
-    uint32_t rank = always ? 0xffffffffu : 0u;  // (a page outside the pool ranks last)
-    const int n = min(32, to - base);
-    auto add = [&](int k, double s) {
+  const int D = p.a.D, lane = threadIdx.x & 31;
+  const int mine = from + step * lane;
+  const bool held = mine < r.n, always = held && (mine < first || mine >= r.n - last);
+  int page = held && !always ? raw : -1;
+  if (page < -1 || page >= p.page_count || (page == -1 && held && !always)) {
+    report_error(p.a.error, TLA_ERR_PAGE);
+    page = -1;
+  }
+  uint32_t rank = always ? 0xffffffffu : 0u;  // (a page outside the pool ranks last)
+  const unsigned scored = __ballot_sync(full, page >= 0);
+  const CT* bounds = static_cast<const CT*>(p.bounds) + static_cast<int64_t>(kvh) * 2 * D;
+  const int64_t stride = static_cast<int64_t>(p.a.Hk) * 2 * D;
+  if constexpr (kD > 0) {
+    constexpr int kVec = 16 / sizeof(CT), kReads = 2 * kD / kVec;        // 16-byte reads per page
+    constexpr int kLanes = kReads < 32 ? kReads : 32, kPer = kReads / kLanes;  // lanes per page, reads per lane
+    constexpr int kPages = 32 / kLanes, kAhead = 8 / kPer;                // pages per warp-wide read; reads in flight
+    const int sub = lane / kLanes, at = lane % kLanes;
+    double v[kPer][kVec];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(full, s, o);
-      if (lane == k && page >= 0) rank = min(rank_of(static_cast<float>(s)), 0xfffffffeu);
-    };
-    const CT* bounds = static_cast<const CT*>(p.bounds) + static_cast<int64_t>(kvh) * 2 * D;
-    const int64_t stride = static_cast<int64_t>(Hk) * 2 * D;
-    if (sizeof(CT) == 2 && D == 128) {  // 8 elements of a page's 256 per lane
-      constexpr int kAhead = 4;
-      double v[8];
+    for (int i = 0; i < kPer; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = vec[lane * 8 + e];
-      for (int k = 0; k < n; k += kAhead) {
-        uint4 u[kAhead];
+      for (int e = 0; e < kVec; ++e) v[i][e] = vec[(i * kLanes + at) * kVec + e];
+    const int n = 32 - __clz(scored);  // (0 when none is scored)
+    for (int k0 = 0; k0 < n; k0 += kAhead * kPages) {
+      uint4 u[kAhead][kPer];
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-          const int at = __shfl_sync(full, page, k + a);
-          u[a] = at < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(bounds + at * stride + lane * 8);
-        }
+      for (int a = 0; a < kAhead; ++a) {
+        const int of = __shfl_sync(full, page, (k0 + a * kPages + sub) & 31);
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) {
-          const CT* x = reinterpret_cast<const CT*>(&u[a]);
-          double s0 = 0, s1 = 0;
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            s0 = fma(v[e], static_cast<double>(to_f32(x[e])), s0);
-            s1 = fma(v[e + 1], static_cast<double>(to_f32(x[e + 1])), s1);
-          }
-          add(k + a, s0 + s1);
-        }
+        for (int i = 0; i < kPer; ++i)
+          u[a][i] = of < 0 || k0 + a * kPages + sub > 31
+                        ? make_uint4(0, 0, 0, 0)
+                        : *reinterpret_cast<const uint4*>(bounds + of * stride + (i * kLanes + at) * kVec);
       }
-    } else {
-      for (int k = 0; k < n; ++k) {
-        const int at = __shfl_sync(full, page, k);
-        double s = 0;
-        if (at >= 0)
-          for (int d = lane; d < 2 * D; d += 32) s = fma(vec[d], static_cast<double>(to_f32(bounds[at * stride + d])), s);
-        add(k, s);
+      double s[kAhead];
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        s[a] = dot16<CT>(u[a][0], v[0]);
+#pragma unroll
+        for (int i = 1; i < kPer; ++i) s[a] += dot16<CT>(u[a][i], v[i]);
+      }
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) s[a] += __shfl_xor_sync(full, s[a], o);
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {  // page k0 + a kPages + j to its lane, from the j-th group of lanes
+#pragma unroll
+        for (int j = 0; j < kPages; ++j) {
+          const double of = kPages == 1 ? s[a] : __shfl_sync(full, s[a], j * kLanes);
+          if (lane == k0 + a * kPages + j && page >= 0) rank = min(rank_of(static_cast<float>(of)), 0xfffffffeu);
+        }
       }
     }
-    if (mine < to) put(mine, rank);
+  } else {
+    for (unsigned left = scored; left != 0; left &= left - 1) {
+      const int k = __ffs(left) - 1, of = __shfl_sync(full, page, k);
+      double s = 0;
+      for (int d = lane; d < 2 * D; d += 32) s = fma(vec[d], static_cast<double>(to_f32(bounds[of * stride + d])), s);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(full, s, o);
+      if (lane == k) rank = min(rank_of(static_cast<float>(s)), 0xfffffffeu);
+    }
   }
+  if (held) put(mine, rank);
+}
+template <typename CT, typename Put>
+__device__ __forceinline__ void score_any(const PagedArgs& p, const double* vec, int kvh, PageRange r, int first,
+                                          int last, int from, int step, int raw, const Put& put) {
+  if (p.a.D == 128)
+    score_32<CT, 128>(p, vec, kvh, r, first, last, from, step, raw, put);
+  else if (p.a.D == 64)
+    score_32<CT, 64>(p, vec, kvh, r, first, last, from, step, raw, put);
+  else
+    score_32<CT, 0>(p, vec, kvh, r, first, last, from, step, raw, put);
 }
 
 // Writes the `count` pages of the highest ranks, ties to the lower page, in
@@ -213,9 +262,10 @@ __device__ __forceinline__ void list_all(const PagedArgs& p, int pos, PageRange 
   for (int i = threadIdx.x; i < count; i += kThreads) out[i] = i < r.n ? r.begin + i : -1;
 }
 
-// A cluster per (sequence, kv head): its blocks score a share of the pages
+// A cluster per (sequence, kv head): its warps score every so many-th page
 // each and leave the ranks in the first block's shared memory, which picks.
-// One launch: what a step waits for here is latency, not the bounds' bytes.
+// One launch: what a step waits for here is latency, not the bounds' bytes, so
+// the position, the query and the first table entries are read side by side.
 template <typename IO, typename CT>
 __global__ void __launch_bounds__(kThreads)
     paged_select_kernel(PagedArgs p, const IO* __restrict__ query, int first, int last, int count,
@@ -228,7 +278,12 @@ __global__ void __launch_bounds__(kThreads)
   cg::cluster_group cluster = cg::this_cluster();
   const int share = cluster.block_rank(), shares = cluster.num_blocks();
   const int pair = blockIdx.x / shares, b = pair / p.a.Hk, kvh = pair - b * p.a.Hk;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int step = kWarps * shares;
+  int from = warp * shares + share;
   const int pos = p.positions[b];
+  int raw = p.a.sliding == 0 ? raw_page(p, b, from + static_cast<int64_t>(step) * lane) : 0;
+  form_vector(p, query, b, kvh, vec);
   const PageRange r = page_range(p, pos);
   int32_t* out = pages_out + static_cast<int64_t>(pair) * count;
   if (r.n <= count) {  // (the same for the whole cluster)
@@ -236,13 +291,15 @@ __global__ void __launch_bounds__(kThreads)
     return;
   }
   // every block of the cluster runs before one writes into another's memory
-  if (shares > 1) cluster.sync();
-  form_vector(p, query, b, kvh, vec);
-  __syncthreads();
+  if (shares > 1)
+    cluster.sync();
+  else
+    __syncthreads();
   uint32_t* held = shares > 1 ? cluster.map_shared_rank(ranks, 0) : ranks;
-  const int per = (r.n + shares - 1) / shares, from = share * per;
-  score_pages<CT>(p, vec, b, kvh, r, first, last, from, min(r.n, from + per),
-                  [&](int i, uint32_t rank) { held[i] = rank; });
+  for (bool again = false; from < r.n; from += 32 * step, again = true) {
+    if (again || p.a.sliding > 0) raw = raw_page(p, b, r.begin + from + static_cast<int64_t>(step) * lane);
+    score_any<CT>(p, vec, kvh, r, first, last, from, step, raw, [&](int i, uint32_t rank) { held[i] = rank; });
+  }
   if (shares > 1)
     cluster.sync();
   else
@@ -259,16 +316,18 @@ __global__ void __launch_bounds__(kThreads)
   extern __shared__ __align__(16) double vec[];
   griddep_wait();
   griddep_launch_dependents();
-  const int kvh = blockIdx.y;
+  const int kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int b = blockIdx.z; b < p.batch; b += gridDim.z) {
     const PageRange r = page_range(p, p.positions[b]);
-    const int from = blockIdx.x * kScorePages, to = min(r.n, from + kScorePages);
-    if (r.n <= count || from >= to) continue;
+    const int from = blockIdx.x * kScorePages + warp * 32;
+    if (r.n <= count || blockIdx.x * kScorePages >= r.n) continue;
     __syncthreads();
     form_vector(p, query, b, kvh, vec);
     __syncthreads();
     uint32_t* held = ranks + (static_cast<int64_t>(b) * p.a.Hk + kvh) * p.width;
-    score_pages<CT>(p, vec, b, kvh, r, first, last, from, to, [&](int i, uint32_t rank) { held[i] = rank; });
+    if (from < r.n)
+      score_any<CT>(p, vec, kvh, r, first, last, from, 1, raw_page(p, b, r.begin + from + static_cast<int64_t>(lane)),
+                    [&](int i, uint32_t rank) { held[i] = rank; });
   }
 }
 __global__ void __launch_bounds__(kThreads)

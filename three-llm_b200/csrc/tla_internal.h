@@ -65,9 +65,7 @@ struct tla_paged {
   int io = 0, kept = 0;     // tla::Type of the activations and of the pages
   int page_shift = 0;       // log2(page_size)
   bool wide = false;        // head_dim 64 or 128, rows of the pool on 16-byte boundaries
-  // tensor-core decode path (16-bit pages, D in {64, 128}, page_size >= 16)
-  bool fast = false;
-  CUtensorMap tmap_k{}, tmap_v{};
+  bool fast = false;        // tensor-core decode path (paged_decode_configure)
 };
 
 namespace tla {
