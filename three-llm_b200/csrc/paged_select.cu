@@ -165,94 +165,106 @@ __device__ __forceinline__ void score_any(const PagedArgs& p, const double* vec,
 }
 
 // Writes the `count` pages of the highest ranks, ties to the lower page, in
-// page order, by one block. The lowest rank that is taken is found two bits at
-// a time from the top: each round counts how many ranks share the bits found
-// so far and have at least 1, 2, 3 in the next two, by votes and sums across
-// the warps (ranks of like pages agree in most high bits, which a table of
-// counters would serialise on), and it ends early when every rank that shares
-// the bits is taken.
+// page order, by one block. The lowest rank that is taken is found three bits
+// at a time, below the leading bits that the lowest and highest rank share:
+// each round counts how many ranks agree in the bits found so far and have at
+// least 1 .. 7 in the next three, by sums across the warps (like pages' ranks
+// crowd into few values of most digits, which a table of counters would
+// serialise on), and it ends early when every rank that agrees is taken. A
+// round costs one barrier.
 struct PickSmem {
-  int counts[2][kWarps][4];
-  int taken[kWarps], same[kWarps];
+  int counts[2][kWarps][8];
+  int sums[2][kWarps];
 };
-__device__ __forceinline__ void pick_pages(const uint32_t* rank, PageRange r, int count, int32_t* out, PickSmem* sm) {
+constexpr uint32_t kAlways = 0xffffffffu;
+
+__device__ __forceinline__ void pick_pages(const uint32_t* rank, PageRange r, int count, int always, int32_t* out,
+                                           PickSmem* sm) {
   const unsigned full = 0xffffffffu;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int want = count - always;  // of the ranks below kAlways that agree with the prefix
   uint32_t prefix = 0;
-  int want = count;  // pages still to take among those that share the bits found
-  int shift = 30;
-  for (;; shift -= 2) {
-    int c1 = 0, c2 = 0, c3 = 0;
+  int shift = 32;  // the prefix's bits from here up are found
+  if (want > 0) {
+    uint32_t low = 0xffffffffu, high = 0u;
     for (int i = tid; i < r.n; i += kThreads) {
-      const uint32_t v = rank[i] >> shift;
-      if (shift < 30 && (v >> 2) != prefix >> (shift + 2)) continue;
-      const int digit = v & 3;
-      c1 += digit >= 1;
-      c2 += digit >= 2;
-      c3 += digit >= 3;
+      const uint32_t v = rank[i];
+      if (v == kAlways) continue;
+      low = min(low, v);
+      high = max(high, v);
     }
-    c1 = __reduce_add_sync(full, c1);
-    c2 = __reduce_add_sync(full, c2);
-    c3 = __reduce_add_sync(full, c3);
-    int* mine = sm->counts[(shift >> 1) & 1][warp];
+    low = __reduce_min_sync(full, low);
+    high = __reduce_max_sync(full, high);
     if (lane == 0) {
-      mine[0] = c1;
-      mine[1] = c2;
-      mine[2] = c3;
+      sm->counts[1][warp][0] = static_cast<int>(low);
+      sm->counts[1][warp][1] = static_cast<int>(high);
     }
     __syncthreads();
-    const int* all = sm->counts[(shift >> 1) & 1][lane % kWarps];
-    c1 = __reduce_add_sync(full, lane < kWarps ? all[0] : 0);
-    c2 = __reduce_add_sync(full, lane < kWarps ? all[1] : 0);
-    c3 = __reduce_add_sync(full, lane < kWarps ? all[2] : 0);
-    uint32_t digit = 0;
-    int here = -1;  // ranks with exactly this digit, where that says that all are taken
-    if (want <= c3) {
-      digit = 3;
-      here = c3;
-    } else if (want <= c2) {
-      digit = 2;
-      want -= c3;
-      here = c2 - c3;
-    } else if (want <= c1) {
-      digit = 1;
-      want -= c2;
-      here = c1 - c2;
-    } else {
-      want -= c1;
+    low = __reduce_min_sync(full, lane < kWarps ? static_cast<uint32_t>(sm->counts[1][lane][0]) : 0xffffffffu);
+    high = __reduce_max_sync(full, lane < kWarps ? static_cast<uint32_t>(sm->counts[1][lane][1]) : 0u);
+    // (n > count, so there is a rank below kAlways, and low <= high)
+    shift = low == high ? 0 : 32 - __clz(low ^ high);
+    prefix = shift >= 32 ? 0u : high >> shift << shift;
+    bool buffer = false;
+    while (shift > 0) {
+      const int bits = min(3, shift), next = shift - bits;
+      int c[7] = {0, 0, 0, 0, 0, 0, 0};  // [k]: ranks with at least k + 1 in the next bits
+      for (int i = tid; i < r.n; i += kThreads) {
+        const uint32_t v = rank[i];
+        if (v == kAlways || (shift < 32 && (v ^ prefix) >> shift != 0)) continue;
+        const int digit = static_cast<int>(v >> next) & ((1 << bits) - 1);
+#pragma unroll
+        for (int k = 0; k < 7; ++k) c[k] += digit > k;
+      }
+      int* mine = sm->counts[buffer][warp];
+#pragma unroll
+      for (int k = 0; k < 7; ++k) {
+        const int s = __reduce_add_sync(full, c[k]);
+        if (lane == k) mine[k] = s;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 7; ++k) c[k] = __reduce_add_sync(full, lane < kWarps ? sm->counts[buffer][lane][k] : 0);
+      buffer = !buffer;
+      uint32_t digit = 0;
+      int above = 0, here = -1;  // ranks of higher digits; of this one, where known
+#pragma unroll
+      for (int k = 6; k >= 0; --k)
+        if (digit == 0) {
+          if (want <= c[k]) {
+            digit = k + 1;
+            here = c[k] - above;
+          } else {
+            above = c[k];
+          }
+        }
+      want -= above;
+      prefix |= digit << next;
+      shift = next;
+      if (here == want) break;
     }
-    prefix |= digit << shift;
-    if (shift == 0 || here == want) break;
   }
-  // taken: ranks whose bits from `shift` up are above the prefix's, and the first `want` that equal it
-  const uint32_t border = prefix >> shift;
-  int taken = 0, equal = 0;  // before this round of pages
+  // taken: kAlways, ranks above the prefix from `shift` up, and the first `want` that agree with it
+  const uint32_t border = shift >= 32 ? 0u : prefix >> shift;
+  int taken = 0, equal = 0;  // in the rounds before; counts of a round in one word, 512 pages at most
+  bool buffer = false;
   for (int base = 0; base < r.n; base += kThreads) {
     const int i = base + tid;
-    const uint32_t v = i < r.n ? rank[i] >> shift : 0u;
-    const bool above = i < r.n && v > border, same = i < r.n && v == border;
-    const unsigned same_mask = __ballot_sync(full, same);
+    const uint32_t v = i < r.n ? rank[i] : 0u;
+    const bool surely = i < r.n && (v == kAlways || (shift < 32 && v >> shift > border));
+    const bool same = i < r.n && !surely && shift < 32 && v >> shift == border;
+    const unsigned sure_mask = __ballot_sync(full, surely), same_mask = __ballot_sync(full, same);
+    if (lane == 0) sm->sums[buffer][warp] = __popc(sure_mask) << 16 | __popc(same_mask);
     __syncthreads();
-    if (lane == 0) sm->same[warp] = __popc(same_mask);
-    __syncthreads();
-    int eq = equal + __popc(same_mask & ((1u << lane) - 1)), all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) eq += sm->same[w];
-      all += sm->same[w];
-    }
-    equal += all;
-    const bool take = above || (same && eq < want);
-    const unsigned take_mask = __ballot_sync(full, take);
-    if (lane == 0) sm->taken[warp] = __popc(take_mask);
-    __syncthreads();
-    int at = taken + __popc(take_mask & ((1u << lane) - 1));
-    all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) at += sm->taken[w];
-      all += sm->taken[w];
-    }
-    if (take) out[at] = r.begin + i;
-    taken += all;
+    const int s = lane < kWarps ? sm->sums[buffer][lane] : 0;
+    const int all = __reduce_add_sync(full, s), prior = __reduce_add_sync(full, lane < warp ? s : 0);
+    buffer = !buffer;
+    const unsigned below = (1u << lane) - 1;
+    const int eq = equal + (prior & 0xffff) + __popc(same_mask & below);
+    const int at = taken + (prior >> 16) + __popc(sure_mask & below) + min(eq, want);
+    if (surely || (same && eq < want)) out[at] = r.begin + i;
+    taken += all >> 16;
+    equal += all & 0xffff;
   }
 }
 
@@ -277,6 +289,7 @@ __global__ void __launch_bounds__(kThreads)
   griddep_launch_dependents();
   cg::cluster_group cluster = cg::this_cluster();
   const int share = cluster.block_rank(), shares = cluster.num_blocks();
+  if (shares > 1) cluster.barrier_arrive();
   const int pair = blockIdx.x / shares, b = pair / p.a.Hk, kvh = pair - b * p.a.Hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int step = kWarps * shares;
@@ -286,15 +299,13 @@ __global__ void __launch_bounds__(kThreads)
   form_vector(p, query, b, kvh, vec);
   const PageRange r = page_range(p, pos);
   int32_t* out = pages_out + static_cast<int64_t>(pair) * count;
+  // every block of the cluster runs before one writes into another's memory
+  if (shares > 1) cluster.barrier_wait();
   if (r.n <= count) {  // (the same for the whole cluster)
     if (share == 0) list_all(p, pos, r, count, out);
     return;
   }
-  // every block of the cluster runs before one writes into another's memory
-  if (shares > 1)
-    cluster.sync();
-  else
-    __syncthreads();
+  __syncthreads();
   uint32_t* held = shares > 1 ? cluster.map_shared_rank(ranks, 0) : ranks;
   for (bool again = false; from < r.n; from += 32 * step, again = true) {
     if (again || p.a.sliding > 0) raw = raw_page(p, b, r.begin + from + static_cast<int64_t>(step) * lane);
@@ -304,7 +315,7 @@ __global__ void __launch_bounds__(kThreads)
     cluster.sync();
   else
     __syncthreads();
-  if (share == 0) pick_pages(ranks, r, count, out, &pick_s);
+  if (share == 0) pick_pages(ranks, r, count, first + last, out, &pick_s);
 }
 
 // The same in two launches, the ranks in the workspace, for sequences of more
@@ -331,7 +342,8 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 __global__ void __launch_bounds__(kThreads)
-    paged_pick_kernel(PagedArgs p, const uint32_t* __restrict__ ranks, int count, int32_t* __restrict__ pages_out) {
+    paged_pick_kernel(PagedArgs p, const uint32_t* __restrict__ ranks, int always, int count,
+                      int32_t* __restrict__ pages_out) {
   __shared__ PickSmem pick_s;
   griddep_wait();
   griddep_launch_dependents();
@@ -341,7 +353,7 @@ __global__ void __launch_bounds__(kThreads)
   if (r.n <= count)
     list_all(p, pos, r, count, out);
   else
-    pick_pages(ranks + static_cast<int64_t>(blockIdx.x) * p.width, r, count, out, &pick_s);
+    pick_pages(ranks + static_cast<int64_t>(blockIdx.x) * p.width, r, count, always, out, &pick_s);
 }
 
 // Pages that a sequence can have in this call.
@@ -388,7 +400,7 @@ cudaError_t select_t(const tla_paged* P, const PagedArgs& p, const void* query, 
       cudaLaunchKernelEx(&cfg, paged_score_kernel<IO, CT>, p, static_cast<const IO*>(query), first, last, count, ranks);
   if (e != cudaSuccess) return e;
   return launch_pdl(paged_pick_kernel, static_cast<unsigned>(pairs), kThreads, 0, stream, p,
-                    static_cast<const uint32_t*>(ranks), count, pages_out);
+                    static_cast<const uint32_t*>(ranks), first + last, count, pages_out);
 }
 
 }  // namespace
