@@ -43,27 +43,6 @@
 
 #include "paged.cuh"
 
-#ifndef CTAS
-#define CTAS 2
-#endif
-#ifndef TILE64
-#define TILE64 32
-#endif
-#ifndef TILE128
-#define TILE128 16
-#endif
-#ifndef STG64
-#define STG64 3
-#endif
-#ifndef STG128
-#define STG128 3
-#endif
-#ifndef SETUP64
-#define SETUP64 8
-#endif
-#ifndef SETUP128
-#define SETUP128 8
-#endif
 namespace tla {
 
 namespace {
@@ -71,23 +50,23 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxBatch = 1024;  // prefix table in shared memory
-constexpr int kCtasPerSm = CTAS;
+constexpr int kCtasPerSm = 2;
 constexpr int kMaxGrid = 1024;   // segment table of the joining kernel
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNowhere = -(1 << 30);  // first position of 16 tokens that take no part
 
 template <int D>
 struct Cfg {
-  static constexpr int kTile = D == 64 ? TILE64 : TILE128;
+  static constexpr int kTile = D == 64 ? 32 : 16;
   static constexpr int kGroups = kTile / 16;
-  static constexpr int kStages = D == 64 ? STG64 : STG128;
+  static constexpr int kStages = 2;
   static constexpr int kHalves = D / 64;  // 128-byte rows per cache row
   static constexpr int kTileBytes = kTile * kHalves * 128;
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kQPitch = D * 2 + 16;
   // A pair costs its query set-up and its epilogue besides its tiles: counted
   // as this many tiles when the shares are cut.
-  static constexpr int kSetup = D == 64 ? SETUP64 : SETUP128;
+  static constexpr int kSetup = 14;
 };
 
 struct DecodeParams {
@@ -175,12 +154,17 @@ __device__ __forceinline__ void scan_prefix(int* prefix, int batch, int lane) {
 __device__ __forceinline__ int effective_grid(int total, int grid, int small) {
   return small < grid && total < 8 * small ? small : grid;
 }
+// First unit of share c (a 64-bit division is on every CTA's way: only where 32 bits do not hold the product).
 __device__ __forceinline__ int cta_begin(int c, int total, int grid) {
+  if (total < (1 << 30) / kMaxGrid)
+    return static_cast<int>(static_cast<unsigned>(c * total) / static_cast<unsigned>(grid));
   return static_cast<int>(static_cast<long long>(c) * total / grid);
 }
 // Largest c with cta_begin(c) <= g.
 __device__ __forceinline__ int cta_of(int g, int total, int grid) {
-  int c = static_cast<int>(static_cast<long long>(g) * grid / total);
+  int c = total < (1 << 30) / kMaxGrid
+              ? static_cast<int>(static_cast<unsigned>(g * grid) / static_cast<unsigned>(total))
+              : static_cast<int>(static_cast<long long>(g) * grid / total);
   while (c + 1 < grid && cta_begin(c + 1, total, grid) <= g) ++c;
   while (c > 0 && cta_begin(c, total, grid) > g) --c;
   return c;
@@ -223,8 +207,11 @@ __device__ __forceinline__ int next_pair(const int* prefix, int batch, int pairs
   return prefix[b] + (g - prefix[b] + per - 1) / per * per;
 }
 
-// 16 bytes to shared memory, zeros instead when `bytes` is 0.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+// 16 bytes to shared memory; zeros instead when `bytes` is 0.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zeros(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -332,12 +319,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   ld.begin = ld.end = 0;
   ld.base = 0;
   ld.list = nullptr;
-  // (entries are only looked at when they are used, so that a window's loads are not waited for)
+  // (Entries are only looked at when they are used, so that a window's loads
+  // are not waited for; a list's end is checked there, too.)
   auto look = [&](int e, int* index, int* page) {
     const bool in = e >= ld.e_first && e < ld.e_end;
-    *index = !in ? 0 : ld.list ? ld.list[e] : e;
-    *page = in ? p.table[static_cast<int64_t>(ld.b) * p.width + *index] : kNowhere;
+    *index = !in ? -1 : ld.list ? ld.list[e] : e;
+    *page = static_cast<unsigned>(*index) < static_cast<unsigned>(p.width)
+                ? p.table[static_cast<int64_t>(ld.b) * p.width + *index] : kNowhere;
   };
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes per row, rows per copy
+  const int r0 = lane / kLanes, chunk = lane % kLanes;
+  // where a lane's 16 bytes go: two places in turn, 1024 bytes on every second copy
+  const uint32_t place0 = sw128(r0 * C::kHalves + (chunk >> 3), chunk & 7);
+  const uint32_t place1 = sw128((r0 + kRows) * C::kHalves + (chunk >> 3), chunk & 7);
+  const int64_t lane_from = r0 * p.slot_stride + chunk * 8;
+  const bool dense = p.slot_stride == D;  // a page's rows of a head are one block
+  const int64_t apart = static_cast<const CT*>(p.value) - static_cast<const CT*>(p.key);
   auto load_next = [&](int stage) {
     while (ld.it >= ld.end && ld.g < te) {  // on to the segment that holds the tile
       while (prefix[ld.b + 1] <= ld.g) ++ld.b;
@@ -349,16 +346,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       const Walk w = walk_of<D>(d, spos[ld.b]);
       const int kvh = sg.pair / d.subs, last_page = w.hi >> shift;
       ld.list = d.pages ? d.pages + (static_cast<int64_t>(ld.b) * p.a.Hk + kvh) * d.count : nullptr;
-      ld.head = kvh * p.head_stride;
+      ld.head = kvh * p.head_stride + lane_from;
       ld.lo = w.lo;
       ld.hi = w.hi;
       ld.first = w.first + sg.lt;
       ld.e_first = ld.list ? 0 : w.lo >> shift;
-      ld.e_end = min(static_cast<int>((static_cast<int64_t>(ld.first + sg.n) * C::kTile - 1) >> shift) + 1,
-                     ld.list ? list_length(p, ld.list, min(d.count, last_page + 1), last_page, lane) : last_page + 1);
+      const int most = min(d.pages ? d.count : last_page + 1, last_page + 1);
+      ld.e_end = min(static_cast<int>((static_cast<int64_t>(ld.first + sg.n) * C::kTile - 1) >> shift) + 1, most);
       ld.base = static_cast<int>((static_cast<int64_t>(ld.first + ld.it - ld.begin) * C::kTile) >> shift);
       look(ld.base + lane, &ld.index, &ld.page);
       look(ld.base + 32 + lane, &ld.index_next, &ld.page_next);
+      if (ld.list) ld.e_end = min(ld.e_end, list_length(p, ld.list, most, last_page, lane));
     }
     if (ld.it < ld.end) {
       const int64_t token = static_cast<int64_t>(ld.first + ld.it - ld.begin) * C::kTile;
@@ -370,13 +368,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         look(ld.base + 32 + lane, &ld.index_next, &ld.page_next);
       }
       const uint32_t kst = ring + stage * C::kStageBytes;
-      constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes per row, rows per copy
-      const int r0 = lane / kLanes, chunk = lane % kLanes;
 #pragma unroll
       for (int u = 0; u < C::kGroups; ++u) {
         const int piece = (offset + u * 16) >> shift;  // pages of under a tile: the group's page within the tile
         const int index = __shfl_sync(0xffffffffu, ld.index, e - ld.base + piece);
         int page = __shfl_sync(0xffffffffu, ld.page, e - ld.base + piece);
+        if (e + piece >= ld.e_end) page = kNowhere;
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.page_count)) {
           if (page != kNowhere) report_error(p.a.error, TLA_ERR_PAGE);
           page = -1;
@@ -384,19 +381,34 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         const int slot = (offset + u * 16) & mask;
         const int at = page < 0 ? kNowhere : (index << shift) + slot;
         if (lane == 0) meta[stage * C::kGroups + u] = at;
-        const int64_t from = page < 0 ? 0 : page * p.page_stride + ld.head + (slot + r0) * p.slot_stride + chunk * 8;
-        const CT* k = static_cast<const CT*>(p.key) + from;
-        const CT* v = static_cast<const CT*>(p.value) + from;
-        const int64_t step = page < 0 ? 0 : kRows * p.slot_stride;
+        const CT* k = static_cast<const CT*>(p.key) + (page * p.page_stride + slot * p.slot_stride + ld.head);
+        const uint32_t dst = kst + u * 16 * C::kHalves * 128;
+        if (at >= ld.lo && at + 15 <= ld.hi) {  // (the same for the whole warp)
+          if (dense) {
 #pragma unroll
-        for (int i = 0; i < 16 / kRows; ++i) {
-          const int r = r0 + i * kRows;
-          const int bytes = at + r >= ld.lo && at + r <= ld.hi ? 16 : 0;
-          const uint32_t dst = kst + sw128((u * 16 + r) * C::kHalves + (chunk >> 3), chunk & 7);
-          copy16(dst, k, bytes);
-          copy16(dst + C::kTileBytes, v, bytes);
-          k += step;
-          v += step;
+            for (int i = 0; i < 16 / kRows; ++i) {
+              const uint32_t to = dst + (i / 2) * 1024 + (i % 2 ? place1 : place0);
+              copy16(to, k + i * kRows * D);
+              copy16(to + C::kTileBytes, k + apart + i * kRows * D);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16 / kRows; ++i) {
+              const uint32_t to = dst + (i / 2) * 1024 + (i % 2 ? place1 : place0);
+              copy16(to, k);
+              copy16(to + C::kTileBytes, k + apart);
+              k += kRows * p.slot_stride;
+            }
+          }
+        } else {  // rows outside the range, and pages that are not there, as zeros
+#pragma unroll 1
+          for (int i = 0; i < 16 / kRows; ++i) {
+            const int tok = at + r0 + i * kRows, bytes = tok >= ld.lo && tok <= ld.hi ? 16 : 0;
+            const CT* from = bytes ? k + i * kRows * p.slot_stride : static_cast<const CT*>(p.key);
+            const uint32_t to = dst + (i / 2) * 1024 + (i % 2 ? place1 : place0);
+            copy16_or_zeros(to, from, bytes);
+            copy16_or_zeros(to + C::kTileBytes, bytes ? from + apart : from, bytes);
+          }
         }
       }
     }
@@ -535,12 +547,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
 #pragma unroll
           for (int u = 0; u < kGroups; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int tok = at[u] + g8 + (e >> 1) * 8;
-              const float v = x[u][nt][e] * scale[nt][e & 1];
-              x[u][nt][e] = whole || (tok >= w.lo && tok <= w.hi) ? v : -INFINITY;
-              top[e & 1] = fmaxf(top[e & 1], x[u][nt][e]);
-            }
+            for (int e = 0; e < 4; ++e) x[u][nt][e] *= scale[nt][e & 1];
+          if (!whole) {
+#pragma unroll
+            for (int u = 0; u < kGroups; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int tok = at[u] + g8 + (e >> 1) * 8;
+                if (tok < w.lo || tok > w.hi) x[u][nt][e] = -INFINITY;
+              }
+          }
+#pragma unroll
+          for (int u = 0; u < kGroups; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], x[u][nt][e]);
           float base[2], keep[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -571,10 +591,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
               pl[u][nt][1] = transpose8(pack_rest(p1, pr[2], pr[3]));
             }
           }
+          if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {  // a maximum rose
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i)
+            for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[nt][i][e] *= keep[e & 1];
+              for (int e = 0; e < 4; ++e) o[nt][i][e] *= keep[e & 1];
+          }
         }
         // O^T += V^T P^T: dimensions g8 and g8 + 8 of each 16
         const uint32_t vbase = kbase + C::kTileBytes;
@@ -627,28 +649,28 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     __syncthreads();
     const bool whole = sg.lt == 0 && sg.n == sg.tiles;
     float* mine = d.scratch + (static_cast<size_t>(cta) * 2 + (g == tb ? 0 : 1)) * rows * (D + 2);
-    for (int i = tid; i < heads * D; i += 128) {
-      const int r = i / D, c = i - r * D;
-      float top = -INFINITY, sum = 0.f, v = 0.f;
+    for (int i = tid; i < heads * (D / 2); i += kThreads) {  // two columns each
+      const int r = i / (D / 2), c = i % (D / 2) * 2;
+      float2 ml[kWarps];
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) top = fmaxf(top, red[(k * rows + r) * (D + 2)]);
-      if (top != -INFINITY) {
+      for (int k = 0; k < kWarps; ++k) ml[k] = *reinterpret_cast<const float2*>(red + (k * rows + r) * (D + 2));
+      const float top = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, v0 = 0.f, v1 = 0.f;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-          const float* rr = red + (k * rows + r) * (D + 2);
-          const float f = ex2(rr[0] - top);
-          sum += rr[1] * f;
-          v += rr[2 + c] * f;
-        }
+      for (int k = 0; k < kWarps; ++k) {
+        const float2 x = *reinterpret_cast<const float2*>(red + (k * rows + r) * (D + 2) + 2 + c);
+        const float f = ex2(ml[k].x - base);
+        sum += ml[k].y * f;
+        v0 += x.x * f;
+        v1 += x.y * f;
       }
       if (whole) {
-        store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * D + c, sum > 0.f ? v / sum : 0.f);
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * D + c, v0 * inv);
+        store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * D + c + 1, v1 * inv);
       } else {
-        mine[r * (D + 2) + 2 + c] = v;
-        if (c == 0) {
-          mine[r * (D + 2)] = top;
-          mine[r * (D + 2) + 1] = sum;
-        }
+        *reinterpret_cast<float2*>(mine + r * (D + 2) + 2 + c) = make_float2(v0, v1);
+        if (c == 0) *reinterpret_cast<float2*>(mine + r * (D + 2)) = make_float2(top, sum);
       }
     }
     __syncthreads();  // red and q_s are free for the next segment
@@ -660,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
 // query head). It recomputes the shares from the positions, which it may read
 // before the first kernel has finished: that kernel only starts its successor
 // once its own wait for what came before is over.
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 4;
 template <int D, typename IO>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(const __grid_constant__ DecodeParams d,
                                                                            int launch_grid) {
@@ -697,14 +719,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
   griddep_wait();
   if (c0 == c1) return;  // one CTA held the whole pair, or there is none
   const int n = c1 - c0 + 1;
+  const bool alone = n <= kBatch;  // few triples: one warp joins them without the others
+  if (alone && warp != 0) return;
+  const int warps = alone ? 1 : kJoinWarps;
   float top = -INFINITY, sum = 0.f, acc[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-  for (int k = warp; k < n; k += kBatch * kJoinWarps) {
+  for (int k = warp; k < n; k += kBatch * warps) {
     float mk[kBatch], lk[kBatch], v[kBatch][kPer];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int at = k + u * kJoinWarps, slot = at < n ? slot_of[at] : -1;
+      const int at = k + u * warps, slot = at < n ? slot_of[at] : -1;
       mk[u] = -INFINITY;
       lk[u] = 0.f;
 #pragma unroll
@@ -733,6 +758,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
       for (int e = 0; e < kPer; ++e) acc[e] += v[u][e] * f;
     }
     top = high;
+  }
+  if (alone) {
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * D + lane + 32 * e, sum > 0.f ? acc[e] / sum : 0.f);
+    return;
   }
   if (lane == 0) {
     red[0][warp] = top;
@@ -819,10 +850,16 @@ long long most_tiles(const PagedArgs& p, int count) {
   return tiles;
 }
 
-#ifndef WHOLE
-#define WHOLE 20
-#endif
-bool whole_pairs(const PagedArgs& p, int count) { return most_tiles(p, count) <= WHOLE; }
+// Short calls give every pair to one CTA and need no second kernel: where a
+// pair has at most 16 tiles (8 sequences of 4 query heads per kv head at
+// head_dim 64: 257 tokens 8.4 us against 9.3 with shares; 513 tokens 10.5
+// against 10.0, which the launch saved outweighs for the caller), or at most
+// 32 when there are pairs for every CTA (64 such sequences of 513 tokens: 22.4
+// us against 26.7; at 1025 tokens and ragged lengths shares win again).
+bool whole_pairs(const tla_paged* P, const PagedArgs& p, int count) {
+  const long long tiles = most_tiles(p, count), pairs = static_cast<long long>(p.batch) * p.a.Hk * subgroups(P);
+  return tiles <= 16 || (tiles <= 32 && pairs >= kCtasPerSm * P->base.ctx->sm_count);
+}
 
 // Whether a call's shares can be cut: the batch's table fits shared memory and
 // its tiles are counted in 32 bits.
@@ -832,7 +869,7 @@ bool paged_decode_takes(const tla_paged* P, const PagedArgs& p, int count) {
 }
 
 size_t paged_decode_workspace(const tla_paged* P, const PagedArgs& p, int count) {
-  if (whole_pairs(p, count)) return 0;
+  if (whole_pairs(P, p, count)) return 0;
   return static_cast<size_t>(kCtasPerSm) * P->base.ctx->sm_count * 2 * subgroup_rows(P) * (P->base.D + 2) *
          sizeof(float);
 }
@@ -850,7 +887,7 @@ cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const vo
   d.subs = subgroups(P);
   d.rows = subgroup_rows(P);
   d.small_grid = 0;
-  d.whole = whole_pairs(p, count) ? 1 : 0;
+  d.whole = whole_pairs(P, p, count) ? 1 : 0;
   return P->base.D == 64 ? launch_d<64>(P, d, stream) : launch_d<128>(P, d, stream);
 }
 

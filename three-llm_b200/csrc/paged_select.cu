@@ -11,6 +11,8 @@
 #include <cooperative_groups.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace tla {
@@ -19,11 +21,10 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kMaxCluster = 8;
+constexpr int kMaxWarps = 16;
+constexpr int kMaxCluster = 16;
 constexpr int kMaxHeld = 48 * 1024;  // ranks that one block's shared memory holds
-constexpr int kScorePages = 32 * kWarps;  // pages per block of the scoring kernel for longer sequences
+constexpr int kScorePages = 32 * kMaxWarps;  // pages per block of the scoring kernel for longer sequences
 
 // Larger scores have larger keys, and every score a key above 0.
 __device__ __forceinline__ uint32_t rank_of(float s) {
@@ -41,9 +42,41 @@ __device__ __forceinline__ PageRange page_range(const PagedArgs& p, int pos) {
   return {lo >> p.page_shift, (hi >> p.page_shift) - (lo >> p.page_shift) + 1};
 }
 
-// The score's vector (N, then P, as the bounds' order), formed by a block.
-template <typename IO>
-__device__ __forceinline__ void form_vector(const PagedArgs& p, const IO* query, int b, int kvh, double* vec) {
+constexpr uint32_t kAlways = 0xffffffffu;  // the rank of a page that always takes part
+
+// 16-bit values become doubles by placing their bits: exponent and mantissa in
+// the high word, without a new bias, give the value times kScale, exactly, for
+// subnormals too (the conversion instructions, one of them per element at an
+// eighth of the rate, would bound the kernel). The vector carries 2^880 in
+// return: no product over- or underflows, and a sum times kBack is the score.
+// (A bound that is not finite counts as a large one.)
+template <typename CT>
+struct Bits;
+template <>
+struct Bits<__half> {
+  static constexpr int kShift = 10;  // 5 + 10 bits, scaled by 2^-1008
+  static constexpr double kForth = 0x1p880, kBack = 0x1p128;
+};
+template <>
+struct Bits<__nv_bfloat16> {
+  static constexpr int kShift = 13;  // 8 + 7 bits, scaled by 2^-896
+  static constexpr double kForth = 0x1p880, kBack = 0x1p16;
+};
+template <>
+struct Bits<float> {
+  static constexpr double kForth = 1, kBack = 1;  // (converted)
+};
+
+// The score's vector (N, then P, as the bounds' order), formed by a block. With
+// `lanes` lanes of `vec` neighbouring elements each, element d lies where a
+// warp's 16-byte reads of its lanes' pairs (2 k, 2 k + 1) are neighbours.
+__device__ __forceinline__ int vec_place(int d, int vec, int lanes) {
+  const int lane = d / vec % lanes, e = d / (vec * lanes) * vec + d % vec;  // e: the lane's element
+  return (e / 2 * lanes + lane) * 2 + (e & 1);
+}
+template <int kThreads, typename IO>
+__device__ __forceinline__ void form_vector(const PagedArgs& p, const IO* query, int b, int kvh, double* vec, int per,
+                                            int lanes, double scale) {
   const int D = p.a.D, G = p.a.G;
   const IO* q = query + (static_cast<int64_t>(b) * p.a.Hq + kvh * G) * D;
   for (int d = threadIdx.x; d < D; d += kThreads) {
@@ -54,21 +87,31 @@ __device__ __forceinline__ void form_vector(const PagedArgs& p, const IO* query,
       neg += fminf(x, 0.f);
       pos += fmaxf(x, 0.f);
     }
-    vec[d] = neg;
-    vec[D + d] = pos;
+    vec[lanes ? vec_place(d, per, lanes) : d] = neg * scale;
+    vec[lanes ? vec_place(D + d, per, lanes) : D + d] = pos * scale;
   }
 }
 
 // 16 bytes of bounds times their part of the vector.
 template <typename CT>
 __device__ __forceinline__ double dot16(uint4 u, const double* v) {
-  constexpr int kVec = 16 / sizeof(CT);
-  const CT* x = reinterpret_cast<const CT*>(&u);
   double s0 = 0, s1 = 0;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  if constexpr (sizeof(CT) == 2) {
+    constexpr uint32_t kRest = 0x7fffu << Bits<CT>::kShift;
 #pragma unroll
-  for (int e = 0; e < kVec; e += 2) {
-    s0 = fma(v[e], static_cast<double>(to_f32(x[e])), s0);
-    s1 = fma(v[e + 1], static_cast<double>(to_f32(x[e + 1])), s1);
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t even = (w[e] << 16 & 0x80000000u) | (w[e] << Bits<CT>::kShift & kRest);
+      const uint32_t odd = (w[e] & 0x80000000u) | (w[e] >> (16 - Bits<CT>::kShift) & kRest);
+      s0 = fma(v[2 * e], __hiloint2double(static_cast<int>(even), 0), s0);
+      s1 = fma(v[2 * e + 1], __hiloint2double(static_cast<int>(odd), 0), s1);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      s0 = fma(v[e], static_cast<double>(__uint_as_float(w[e])), s0);
+      s1 = fma(v[e + 1], static_cast<double>(__uint_as_float(w[e + 1])), s1);
+    }
   }
   return s0 + s1;
 }
@@ -95,29 +138,34 @@ __device__ __forceinline__ void score_32(const PagedArgs& p, const double* vec, 
     report_error(p.a.error, TLA_ERR_PAGE);
     page = -1;
   }
-  uint32_t rank = always ? 0xffffffffu : 0u;  // (a page outside the pool ranks last)
+  if (held && page < 0) put(mine, always ? kAlways : 0u);  // (a page outside the pool ranks last)
   const unsigned scored = __ballot_sync(full, page >= 0);
   const CT* bounds = static_cast<const CT*>(p.bounds) + static_cast<int64_t>(kvh) * 2 * D;
   const int64_t stride = static_cast<int64_t>(p.a.Hk) * 2 * D;
   if constexpr (kD > 0) {
     constexpr int kVec = 16 / sizeof(CT), kReads = 2 * kD / kVec;        // 16-byte reads per page
     constexpr int kLanes = kReads < 32 ? kReads : 32, kPer = kReads / kLanes;  // lanes per page, reads per lane
-    constexpr int kPages = 32 / kLanes, kAhead = 8 / kPer;                // pages per warp-wide read; reads in flight
+    constexpr int kPages = 32 / kLanes, kMost = 8 / kPer;  // pages per warp-wide read; reads in flight
     const int sub = lane / kLanes, at = lane % kLanes;
     double v[kPer][kVec];
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[i][e] = vec[(i * kLanes + at) * kVec + e];
+      for (int e = 0; e < kVec; e += 2) {
+        const double2 x = reinterpret_cast<const double2*>(vec)[(i * kVec + e) / 2 * kLanes + at];
+        v[i][e] = x.x;
+        v[i][e + 1] = x.y;
+      }
     const int n = 32 - __clz(scored);  // (0 when none is scored)
-    for (int k0 = 0; k0 < n; k0 += kAhead * kPages) {
+    auto round = [&](auto ahead, int k0) {
+      constexpr int kAhead = decltype(ahead)::value;
       uint4 u[kAhead][kPer];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
-        const int of = __shfl_sync(full, page, (k0 + a * kPages + sub) & 31);
+        const int k = k0 + a * kPages + sub, of = __shfl_sync(full, page, k & 31);
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-          u[a][i] = of < 0 || k0 + a * kPages + sub > 31
+          u[a][i] = of < 0 || k > 31
                         ? make_uint4(0, 0, 0, 0)
                         : *reinterpret_cast<const uint4*>(bounds + of * stride + (i * kLanes + at) * kVec);
       }
@@ -128,19 +176,28 @@ __device__ __forceinline__ void score_32(const PagedArgs& p, const double* vec, 
 #pragma unroll
         for (int i = 1; i < kPer; ++i) s[a] += dot16<CT>(u[a][i], v[i]);
       }
+      // Sums across the page's lanes: as long as there are several pages, a
+      // lane hands half of them over and goes on with the other half.
+      int o = kLanes / 2;
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1)
+      for (int left = kAhead; left > 1; left /= 2, o /= 2) {
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) s[a] += __shfl_xor_sync(full, s[a], o);
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {  // page k0 + a kPages + j to its lane, from the j-th group of lanes
-#pragma unroll
-        for (int j = 0; j < kPages; ++j) {
-          const double of = kPages == 1 ? s[a] : __shfl_sync(full, s[a], j * kLanes);
-          if (lane == k0 + a * kPages + j && page >= 0) rank = min(rank_of(static_cast<float>(of)), 0xfffffffeu);
+        for (int a = 0; a < left / 2; ++a) {
+          const bool upper = (lane & o) != 0;
+          const double given = upper ? s[a] : s[a + left / 2];
+          s[a] = (upper ? s[a + left / 2] : s[a]) + __shfl_xor_sync(full, given, o);
         }
       }
-    }
+      constexpr int kOwners = kLanes / kAhead;  // lanes that end up with the same page
+#pragma unroll
+      for (int o2 = kOwners / 2; o2 > 0; o2 /= 2) s[0] += __shfl_xor_sync(full, s[0], o2);
+      const int k = k0 + at / kOwners * kPages + sub;
+      if (at % kOwners == 0 && (scored >> (k & 31) & 1) && k < 32)
+        put(from + step * k, min(rank_of(static_cast<float>(s[0] * Bits<CT>::kBack)), 0xfffffffeu));
+    };
+    int k0 = 0;
+    for (; n - k0 > 2 * kPages; k0 += kMost * kPages) round(std::integral_constant<int, kMost>(), k0);
+    for (; k0 < n; k0 += kPages) round(std::integral_constant<int, 1>(), k0);
   } else {
     for (unsigned left = scored; left != 0; left &= left - 1) {
       const int k = __ffs(left) - 1, of = __shfl_sync(full, page, k);
@@ -148,10 +205,15 @@ __device__ __forceinline__ void score_32(const PagedArgs& p, const double* vec, 
       for (int d = lane; d < 2 * D; d += 32) s = fma(vec[d], static_cast<double>(to_f32(bounds[of * stride + d])), s);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(full, s, o);
-      if (lane == k) rank = min(rank_of(static_cast<float>(s)), 0xfffffffeu);
+      if (lane == k) put(mine, min(rank_of(static_cast<float>(s)), 0xfffffffeu));
     }
   }
-  if (held) put(mine, rank);
+}
+// Lanes that hold a page's 16-byte pieces (0: any other head_dim).
+template <typename CT>
+__device__ __forceinline__ int piece_lanes(int D) {
+  const int reads = 2 * D * static_cast<int>(sizeof(CT)) / 16;
+  return D == 64 || D == 128 ? min(reads, 32) : 0;
 }
 template <typename CT, typename Put>
 __device__ __forceinline__ void score_any(const PagedArgs& p, const double* vec, int kvh, PageRange r, int first,
@@ -173,13 +235,14 @@ __device__ __forceinline__ void score_any(const PagedArgs& p, const double* vec,
 // serialise on), and it ends early when every rank that agrees is taken. A
 // round costs one barrier.
 struct PickSmem {
-  int counts[2][kWarps][8];
-  int sums[2][kWarps];
+  int counts[2][kMaxWarps][4];
+  int sure[kMaxWarps], same[kMaxWarps];
 };
-constexpr uint32_t kAlways = 0xffffffffu;
 
+template <int kThreads>
 __device__ __forceinline__ void pick_pages(const uint32_t* rank, PageRange r, int count, int always, int32_t* out,
                                            PickSmem* sm) {
+  constexpr int kWarps = kThreads / 32;
   const unsigned full = 0xffffffffu;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int want = count - always;  // of the ranks below kAlways that agree with the prefix
@@ -187,11 +250,11 @@ __device__ __forceinline__ void pick_pages(const uint32_t* rank, PageRange r, in
   int shift = 32;  // the prefix's bits from here up are found
   if (want > 0) {
     uint32_t low = 0xffffffffu, high = 0u;
+#pragma unroll 4
     for (int i = tid; i < r.n; i += kThreads) {
       const uint32_t v = rank[i];
-      if (v == kAlways) continue;
       low = min(low, v);
-      high = max(high, v);
+      high = max(high, v == kAlways ? 0u : v);
     }
     low = __reduce_min_sync(full, low);
     high = __reduce_max_sync(full, high);
@@ -208,34 +271,38 @@ __device__ __forceinline__ void pick_pages(const uint32_t* rank, PageRange r, in
     bool buffer = false;
     while (shift > 0) {
       const int bits = min(3, shift), next = shift - bits;
-      int c[7] = {0, 0, 0, 0, 0, 0, 0};  // [k]: ranks with at least k + 1 in the next bits
+      // [k]: ranks with at least k + 1 in the next bits (low half) and at least k + 5 (high half); a
+      // block's counts stay under 2^16
+      int c[4] = {0, 0, 0, 0};
+#pragma unroll 4
       for (int i = tid; i < r.n; i += kThreads) {
         const uint32_t v = rank[i];
-        if (v == kAlways || (shift < 32 && (v ^ prefix) >> shift != 0)) continue;
-        const int digit = static_cast<int>(v >> next) & ((1 << bits) - 1);
+        const bool out_of = v == kAlways || (shift < 32 && (v ^ prefix) >> shift != 0);
+        const int digit = out_of ? 0 : static_cast<int>(v >> next) & ((1 << bits) - 1);
 #pragma unroll
-        for (int k = 0; k < 7; ++k) c[k] += digit > k;
+        for (int k = 0; k < 4; ++k) c[k] += (digit > k) + ((digit > k + 4) << 16);
       }
       int* mine = sm->counts[buffer][warp];
 #pragma unroll
-      for (int k = 0; k < 7; ++k) {
+      for (int k = 0; k < 4; ++k) {
         const int s = __reduce_add_sync(full, c[k]);
         if (lane == k) mine[k] = s;
       }
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 7; ++k) c[k] = __reduce_add_sync(full, lane < kWarps ? sm->counts[buffer][lane][k] : 0);
+      for (int k = 0; k < 4; ++k) c[k] = __reduce_add_sync(full, lane < kWarps ? sm->counts[buffer][lane][k] : 0);
       buffer = !buffer;
       uint32_t digit = 0;
       int above = 0, here = -1;  // ranks of higher digits; of this one, where known
 #pragma unroll
       for (int k = 6; k >= 0; --k)
         if (digit == 0) {
-          if (want <= c[k]) {
+          const int n = k >= 4 ? static_cast<int>(static_cast<uint32_t>(c[k - 4]) >> 16) : c[k] & 0xffff;
+          if (want <= n) {
             digit = k + 1;
-            here = c[k] - above;
+            here = n - above;
           } else {
-            above = c[k];
+            above = n;
           }
         }
       want -= above;
@@ -246,29 +313,44 @@ __device__ __forceinline__ void pick_pages(const uint32_t* rank, PageRange r, in
   }
   // taken: kAlways, ranks above the prefix from `shift` up, and the first `want` that agree with it
   const uint32_t border = shift >= 32 ? 0u : prefix >> shift;
-  int taken = 0, equal = 0;  // in the rounds before; counts of a round in one word, 512 pages at most
-  bool buffer = false;
-  for (int base = 0; base < r.n; base += kThreads) {
-    const int i = base + tid;
-    const uint32_t v = i < r.n ? rank[i] : 0u;
-    const bool surely = i < r.n && (v == kAlways || (shift < 32 && v >> shift > border));
-    const bool same = i < r.n && !surely && shift < 32 && v >> shift == border;
+  // Each warp goes over its part of the pages twice: to count, and to write
+  // behind what the warps before it write.
+  const int per = (r.n + kThreads - 1) / kThreads * 32, from = min(r.n, warp * per), to = min(r.n, from + per);
+  auto look = [&](int i, bool* surely, bool* same) {
+    const uint32_t v = i < to ? rank[i] : 0u;
+    *surely = i < to && (v == kAlways || (shift < 32 && v >> shift > border));
+    *same = i < to && !*surely && shift < 32 && v >> shift == border;
+  };
+  int sure_n = 0, same_n = 0;
+#pragma unroll 4
+  for (int base = from; base < to; base += 32) {
+    bool surely, same;
+    look(base + lane, &surely, &same);
+    sure_n += __popc(__ballot_sync(full, surely));
+    same_n += __popc(__ballot_sync(full, same));
+  }
+  if (lane == 0) {
+    sm->sure[warp] = sure_n;
+    sm->same[warp] = same_n;
+  }
+  __syncthreads();
+  int taken = __reduce_add_sync(full, lane < warp ? sm->sure[lane] : 0);
+  int equal = __reduce_add_sync(full, lane < warp ? sm->same[lane] : 0);
+  const unsigned below = (1u << lane) - 1;
+#pragma unroll 4
+  for (int base = from; base < to; base += 32) {
+    bool surely, same;
+    look(base + lane, &surely, &same);
     const unsigned sure_mask = __ballot_sync(full, surely), same_mask = __ballot_sync(full, same);
-    if (lane == 0) sm->sums[buffer][warp] = __popc(sure_mask) << 16 | __popc(same_mask);
-    __syncthreads();
-    const int s = lane < kWarps ? sm->sums[buffer][lane] : 0;
-    const int all = __reduce_add_sync(full, s), prior = __reduce_add_sync(full, lane < warp ? s : 0);
-    buffer = !buffer;
-    const unsigned below = (1u << lane) - 1;
-    const int eq = equal + (prior & 0xffff) + __popc(same_mask & below);
-    const int at = taken + (prior >> 16) + __popc(sure_mask & below) + min(eq, want);
-    if (surely || (same && eq < want)) out[at] = r.begin + i;
-    taken += all >> 16;
-    equal += all & 0xffff;
+    const int eq = equal + __popc(same_mask & below), at = taken + __popc(sure_mask & below) + min(eq, want);
+    if (surely || (same && eq < want)) out[at] = r.begin + base + lane;
+    taken += __popc(sure_mask);
+    equal += __popc(same_mask);
   }
 }
 
 // All of a pair's pages, when there are no more than `count`.
+template <int kThreads>
 __device__ __forceinline__ void list_all(const PagedArgs& p, int pos, PageRange r, int count, int32_t* out) {
   if (r.n == 0 && pos >= 0 && threadIdx.x == 0) report_error(p.a.error, TLA_ERR_POSITION);
   for (int i = threadIdx.x; i < count; i += kThreads) out[i] = i < r.n ? r.begin + i : -1;
@@ -278,12 +360,13 @@ __device__ __forceinline__ void list_all(const PagedArgs& p, int pos, PageRange 
 // each and leave the ranks in the first block's shared memory, which picks.
 // One launch: what a step waits for here is latency, not the bounds' bytes, so
 // the position, the query and the first table entries are read side by side.
-template <typename IO, typename CT>
+template <typename IO, typename CT, int kThreads>
 __global__ void __launch_bounds__(kThreads)
     paged_select_kernel(PagedArgs p, const IO* __restrict__ query, int first, int last, int count,
                         int32_t* __restrict__ pages_out) {
   extern __shared__ __align__(16) double vec[];  // [2][D], then the ranks
   __shared__ PickSmem pick_s;
+  constexpr int kWarps = kThreads / 32;
   uint32_t* ranks = reinterpret_cast<uint32_t*>(vec + 2 * p.a.D);
   griddep_wait();
   griddep_launch_dependents();
@@ -296,13 +379,14 @@ __global__ void __launch_bounds__(kThreads)
   int from = warp * shares + share;
   const int pos = p.positions[b];
   int raw = p.a.sliding == 0 ? raw_page(p, b, from + static_cast<int64_t>(step) * lane) : 0;
-  form_vector(p, query, b, kvh, vec);
+  form_vector<kThreads>(p, query, b, kvh, vec, 16 / static_cast<int>(sizeof(CT)), piece_lanes<CT>(p.a.D),
+              piece_lanes<CT>(p.a.D) ? Bits<CT>::kForth : 1);
   const PageRange r = page_range(p, pos);
   int32_t* out = pages_out + static_cast<int64_t>(pair) * count;
   // every block of the cluster runs before one writes into another's memory
   if (shares > 1) cluster.barrier_wait();
   if (r.n <= count) {  // (the same for the whole cluster)
-    if (share == 0) list_all(p, pos, r, count, out);
+    if (share == 0) list_all<kThreads>(p, pos, r, count, out);
     return;
   }
   __syncthreads();
@@ -315,13 +399,13 @@ __global__ void __launch_bounds__(kThreads)
     cluster.sync();
   else
     __syncthreads();
-  if (share == 0) pick_pages(ranks, r, count, first + last, out, &pick_s);
+  if (share == 0) pick_pages<kThreads>(ranks, r, count, first + last, out, &pick_s);
 }
 
 // The same in two launches, the ranks in the workspace, for sequences of more
 // pages than shared memory holds ranks.
 template <typename IO, typename CT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kMaxWarps * 32)
     paged_score_kernel(PagedArgs p, const IO* __restrict__ query, int first, int last, int count,
                        uint32_t* __restrict__ ranks) {
   extern __shared__ __align__(16) double vec[];
@@ -333,7 +417,8 @@ __global__ void __launch_bounds__(kThreads)
     const int from = blockIdx.x * kScorePages + warp * 32;
     if (r.n <= count || blockIdx.x * kScorePages >= r.n) continue;
     __syncthreads();
-    form_vector(p, query, b, kvh, vec);
+    form_vector<kMaxWarps * 32>(p, query, b, kvh, vec, 16 / static_cast<int>(sizeof(CT)), piece_lanes<CT>(p.a.D),
+              piece_lanes<CT>(p.a.D) ? Bits<CT>::kForth : 1);
     __syncthreads();
     uint32_t* held = ranks + (static_cast<int64_t>(b) * p.a.Hk + kvh) * p.width;
     if (from < r.n)
@@ -341,7 +426,7 @@ __global__ void __launch_bounds__(kThreads)
                     [&](int i, uint32_t rank) { held[i] = rank; });
   }
 }
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kMaxWarps * 32)
     paged_pick_kernel(PagedArgs p, const uint32_t* __restrict__ ranks, int always, int count,
                       int32_t* __restrict__ pages_out) {
   __shared__ PickSmem pick_s;
@@ -351,9 +436,9 @@ __global__ void __launch_bounds__(kThreads)
   const PageRange r = page_range(p, pos);
   int32_t* out = pages_out + static_cast<int64_t>(blockIdx.x) * count;
   if (r.n <= count)
-    list_all(p, pos, r, count, out);
+    list_all<kMaxWarps * 32>(p, pos, r, count, out);
   else
-    pick_pages(ranks + static_cast<int64_t>(blockIdx.x) * p.width, r, count, always, out, &pick_s);
+    pick_pages<kMaxWarps * 32>(ranks + static_cast<int64_t>(blockIdx.x) * p.width, r, count, always, out, &pick_s);
 }
 
 // Pages that a sequence can have in this call.
@@ -372,24 +457,34 @@ cudaError_t select_t(const tla_paged* P, const PagedArgs& p, const void* query, 
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  cfg.blockDim = dim3(kMaxWarps * 32);
   if (most <= kMaxHeld) {
-    // Blocks per pair: as many as leave every SM one block, at least 64 pages each.
+    // Larger blocks for longer sequences: their first one picks alone, and its
+    // rounds and the list's writing go over all pages.
+    auto k = paged_select_kernel<IO, CT, 128>;
+    int warps = 4;
+    if (most > 256) k = paged_select_kernel<IO, CT, 256>, warps = 8;
+    if (most > 1024) k = paged_select_kernel<IO, CT, 512>, warps = 16;
+    // Blocks per pair: up to eight per SM in all, at least two pages per warp.
     int shares = 1;
-    while (shares < kMaxCluster && pairs * shares * 2 <= P->base.ctx->sm_count && most > 64 * shares) shares *= 2;
-    auto k = paged_select_kernel<IO, CT>;
+    while (shares < kMaxCluster && pairs * shares * 2 <= 8 * P->base.ctx->sm_count && most > 2 * warps * shares)
+      shares *= 2;
     const size_t smem = vec + (most > count ? most * sizeof(uint32_t) : 0);
-    if (smem > 48 * 1024) {
-      const cudaError_t e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem));
-      if (e != cudaSuccess) return e;
-    }
+    cudaError_t e;
+    if (smem > 48 * 1024 && (e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem))) != cudaSuccess)
+      return e;
+    if (shares > 8 &&  // more than the cluster that every kernel may ask for
+        (e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) !=
+            cudaSuccess)
+      return e;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = shares;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(pairs * shares));
+    cfg.blockDim = dim3(warps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, k, p, static_cast<const IO*>(query), first, last, count, pages_out);
@@ -399,7 +494,7 @@ cudaError_t select_t(const tla_paged* P, const PagedArgs& p, const void* query, 
   const cudaError_t e =
       cudaLaunchKernelEx(&cfg, paged_score_kernel<IO, CT>, p, static_cast<const IO*>(query), first, last, count, ranks);
   if (e != cudaSuccess) return e;
-  return launch_pdl(paged_pick_kernel, static_cast<unsigned>(pairs), kThreads, 0, stream, p,
+  return launch_pdl(paged_pick_kernel, static_cast<unsigned>(pairs), kMaxWarps * 32, 0, stream, p,
                     static_cast<const uint32_t*>(ranks), first + last, count, pages_out);
 }
 
