@@ -133,11 +133,15 @@ class PagedAttention:
 
     def _sequences(self, positions, page_table):
         """(batch, table width) of a call."""
-        if positions.dim() != 1 or page_table.dim() != 2:
-            raise ValueError("positions must be [batch] and page_table [batch, width]")
-        batch, width = positions.shape[0], page_table.shape[1]
-        self._ints(positions, "positions", (batch,))
-        self._ints(page_table, "page_table", (batch, width))
+        try:
+            (batch,), (rows, width) = positions.shape, page_table.shape
+        except ValueError:
+            raise ValueError("positions must be [batch] and page_table [batch, width]") from None
+        if (positions.dtype is not torch.int32 or page_table.dtype is not torch.int32
+                or positions.get_device() != self._index or page_table.get_device() != self._index
+                or not positions.is_contiguous() or not page_table.is_contiguous() or rows != batch):
+            self._ints(positions, "positions", (batch,))
+            self._ints(page_table, "page_table", (batch, width))
         return batch, width
 
     def _on(self, stream):
@@ -148,14 +152,15 @@ class PagedAttention:
             raise ValueError("the stream and the pages are on different devices")
         return stream.cuda_stream
 
-    def _new(self, shape, dtype, stream):
-        """A tensor that belongs to the call's stream."""
+    @staticmethod
+    def _new(like, shape, stream, dtype=None):
+        """A tensor on `like`'s device that belongs to the call's stream."""
         if stream is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
         with torch.cuda.stream(stream):
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return like.new_empty(shape, dtype=dtype or like.dtype)
 
-    def _workspace(self, batch, width, count, which, stream):
+    def _workspace(self, like, batch, width, count, which, stream):
         """(the tensor that keeps it, its address, its size) of a call's workspace; which: 0 decode, 1 select."""
         sizes = self._workspace_bytes.get((batch, width, count))
         if sizes is None:
@@ -166,7 +171,7 @@ class PagedAttention:
         size = sizes[which]
         if size == 0:
             return None, None, 0
-        work = self._new(size, torch.uint8, stream)
+        work = self._new(like, size, stream, torch.uint8)
         return work, work.data_ptr(), size
 
     # ---- the operators
@@ -187,7 +192,7 @@ class PagedAttention:
         elif rows != batch:
             raise ValueError(f"{rows} rows for {batch} sequences need row_offsets")
         if query is None:
-            query = self._new((rows, self.qSize), self.dtype, stream)
+            query = self._new(qkv, (rows, self.qSize), stream)
         else:
             self._rows(query, "query", rows, self.qSize)
         rc = self._lib.tla_paged_append(self.handle, qkv.data_ptr(), positions.data_ptr(), offsets,
@@ -198,7 +203,8 @@ class PagedAttention:
 
     def decode(self, query, positions, page_table, pages=None, gate=None, out=None, stream=None):
         """Attention of one new token per sequence: query [batch, headCount * headDim] as append
-        returned it; pages None, or int32 [batch, kvHeadCount, count] as select returned them."""
+        returned it; pages None, or int32 [batch, kvHeadCount, count] as select returned them.
+        The output has the query's shape."""
         on = self._on(stream)
         batch, width = self._sequences(positions, page_table)
         self._rows(query, "query", batch, self.qSize)
@@ -213,10 +219,10 @@ class PagedAttention:
             self._rows(gate, "gate", batch, self.qSize)
             gate = gate.data_ptr()
         if out is None:
-            out = self._new((batch, self.qSize), self.dtype, stream)
+            out = torch.empty_like(query) if stream is None else self._new(query, query.shape, stream)
         else:
             self._rows(out, "out", batch, self.qSize)
-        work, at, size = self._workspace(batch, width, count, 0, stream)
+        work, at, size = self._workspace(query, batch, width, count, 0, stream)
         rc = self._lib.tla_paged_decode(self.handle, query.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
                                         width, listed, count, gate, out.data_ptr(), batch, at, size, on)
         if rc:
@@ -231,10 +237,10 @@ class PagedAttention:
         self._rows(query, "query", batch, self.qSize)
         count = int(count)
         if pages is None:
-            pages = self._new((batch, self.kvHeadCount, max(count, 0)), torch.int32, stream)
+            pages = self._new(query, (batch, self.kvHeadCount, max(count, 0)), stream, torch.int32)
         else:
             self._ints(pages, "pages", (batch, self.kvHeadCount, count))
-        work, at, size = self._workspace(batch, width, 0, 1, stream)
+        work, at, size = self._workspace(query, batch, width, 0, 1, stream)
         rc = self._lib.tla_paged_select(self.handle, query.data_ptr(), positions.data_ptr(), page_table.data_ptr(),
                                         width, int(first), int(last), pages.data_ptr(), count, batch, at, size, on)
         if rc:
