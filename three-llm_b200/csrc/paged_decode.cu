@@ -37,6 +37,7 @@
 // of two and split into two float16 parts, and so is each weight; with both
 // parts multiplied the products carry 22 bits, and the output keeps float32's
 // use for its caller. K and V are exact as stored.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <type_traits>
@@ -45,12 +46,15 @@
 
 namespace tla {
 
+namespace cg = cooperative_groups;
+
 namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxBatch = 1024;  // prefix table in shared memory
 constexpr int kCtasPerSm = 2;
+constexpr int kMaxCluster = 16;
 constexpr int kMaxGrid = 1024;   // segment table of the joining kernel
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNowhere = -(1 << 30);  // first position of 16 tokens that take no part
@@ -80,11 +84,11 @@ struct DecodeParams {
   int subs;        // groups of up to 16 query heads per kv head
   int rows;        // query heads per such group, the last one's may be fewer
   int small_grid;
-  int whole;       // every pair goes to one CTA: nothing is joined
+  int cluster;     // CTAs per pair, joined within their cluster; 0: shares over all pairs
 };
 
 struct SmemLayout {
-  int stages, q, red, meta, prefix, total;
+  int stages, q, red, part, meta, prefix, total;
 };
 template <int D>
 __host__ __device__ inline SmemLayout smem_layout(int rows, int batch, bool split) {
@@ -97,6 +101,8 @@ __host__ __device__ inline SmemLayout smem_layout(int rows, int batch, bool spli
   off += (split ? 2 : 1) * 16 * C::kQPitch;
   s.red = off;
   off += kWarps * rows * (D + 2) * 4;
+  s.part = off;  // the CTA's triple for its cluster
+  off += rows * (D + 2) * 4;
   off = (off + 15) & ~15;
   s.meta = off;
   off += kWarps * C::kStages * C::kGroups * 4;
@@ -190,23 +196,6 @@ __device__ __forceinline__ Seg seg_at(const int* prefix, int b, int pairs, int g
   return s;
 }
 
-// The first pair that starts at or after unit g.
-__device__ __forceinline__ int next_pair(const int* prefix, int batch, int pairs, int g) {
-  if (g >= prefix[batch]) return prefix[batch];
-  int b = 0, n = batch;  // prefix[b] <= g < prefix[b + n]
-  while (n > 1) {
-    const int half = n / 2;
-    if (prefix[b + half] <= g) {
-      b += half;
-      n -= half;
-    } else {
-      n = half;
-    }
-  }
-  const int per = (prefix[b + 1] - prefix[b]) / pairs;
-  return prefix[b] + (g - prefix[b] + per - 1) / per * per;
-}
-
 // 16 bytes to shared memory; zeros instead when `bytes` is 0.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -278,29 +267,59 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   if (tid == 0) prefix[0] = 0;
   griddep_wait();
   griddep_launch_dependents();
-  for (int b = tid; b < p.batch; b += kThreads) {
-    const int pos = p.positions[b];
-    if (pos >= p.capacity && cta == 0) report_error(p.a.error, TLA_ERR_POSITION);
-    spos[b] = pos;
-    prefix[b + 1] = units_of<D>(d, pos);
+  int tb = 0, te = 1;  // the share's units; one segment with a cluster per pair
+  Seg only;
+  int only_b = 0, only_pos = 0;
+  if (d.cluster) {
+    const int all = cta / d.cluster, rank = cta - all * d.cluster;
+    only_b = all / pairs;
+    only_pos = p.positions[only_b];
+    only.pair = all - only_b * pairs;
+    if (only_pos >= p.capacity && tid == 0 && rank == 0) report_error(p.a.error, TLA_ERR_POSITION);
+    only.tiles = walk_of<D>(d, only_pos).tiles;
+    only.lt = rank * only.tiles / d.cluster;
+    only.n = (rank + 1) * only.tiles / d.cluster - only.lt;
+    only.start = 0;
+    only.next = 1;
+    if (only.tiles == 0) {  // (the same for the whole cluster) no sequence: zeros
+      const int kvh = only.pair / d.subs, sub = only.pair - kvh * d.subs;
+      const int h0 = kvh * G + sub * rows, heads = min(rows, (kvh + 1) * G - h0);
+      for (int i = tid; rank == 0 && i < heads * D; i += kThreads)
+        static_cast<IO*>(d.out)[(static_cast<int64_t>(only_b) * Hq + h0) * D + i] = from_f32<IO>(0.f);
+      return;
+    }
+  } else {
+    for (int b = tid; b < p.batch; b += kThreads) {
+      const int pos = p.positions[b];
+      if (pos >= p.capacity && cta == 0) report_error(p.a.error, TLA_ERR_POSITION);
+      spos[b] = pos;
+      prefix[b + 1] = units_of<D>(d, pos);
+    }
+    __syncthreads();
+    if (warp == 0) scan_prefix(prefix, p.batch, lane);
+    __syncthreads();
+    const int total = prefix[p.batch];
+    // rows without a sequence, spread over the whole launch
+    for (int b = cta; b < p.batch; b += gridDim.x)
+      if (prefix[b + 1] == prefix[b])
+        for (int i = tid; i < Hq * D; i += kThreads)
+          static_cast<IO*>(d.out)[static_cast<int64_t>(b) * Hq * D + i] = from_f32<IO>(0.f);
+    const int grid = effective_grid(total, gridDim.x, d.small_grid);
+    if (total == 0 || cta >= grid) return;
+    tb = cta_begin(cta, total, grid);
+    te = cta_begin(cta + 1, total, grid);
+    if (tb >= te) return;
   }
-  __syncthreads();
-  if (warp == 0) scan_prefix(prefix, p.batch, lane);
-  __syncthreads();
-  const int total = prefix[p.batch];
-  // rows without a sequence, spread over the whole launch
-  for (int b = cta; b < p.batch; b += gridDim.x)
-    if (prefix[b + 1] == prefix[b])
-      for (int i = tid; i < Hq * D; i += kThreads)
-        static_cast<IO*>(d.out)[static_cast<int64_t>(b) * Hq * D + i] = from_f32<IO>(0.f);
-  const int grid = effective_grid(total, gridDim.x, d.small_grid);
-  if (total == 0 || cta >= grid) return;
-  int tb = cta_begin(cta, total, grid), te = cta_begin(cta + 1, total, grid);
-  if (d.whole) {
-    tb = next_pair(prefix, p.batch, pairs, tb);
-    te = next_pair(prefix, p.batch, pairs, te);
-  }
-  if (tb >= te) return;
+  // the segment at unit g, *b its sequence (found from the one before)
+  auto segment = [&](int* b, int g) -> Seg {
+    if (d.cluster) {
+      *b = only_b;
+      return only;
+    }
+    while (prefix[*b + 1] <= g) ++*b;
+    return seg_at<D>(prefix, *b, pairs, g, te);
+  };
+  auto walk = [&](int b) -> Walk { return walk_of<D>(d, d.cluster ? only_pos : spos[b]); };
   const int shift = p.page_shift, mask = (1 << shift) - 1;
 
   // ================================================================== copies
@@ -337,13 +356,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   const int64_t apart = static_cast<const CT*>(p.value) - static_cast<const CT*>(p.key);
   auto load_next = [&](int stage) {
     while (ld.it >= ld.end && ld.g < te) {  // on to the segment that holds the tile
-      while (prefix[ld.b + 1] <= ld.g) ++ld.b;
-      const Seg sg = seg_at<D>(prefix, ld.b, pairs, ld.g, te);
+      const Seg sg = segment(&ld.b, ld.g);
       ld.g = sg.next;
       ld.begin = ld.end;
       ld.end += sg.n;
       if (ld.it >= ld.end) continue;
-      const Walk w = walk_of<D>(d, spos[ld.b]);
+      const Walk w = walk(ld.b);
       const int kvh = sg.pair / d.subs, last_page = w.hi >> shift;
       ld.list = d.pages ? d.pages + (static_cast<int64_t>(ld.b) * p.a.Hk + kvh) * d.count : nullptr;
       ld.head = kvh * p.head_stride + lane_from;
@@ -429,15 +447,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   int it0 = 0, stage = 0;  // the share's tiles before this segment; the ring's oldest tile
   int b = 0;
   for (int g = tb; g < te;) {
-    while (prefix[b + 1] <= g) ++b;
-    const Seg sg = seg_at<D>(prefix, b, pairs, g, te);
-    if (sg.n == 0) {  // the share ends inside the pair's set-up units
+    const Seg sg = segment(&b, g);
+    if (sg.n == 0 && !d.cluster) {  // the share ends inside the pair's set-up units
       g = sg.next;
       continue;
     }
     const int kvh = sg.pair / d.subs, sub = sg.pair - kvh * d.subs;
     const int h0 = kvh * G + sub * rows, heads = min(rows, (kvh + 1) * G - h0);
-    const Walk w = walk_of<D>(d, spos[b]);
+    const Walk w = walk(b);
     const IO* q = static_cast<const IO*>(d.query) + (static_cast<int64_t>(b) * Hq + h0) * D;
     // ---- the group's queries, 8 elements per thread and trip; rows past the group are zeros
     if constexpr (SPLIT) {
@@ -647,8 +664,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         }
       }
     __syncthreads();
-    const bool whole = sg.lt == 0 && sg.n == sg.tiles;
-    float* mine = d.scratch + (static_cast<size_t>(cta) * 2 + (g == tb ? 0 : 1)) * rows * (D + 2);
+    const bool whole = d.cluster ? d.cluster == 1 : sg.lt == 0 && sg.n == sg.tiles;
+    float* mine = d.cluster ? reinterpret_cast<float*>(smem + L.part)
+                            : d.scratch + (static_cast<size_t>(cta) * 2 + (g == tb ? 0 : 1)) * rows * (D + 2);
     for (int i = tid; i < heads * (D / 2); i += kThreads) {  // two columns each
       const int r = i / (D / 2), c = i % (D / 2) * 2;
       float2 ml[kWarps];
@@ -675,6 +693,44 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     }
     __syncthreads();  // red and q_s are free for the next segment
     g = sg.next;
+  }
+
+  if (d.cluster > 1) {  // join the cluster's triples, a part of the columns in each of its CTAs
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int kvh = only.pair / d.subs, sub = only.pair - kvh * d.subs;
+    const int h0 = kvh * G + sub * rows, heads = min(rows, (kvh + 1) * G - h0);
+    float* part = reinterpret_cast<float*>(smem + L.part);
+    for (int i = cluster.block_rank() * kThreads + tid; i < heads * (D / 2); i += d.cluster * kThreads) {
+      const int r = i / (D / 2), c = i % (D / 2) * 2;
+      float2 ml[kMaxCluster], x[kMaxCluster];
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kMaxCluster; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+        x[k] = make_float2(0.f, 0.f);
+        if (k < d.cluster) {
+          const float* of = cluster.map_shared_rank(part, k) + r * (D + 2);
+          ml[k] = *reinterpret_cast<const float2*>(of);
+          x[k] = *reinterpret_cast<const float2*>(of + 2 + c);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kMaxCluster; ++k) top = fmaxf(top, ml[k].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, v0 = 0.f, v1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < kMaxCluster; ++k) {
+        const float f = ex2(ml[k].x - base);
+        sum += ml[k].y * f;
+        v0 += x[k].x * f;
+        v1 += x[k].y * f;
+      }
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * D + c, v0 * inv);
+      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * D + c + 1, v1 * inv);
+    }
+    cluster.sync();  // the others may still read this CTA's triple
   }
 }
 
@@ -796,6 +852,25 @@ cudaError_t launch_t(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   const int smem = smem_layout<D>(d.rows, d.p.batch, SPLIT).total;
   cudaError_t e = raise_smem_limit(k, smem);
   if (e != cudaSuccess) return e;
+  if (d.cluster) {
+    if (d.cluster > 8 &&  // more than the cluster that every kernel may ask for
+        (e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
+      return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(d.p.batch) * P->base.Hk * d.subs * d.cluster);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = d.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = d.cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, d);
+  }
   // two CTAs per SM by registers (the launch bounds), if shared memory holds
   // two (228 KB, 1 KB of it reserved per CTA)
   int per_sm = 228 * 1024 / (smem + 1024);
@@ -803,7 +878,7 @@ cudaError_t launch_t(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   const int grid = per_sm * P->base.ctx->sm_count;
   d.small_grid = P->base.ctx->sm_count;
   e = launch_pdl(kernel, grid, kThreads, smem, stream, d);
-  if (e != cudaSuccess || d.whole) return e;
+  if (e != cudaSuccess) return e;
   return launch_pdl(paged_decode_join_kernel<D, IO>, static_cast<unsigned>(d.p.batch) * P->base.Hq, kJoinWarps * 32, 0,
                     stream, d, grid);
 }
@@ -850,15 +925,17 @@ long long most_tiles(const PagedArgs& p, int count) {
   return tiles;
 }
 
-// Short calls give every pair to one CTA and need no second kernel: where a
-// pair has at most 16 tiles (8 sequences of 4 query heads per kv head at
-// head_dim 64: 257 tokens 8.4 us against 9.3 with shares; 513 tokens 10.5
-// against 10.0, which the launch saved outweighs for the caller), or at most
-// 32 when there are pairs for every CTA (64 such sequences of 513 tokens: 22.4
-// us against 26.7; at 1025 tokens and ragged lengths shares win again).
-bool whole_pairs(const tla_paged* P, const PagedArgs& p, int count) {
+#ifndef TGT
+#define TGT 16
+#endif
+#ifndef ACC
+#define ACC 40
+#endif
+int cluster_size(const tla_paged* P, const PagedArgs& p, int count) {
   const long long tiles = most_tiles(p, count), pairs = static_cast<long long>(p.batch) * p.a.Hk * subgroups(P);
-  return tiles <= 16 || (tiles <= 32 && pairs >= kCtasPerSm * P->base.ctx->sm_count);
+  int n = 1;
+  while (n < kMaxCluster && tiles > TGT * n && pairs * n * 2 <= kCtasPerSm * P->base.ctx->sm_count) n *= 2;
+  return tiles <= ACC * n ? n : 0;
 }
 
 // Whether a call's shares can be cut: the batch's table fits shared memory and
@@ -869,7 +946,7 @@ bool paged_decode_takes(const tla_paged* P, const PagedArgs& p, int count) {
 }
 
 size_t paged_decode_workspace(const tla_paged* P, const PagedArgs& p, int count) {
-  if (whole_pairs(P, p, count)) return 0;
+  if (cluster_size(P, p, count) > 0) return 0;
   return static_cast<size_t>(kCtasPerSm) * P->base.ctx->sm_count * 2 * subgroup_rows(P) * (P->base.D + 2) *
          sizeof(float);
 }
@@ -887,7 +964,7 @@ cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const vo
   d.subs = subgroups(P);
   d.rows = subgroup_rows(P);
   d.small_grid = 0;
-  d.whole = whole_pairs(P, p, count) ? 1 : 0;
+  d.cluster = cluster_size(P, p, count);
   return P->base.D == 64 ? launch_d<64>(P, d, stream) : launch_d<128>(P, d, stream);
 }
 
