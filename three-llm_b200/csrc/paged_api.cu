@@ -1,6 +1,8 @@
 // C ABI of the paged key-value cache: layers over a caller's page pool,
 // argument checks and dispatch. No entry point allocates after
 // tla_paged_create or keeps anything between calls.
+#include <math.h>
+
 #include <new>
 #include <utility>
 
@@ -21,6 +23,7 @@ PagedArgs paged_args(const tla_paged* P, const int32_t* positions, const int32_t
   p.slot_stride = P->pool.slot_stride;
   p.table = table;
   p.positions = positions;
+  p.turns = P->d_turns;
   p.width = width;
   p.batch = batch;
   p.page_count = P->pool.page_count;
@@ -116,6 +119,19 @@ int tla_paged_create(tla_ctx* ctx, const tla_attn_config* cfg, const tla_page_po
             (pool->page_size == 1 || pool->slot_stride % vec == 0);
   tla::paged_decode_configure(P);
   rc = tla::layer_tables(&P->base, inv, q_norm_weight, k_norm_weight);
+  const int half = L.rotary / 2;
+  if (rc == TLA_OK && half > 0) {
+    std::vector<float2> turns(static_cast<size_t>(tla::kTurnSteps) * half);
+    for (int s = 0; s < tla::kTurnSteps; ++s)
+      for (int j = 0; j < half; ++j) {
+        const double angle = j < L.pair_count ? s * static_cast<double>(inv[j]) : 0.0;
+        turns[static_cast<size_t>(s) * half + j] =
+            make_float2(static_cast<float>(cos(angle)), static_cast<float>(sin(angle)));
+      }
+    rc = tla::dev_alloc(&P->d_turns, turns.size());
+    if (rc == TLA_OK)
+      rc = from_cuda(cudaMemcpy(P->d_turns, turns.data(), turns.size() * sizeof(float2), cudaMemcpyHostToDevice));
+  }
   if (rc != TLA_OK) {
     tla_paged_destroy(P);
     return rc;
@@ -131,6 +147,7 @@ int tla_paged_create(tla_ctx* ctx, const tla_attn_config* cfg, const tla_page_po
 int tla_paged_destroy(tla_paged* P) {
   if (!P) return TLA_OK;
   DeviceGuard g(P->base.ctx->device);
+  cudaFree(P->d_turns);
   cudaFree(P->base.d_inv_freq);
   cudaFree(P->base.d_qnorm);
   cudaFree(P->base.d_knorm);

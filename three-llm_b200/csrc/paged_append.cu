@@ -198,27 +198,27 @@ __device__ __forceinline__ float4 high4(float4 a, float4 b) {
 // lane needs another's; dimensions past the rotary ones pair up among
 // themselves and stay). `parts` warps share a row's heads, so that few rows
 // still fill the GPU; a warp forms the row's cosines and sines once, one or
-// two per lane, and hands them out by shuffles. Rows of a long prompt are
-// bound by memory (about 60 instructions per lane and 16 bytes read).
+// two per lane, and hands them out by shuffles. Without `keys` the row's keys
+// are left to the blocks that go by pages. `unit`: the warp's (row, part).
 template <typename IO, typename CT, int D>
-__global__ void __launch_bounds__(kThreads, 5)
-    paged_append_rows_kernel(PagedArgs p, const IO* __restrict__ qkv, const int32_t* __restrict__ offsets, int rows,
-                             IO* __restrict__ query_out, int parts, int part_heads) {
+__device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __restrict__ qkv,
+                                            const int32_t* __restrict__ offsets, int rows,
+                                            IO* __restrict__ query_out, int parts, int part_heads, bool keys,
+                                            int64_t unit) {
   constexpr int kLanes = D / 8, kPer = 32 / kLanes;  // lanes per head, heads per warp-wide load
   constexpr int kLoads = sizeof(IO) == 2 ? 4 : 2;    // warp-wide loads in flight
   const unsigned full = 0xffffffffu;
   const LayerArgs& a = p.a;
   const int Hq = a.Hq, Hk = a.Hk, heads = Hq + 2 * Hk, half = a.rotary / 2;
   const int lane = threadIdx.x & 31, group = lane / kLanes, i0 = 4 * (lane % kLanes);
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
   const int row = static_cast<int>(unit / parts), part = static_cast<int>(unit % parts);
   // the first elements of the lane's four pairs, and their partners
   const int d0 = i0 < half ? i0 : a.rotary + i0 - half;
   const int d1 = d0 + (i0 < half ? half : (D - a.rotary) / 2);
-  griddep_wait();
-  griddep_launch_dependents();
   if (row >= rows) return;
-  const int h_begin = part * part_heads, h_end = min(heads, h_begin + part_heads);
+  // the part's heads: queries, keys (or none), values
+  const int k_heads = keys ? Hk : 0, h_begin = part * part_heads;
+  const int h_end = min(Hq + k_heads + Hk, h_begin + part_heads);
   const IO* src = qkv + static_cast<int64_t>(row) * heads * D;
   const int b = sequence_of_warp(offsets, p.batch, row, lane);
   if (b < 0) return;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 5)
   // (a part with queries only does not need the page)
   const int page = h_end > Hq ? pool_page(p, b, pos >> p.page_shift) : -1;
   float cos4[4], sin4[4];
-  if (h_begin < Hq + Hk) {
+  if (h_begin < Hq + k_heads) {
     float c0 = 1.f, s0 = 0.f, c1 = 1.f, s1 = 0.f;
     if (lane < min(a.pair_count, half)) rope_cos_sin(pos, a.inv_freq[lane], &c0, &s0);
     if (D == 128 && lane + 32 < min(a.pair_count, half)) rope_cos_sin(pos, a.inv_freq[lane + 32], &c1, &s1);
@@ -339,41 +339,9 @@ __global__ void __launch_bounds__(kThreads, 5)
     }
   };
   heads_of(std::integral_constant<int, 0>(), h_begin, min(h_end, Hq), a.q_norm, a.q_norm != nullptr);
-  heads_of(std::integral_constant<int, 1>(), max(h_begin, Hq), min(h_end, Hq + Hk), a.k_norm, a.k_norm != nullptr);
-  heads_of(std::integral_constant<int, 2>(), max(h_begin, Hq + Hk), h_end, nullptr, a.v_norm != 0);
-}
-
-// Smaller and larger elements of 16 bytes.
-__device__ __forceinline__ uint32_t low_pair(uint32_t a, uint32_t b, __half) {
-  const __half2 v = __hmin2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t high_pair(uint32_t a, uint32_t b, __half) {
-  const __half2 v = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t low_pair(uint32_t a, uint32_t b, __nv_bfloat16) {
-  const __nv_bfloat162 v = __hmin2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t high_pair(uint32_t a, uint32_t b, __nv_bfloat16) {
-  const __nv_bfloat162 v = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t low_pair(uint32_t a, uint32_t b, float) {
-  return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b)));
-}
-__device__ __forceinline__ uint32_t high_pair(uint32_t a, uint32_t b, float) {
-  return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
-}
-template <typename CT>
-__device__ __forceinline__ uint4 low_vec(uint4 a, uint4 b) {
-  return make_uint4(low_pair(a.x, b.x, CT()), low_pair(a.y, b.y, CT()), low_pair(a.z, b.z, CT()), low_pair(a.w, b.w, CT()));
-}
-template <typename CT>
-__device__ __forceinline__ uint4 high_vec(uint4 a, uint4 b) {
-  return make_uint4(high_pair(a.x, b.x, CT()), high_pair(a.y, b.y, CT()), high_pair(a.z, b.z, CT()),
-                    high_pair(a.w, b.w, CT()));
+  heads_of(std::integral_constant<int, 1>(), max(h_begin, Hq), min(h_end, Hq + k_heads), a.k_norm, a.k_norm != nullptr);
+  const int skipped = Hk - k_heads;
+  heads_of(std::integral_constant<int, 2>(), max(h_begin + skipped, Hq + Hk), h_end + skipped, nullptr, a.v_norm != 0);
 }
 
 // Pages that sequence b's chunk goes to (0: none), its rows cut off where the
@@ -391,42 +359,30 @@ __device__ __forceinline__ int pages_of(const PagedArgs& p, const Chunk& c) {
   return c.n == 0 ? 0 : ((c.start + c.n - 1) >> p.page_shift) - (c.start >> p.page_shift) + 1;
 }
 
-// Bounds of the pages that the chunks went to, from the keys as stored, which
-// L2 still holds: a block per touched page and two kv heads, four warps per
-// head, their lanes over 16 bytes of a row each and over the rows: a 64-token
-// page's reads are all in flight at once, since latency is what this pass
-// costs. Block k finds the k-th touched page by a scan of the sequences' page
-// counts.
-constexpr int kBoundsHeads = 2, kBoundsWarps = 4;
-template <typename CT, int D>
-__global__ void __launch_bounds__(kBoundsHeads * kBoundsWarps * 32)
-    paged_bounds_rows_kernel(PagedArgs p, const int32_t* __restrict__ offsets, int rows) {
-  constexpr int kVec = 16 / sizeof(CT), kLanes = D / kVec, kRows = 32 / kLanes;
-  const unsigned full = 0xffffffffu;
-  __shared__ int sums[kBoundsHeads * kBoundsWarps];
+// The touched page of a launch that a block works on: page `want` of all the
+// chunks' touched pages in order, found by a scan of the sequences' page
+// counts. False when there are fewer.
+template <int kBlock>
+__device__ __forceinline__ bool find_page(const PagedArgs& p, const int32_t* offsets, int rows, int want, int* b_out,
+                                          int* nth) {
+  __shared__ int sums[kBlock / 32];
   __shared__ int found[2];
-  __shared__ uint4 part_s[kBoundsHeads][kBoundsWarps][2][kLanes];
-  griddep_wait();
-  griddep_launch_dependents();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, Hk = p.a.Hk, threads = blockDim.x;
-  const int groups = (Hk + kBoundsHeads - 1) / kBoundsHeads;
-  const int want = blockIdx.x / groups, head = warp / kBoundsWarps, w = warp % kBoundsWarps;
-  const int kvh = (blockIdx.x - want * groups) * kBoundsHeads + head;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int before = 0;
   if (tid == 0) found[0] = -1;
-  for (int base = 0; base < p.batch; base += threads) {
+  for (int base = 0; base < p.batch; base += kBlock) {
     const int b = base + tid;
     const int n = b < p.batch ? pages_of(p, chunk_of(p, offsets, rows, b)) : 0;
     int scan = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(full, scan, o);
+      const int v = __shfl_up_sync(0xffffffffu, scan, o);
       if (lane >= o) scan += v;
     }
     if (lane == 31) sums[warp] = scan;
     __syncthreads();
     int all = 0;
-    for (int i = 0; i < threads / 32; ++i) {
+    for (int i = 0; i < kBlock / 32; ++i) {
       if (i < warp) scan += sums[i];
       all += sums[i];
     }
@@ -439,60 +395,181 @@ __global__ void __launch_bounds__(kBoundsHeads * kBoundsWarps * 32)
     __syncthreads();
     if (found[0] >= 0) break;
   }
-  const int b = found[0];
-  if (b < 0) return;
+  *b_out = found[0];
+  *nth = found[1];
+  return found[0] >= 0;
+}
+
+// The keys of one touched page and `heads` kv heads (1, 2, 4 or 8), and the
+// page's bounds: 8 / heads warps per head keep the smallest and largest keys
+// in registers while they rotate and store them. The cosines and
+// sines of kPageSlots slots are formed in shared memory at a time, from those
+// of the first slot and a table of those of 0 .. kPageSlots - 1 steps:
+// cos(a + b) = cos a cos b - sin a sin b and its like add three roundings and
+// spare 31 of 32 evaluations, which with few rows per block would bound it.
+constexpr int kPageThreads = 256, kPageSlots = kTurnSteps;
+template <typename IO, typename CT, int D>
+__device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __restrict__ qkv,
+                                            const int32_t* __restrict__ offsets, int rows, int heads, int unit) {
+  constexpr int kLanes = D / 8, kPer = 32 / kLanes, kWarps = kPageThreads / 32;
+  constexpr int kLoads = 4;  // warp-wide loads in flight
+  const unsigned full = 0xffffffffu;
+  __shared__ float2 base_s[D / 2];
+  __shared__ float2 turn_s[kPageSlots][D / 2];
+  __shared__ __align__(16) float join_s[kWarps][2][D];
+  const LayerArgs& a = p.a;
+  const int Hk = a.Hk, half = a.rotary / 2, pairs = min(a.pair_count, half);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = lane / kLanes, i0 = 4 * (lane % kLanes);
+  const int groups = (Hk + heads - 1) / heads;
+  int b, nth;
+  if (!find_page<kPageThreads>(p, offsets, rows, unit / groups, &b, &nth)) return;
   const Chunk c = chunk_of(p, offsets, rows, b);
-  const int index = (c.start >> p.page_shift) + found[1], size = 1 << p.page_shift;
-  const int page = p.table[static_cast<int64_t>(b) * p.width + index];
-  if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.page_count)) return;  // reported by the append
-  // the page's new slots
-  const int64_t from = static_cast<int64_t>(index) << p.page_shift;
+  const int index = (c.start >> p.page_shift) + nth, size = 1 << p.page_shift;
+  const int page = pool_page(p, b, index);
+  if (page < 0) return;
+  const int64_t from = static_cast<int64_t>(index) << p.page_shift;  // the position of slot 0
   const int begin = static_cast<int>(max(static_cast<int64_t>(0), c.start - from));
   const int end = static_cast<int>(min(static_cast<int64_t>(size), c.start + static_cast<int64_t>(c.n) - from));
-  const int d = (lane % kLanes) * kVec, r = w * kRows + lane / kLanes;
-  if (kvh < Hk) {
-    const CT* key = static_cast<const CT*>(p.key) + pool_row(p, page, kvh, 0) + d;
-    // rows past the end repeat the last one: the smallest and largest stay
-    uint4 low = *reinterpret_cast<const uint4*>(key + min(begin + r, end - 1) * p.slot_stride), high = low;
-#pragma unroll 8
-    for (int s = begin + r + kBoundsWarps * kRows; s < end; s += kBoundsWarps * kRows) {
-      const uint4 u = *reinterpret_cast<const uint4*>(key + s * p.slot_stride);
-      low = low_vec<CT>(low, u);
-      high = high_vec<CT>(high, u);
+  const int64_t row0 = c.row + from - c.start;  // the row of slot 0 (of slots >= begin)
+  const int d0 = i0 < half ? i0 : a.rotary + i0 - half;
+  const int d1 = d0 + (i0 < half ? half : (D - a.rotary) / 2);
+  const int shares = kWarps / heads, share = warp / heads;  // warps per head, and this one's place
+  const int kvh = unit % groups * heads + warp % heads;
+  const int row_size = (a.Hq + 2 * Hk) * D;
+  float4 low0 = make_float4(INFINITY, INFINITY, INFINITY, INFINITY), low1 = low0;
+  float4 high0 = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), high1 = high0;
+  for (int s0 = begin; s0 < end; s0 += kPageSlots) {
+    const int slots = min(kPageSlots, end - s0);
+    __syncthreads();
+    for (int j = tid; j < pairs; j += kPageThreads) {
+      float cs, sn;
+      rope_cos_sin(static_cast<int>(from + s0), a.inv_freq[j], &cs, &sn);
+      base_s[j] = make_float2(cs * a.attn_factor, sn * a.attn_factor);
     }
+    __syncthreads();
+    for (int i = tid; i < slots * (D / 2); i += kPageThreads) {
+      const int s = i / (D / 2), j = i - s * (D / 2);
+      float2 v = make_float2(1.f, 0.f);
+      if (j < pairs) {
+        const float2 x = base_s[j], y = p.turns[s * half + j];
+        v = make_float2(x.x * y.x - x.y * y.y, x.y * y.x + x.x * y.y);
+      }
+      turn_s[s][j] = v;
+    }
+    __syncthreads();
+    if (kvh >= Hk) continue;
+    const IO* in = qkv + (row0 + s0) * row_size + (a.Hq + kvh) * D;
+    CT* out = static_cast<CT*>(p.key) + pool_row(p, page, kvh, s0);
+    for (int s1 = share * kPer + group; s1 - group < slots; s1 += shares * kPer * kLoads) {
+      Raw4<IO> lo[kLoads], hi[kLoads];
 #pragma unroll
-    for (int o = kLanes; o < 32; o <<= 1) {
-      const uint4 a = make_uint4(__shfl_xor_sync(full, low.x, o), __shfl_xor_sync(full, low.y, o),
-                                 __shfl_xor_sync(full, low.z, o), __shfl_xor_sync(full, low.w, o));
-      const uint4 h = make_uint4(__shfl_xor_sync(full, high.x, o), __shfl_xor_sync(full, high.y, o),
-                                 __shfl_xor_sync(full, high.z, o), __shfl_xor_sync(full, high.w, o));
-      low = low_vec<CT>(low, a);
-      high = high_vec<CT>(high, h);
+      for (int k = 0; k < kLoads; ++k) {
+        const int s = s1 + k * shares * kPer;
+        lo[k] = s < slots ? raw4(in + static_cast<int64_t>(s) * row_size + d0) : Raw4<IO>{};
+        hi[k] = s < slots ? raw4(in + static_cast<int64_t>(s) * row_size + d1) : Raw4<IO>{};
+      }
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k) {
+        const int s = s1 + k * shares * kPer;
+        float4 xf = floats(lo[k]), yf = floats(hi[k]);
+        float x[4] = {xf.x, xf.y, xf.z, xf.w}, y[4] = {yf.x, yf.y, yf.z, yf.w};
+        if (a.k_norm) {  // math.ts:78-97
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ss += x[e] * x[e] + y[e] * y[e];
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(full, ss, o);
+          const float r = rsqrtf(ss * (1.f / D) + a.rms_eps);  // (2 ulp)
+          const float add = a.offset_rms ? 1.f : 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] *= r * (add + __ldg(a.k_norm + d0 + e));
+            y[e] *= r * (add + __ldg(a.k_norm + d1 + e));
+          }
+        }
+        if (s >= slots) continue;
+        if (i0 < half) {  // RoPE, math.ts:134-147
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 t = turn_s[s][i0 + e];
+            const float u = x[e] * t.x - y[e] * t.y;
+            y[e] = y[e] * t.x + x[e] * t.y;
+            x[e] = u;
+          }
+        }
+        xf = as_stored<CT>(make_float4(x[0], x[1], x[2], x[3]));
+        yf = as_stored<CT>(make_float4(y[0], y[1], y[2], y[3]));
+        store4(out + s * p.slot_stride + d0, xf);
+        store4(out + s * p.slot_stride + d1, yf);
+        low0 = low4(low0, xf);
+        low1 = low4(low1, yf);
+        high0 = high4(high0, xf);
+        high1 = high4(high1, yf);
+      }
     }
-    if (lane < kLanes) {
-      part_s[head][w][0][lane] = low;
-      part_s[head][w][1][lane] = high;
-    }
+  }
+  // across the lanes' slots, then the warps of a head
+#pragma unroll
+  for (int o = kLanes; o < 32; o <<= 1) {
+    auto from_lane = [&](float4 v) {
+      return make_float4(__shfl_xor_sync(full, v.x, o), __shfl_xor_sync(full, v.y, o), __shfl_xor_sync(full, v.z, o),
+                         __shfl_xor_sync(full, v.w, o));
+    };
+    low0 = low4(low0, from_lane(low0));
+    low1 = low4(low1, from_lane(low1));
+    high0 = high4(high0, from_lane(high0));
+    high1 = high4(high1, from_lane(high1));
+  }
+  if (group == 0) {
+    *reinterpret_cast<float4*>(&join_s[warp][0][d0]) = low0;
+    *reinterpret_cast<float4*>(&join_s[warp][0][d1]) = low1;
+    *reinterpret_cast<float4*>(&join_s[warp][1][d0]) = high0;
+    *reinterpret_cast<float4*>(&join_s[warp][1][d1]) = high1;
   }
   __syncthreads();
-  if (kvh >= Hk || w != 0) return;
-  // the first lanes join the lows, the next the highs
-  for (int i = lane; i < 2 * kLanes; i += 32) {
-    const bool is_low = i < kLanes;
-    const int at = is_low ? i : i - kLanes;
-    uint4 v = part_s[head][0][is_low ? 0 : 1][at];
-#pragma unroll
-    for (int k = 1; k < kBoundsWarps; ++k) {
-      const uint4 u = part_s[head][k][is_low ? 0 : 1][at];
-      v = is_low ? low_vec<CT>(v, u) : high_vec<CT>(v, u);
+  for (int i = tid; i < heads * 2 * D; i += kPageThreads) {  // [head][low, high][d]
+    const int h = i / (2 * D), at = i - h * 2 * D, head = unit % groups * heads + h;
+    const bool is_low = at < D;
+    const int e = is_low ? at : at - D;
+    if (head >= Hk) continue;
+    float v = join_s[h][is_low ? 0 : 1][e];
+    for (int k = 1; k < shares; ++k) {
+      const float u = join_s[h + k * heads][is_low ? 0 : 1][e];
+      v = (is_low ? u < v : u > v) ? u : v;
     }
-    CT* out = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D + (is_low ? 0 : D) + at * kVec;
+    CT* to = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + head) * 2 * D + at;
     if (begin > 0) {
-      const uint4 u = *reinterpret_cast<const uint4*>(out);
-      v = is_low ? low_vec<CT>(v, u) : high_vec<CT>(v, u);
+      const float u = to_f32(to[0]);
+      v = (is_low ? v < u : v > u) ? v : u;
     }
-    *reinterpret_cast<uint4*>(out) = v;
+    to[0] = from_f32<CT>(v);
   }
+}
+
+// Rows only.
+template <typename IO, typename CT, int D>
+__global__ void __launch_bounds__(kThreads, 5)
+    paged_append_rows_kernel(PagedArgs p, const IO* __restrict__ qkv, const int32_t* __restrict__ offsets, int rows,
+                             IO* __restrict__ query_out, int parts, int part_heads) {
+  griddep_wait();
+  griddep_launch_dependents();
+  append_rows<IO, CT, D>(p, qkv, offsets, rows, query_out, parts, part_heads, true,
+                         static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5));
+}
+
+// Chunks into a pool with bounds: the first blocks take the touched pages'
+// keys, the others the rows' queries and values.
+template <typename IO, typename CT, int D>
+__global__ void __launch_bounds__(kPageThreads, 3)
+    paged_append_chunks_kernel(PagedArgs p, const IO* __restrict__ qkv, const int32_t* __restrict__ offsets, int rows,
+                               IO* __restrict__ query_out, int parts, int part_heads, int page_blocks, int page_heads) {
+  griddep_wait();
+  griddep_launch_dependents();
+  if (static_cast<int>(blockIdx.x) < page_blocks)
+    append_page<IO, CT, D>(p, qkv, offsets, rows, page_heads, blockIdx.x);
+  else
+    append_rows<IO, CT, D>(p, qkv, offsets, rows, query_out, parts, part_heads, false,
+                           static_cast<int64_t>(blockIdx.x - page_blocks) * (kPageThreads / 32) + (threadIdx.x >> 5));
 }
 
 // Bounds of the pages that a chunk touched, any shape: the block of a page's
@@ -531,47 +608,50 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-template <typename CT>
-cudaError_t bounds_t(const PagedArgs& p, bool rows_ok, const int32_t* offsets, int rows, cudaStream_t stream) {
-  if (!rows_ok) return launch_pdl(paged_bounds_kernel<CT>, rows, kThreads, 0, stream, p, offsets, rows);
-  // a chunk of n rows touches at most (n - 1) / page_size + 2 pages, and no more than its rows
-  const long long pages = min(static_cast<long long>(rows), (static_cast<long long>(rows) >> p.page_shift) + 2LL * p.batch);
-  auto k = p.a.D == 64 ? paged_bounds_rows_kernel<CT, 64> : paged_bounds_rows_kernel<CT, 128>;
-  const int heads = p.a.Hk < kBoundsHeads ? p.a.Hk : kBoundsHeads;
-  return launch_pdl(k, static_cast<unsigned>(pages * ((p.a.Hk + kBoundsHeads - 1) / kBoundsHeads)),
-                    heads * kBoundsWarps * 32, 0, stream, p, offsets, rows);
-}
-
 template <typename IO, typename CT>
 cudaError_t append_t(const tla_paged* P, const PagedArgs& p, const void* qkv, const int32_t* offsets, int rows,
                      void* query_out, cudaStream_t stream) {
-  const int D = p.a.D, heads = p.a.Hq + 2 * p.a.Hk;
-  const bool rows_ok = P->wide && p.a.rotary % 8 == 0;
-  cudaError_t e;
-  if (rows_ok) {
+  const int D = p.a.D;
+  const bool by_pages = p.bounds && offsets;
+  if (P->wide && p.a.rotary % 8 == 0) {
     // Warps per row: enough for 16 on every SM, at most one per warp-wide load
     // (64 rows of 48 heads: 12 warps per row).
-    const int per = 256 / D, most = (heads + per - 1) / per;
+    const int heads = p.a.Hq + (by_pages ? 1 : 2) * p.a.Hk, per = 256 / D, most = (heads + per - 1) / per;
     long long parts = (16LL * P->base.ctx->sm_count + rows - 1) / rows;
     parts = parts < 1 ? 1 : parts > most ? most : parts;
     const int part_heads = (most + static_cast<int>(parts) - 1) / static_cast<int>(parts) * per;
     parts = (heads + part_heads - 1) / part_heads;
-    const unsigned blocks = static_cast<unsigned>((rows * parts + 3) / 4);
-    auto k = D == 64 ? paged_append_rows_kernel<IO, CT, 64> : paged_append_rows_kernel<IO, CT, 128>;
-    e = launch_pdl(k, blocks, kThreads, 0, stream, p, static_cast<const IO*>(qkv), offsets, rows,
-                   static_cast<IO*>(query_out), static_cast<int>(parts), part_heads);
-  } else {
-    const size_t smem = sizeof(float) * (static_cast<size_t>(heads) * D + p.a.rotary);
-    auto k = paged_append_kernel<IO, CT>;
-    if (smem > 48 * 1024) {
-      e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem));
-      if (e != cudaSuccess) return e;
+    if (!by_pages) {
+      auto k = D == 64 ? paged_append_rows_kernel<IO, CT, 64> : paged_append_rows_kernel<IO, CT, 128>;
+      return launch_pdl(k, static_cast<unsigned>((rows * parts + 3) / 4), kThreads, 0, stream, p,
+                        static_cast<const IO*>(qkv), offsets, rows, static_cast<IO*>(query_out),
+                        static_cast<int>(parts), part_heads);
     }
-    e = launch_pdl(k, rows, kThreads, smem, stream, p, static_cast<const IO*>(qkv), offsets, rows,
-                   static_cast<IO*>(query_out));
+    // a chunk of n rows touches at most (n - 1) / page_size + 2 pages, and no more than its rows
+    const long long pages =
+        min(static_cast<long long>(rows), (static_cast<long long>(rows) >> p.page_shift) + 2LL * p.batch);
+    // kv heads per page block: all eight warps on one while that gives no more
+    // than two blocks per SM (one or four: 24 and 23 us for 16 chunks of up to
+    // 500 rows, 48 heads of 64, against 20)
+    int page_heads = 1;
+    while (page_heads < 8 && page_heads < p.a.Hk && pages * ((p.a.Hk + page_heads - 1) / page_heads) > 2 * P->base.ctx->sm_count)
+      page_heads *= 2;
+    const long long blocks = pages * ((p.a.Hk + page_heads - 1) / page_heads);
+    const int warps = kPageThreads / 32;
+    auto k = D == 64 ? paged_append_chunks_kernel<IO, CT, 64> : paged_append_chunks_kernel<IO, CT, 128>;
+    return launch_pdl(k, static_cast<unsigned>(blocks + (rows * parts + warps - 1) / warps), kPageThreads, 0, stream, p,
+                      static_cast<const IO*>(qkv), offsets, rows, static_cast<IO*>(query_out), static_cast<int>(parts),
+                      part_heads, static_cast<int>(blocks), page_heads);
   }
-  if (e != cudaSuccess || !p.bounds || !offsets) return e;
-  return bounds_t<CT>(p, P->wide, offsets, rows, stream);
+  const size_t smem = sizeof(float) * (static_cast<size_t>(p.a.Hq + 2 * p.a.Hk) * D + p.a.rotary);
+  auto k = paged_append_kernel<IO, CT>;
+  cudaError_t e = cudaSuccess;
+  if (smem > 48 * 1024) e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(k, rows, kThreads, smem, stream, p, static_cast<const IO*>(qkv), offsets, rows,
+                 static_cast<IO*>(query_out));
+  if (e != cudaSuccess || !by_pages) return e;
+  return launch_pdl(paged_bounds_kernel<CT>, rows, kThreads, 0, stream, p, offsets, rows);
 }
 
 }  // namespace

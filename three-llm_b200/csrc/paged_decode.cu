@@ -925,17 +925,22 @@ long long most_tiles(const PagedArgs& p, int count) {
   return tiles;
 }
 
-#ifndef TGT
-#define TGT 16
-#endif
-#ifndef ACC
-#define ACC 40
-#endif
+// CTAs per pair when a cluster takes it, 0 when the pairs' tiles are cut into
+// shares. A cluster joins its triples itself: one launch, no workspace, only
+// its own sequence's position to wait for. It gets a CTA per four tiles, up to
+// 16 and up to two CTAs per SM in all. Shares balance unequal lengths and fill
+// every SM; they win where a CTA of a cluster would get many tiles. Measured
+// (shares / cluster, us; head_dim 64, 4 query heads for each of 8 kv heads):
+// 1 x 1025 tokens 6.9 / 5.9, 8 x 4097 18.0 / 16.6, 64 x 1025 35.0 / 29.6; of
+// lengths from a sixteenth up: 64 x 2049 30.7 / 28.5 (65 tiles per CTA), 16 x
+// 2049 12.6 / 13.5 (33), 64 x 4097 45.5 / 48.3; 1 x 8193 8.9 / 9.4 (17, on 128
+// CTAs only).
 int cluster_size(const tla_paged* P, const PagedArgs& p, int count) {
   const long long tiles = most_tiles(p, count), pairs = static_cast<long long>(p.batch) * p.a.Hk * subgroups(P);
+  const int sms = P->base.ctx->sm_count;
   int n = 1;
-  while (n < kMaxCluster && tiles > TGT * n && pairs * n * 2 <= kCtasPerSm * P->base.ctx->sm_count) n *= 2;
-  return tiles <= ACC * n ? n : 0;
+  while (n < kMaxCluster && tiles > 4 * n && pairs * n * 2 <= kCtasPerSm * sms) n *= 2;
+  return tiles <= (pairs * n > sms ? 40 : 20) * n ? n : 0;
 }
 
 // Whether a call's shares can be cut: the batch's table fits shared memory and

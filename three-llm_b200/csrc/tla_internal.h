@@ -65,12 +65,14 @@ struct tla_paged {
   int io = 0, kept = 0;     // tla::Type of the activations and of the pages
   int page_shift = 0;       // log2(page_size)
   bool wide = false;        // head_dim 64 or 128, rows of the pool on 16-byte boundaries
+  float2* d_turns = nullptr;  // [kTurnSteps][rotary / 2]: cos and sin of 0, 1, .. steps of each pair
   bool fast = false;        // tensor-core decode path (paged_decode_configure)
 };
 
 namespace tla {
 
 enum Type { kFp16 = 0, kBf16 = 1, kFp32 = 2 };
+constexpr int kTurnSteps = 32;
 
 // Launch with programmatic dependent launch allowed: the kernel may start
 // while the previous kernel in the stream finishes; it waits (griddep_wait)
@@ -200,6 +202,7 @@ struct PagedArgs {
   int64_t page_stride, head_stride, slot_stride;  // elements
   const int32_t* table;                           // [batch][width]
   const int32_t* positions;                       // [batch]
+  const float2* turns;                            // tla_paged::d_turns
   int width, batch;
   int page_count, page_shift;
   int capacity;  // tokens a sequence can hold: min(max_tokens, width * page_size)
