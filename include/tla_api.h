@@ -340,7 +340,9 @@ int tla_decode_noalloc(const tla_attn_config* config, void* key_cache, void* val
  * The calls are stream-ordered, allocate nothing and hold no state between
  * calls outside the caller's buffers: calls on one layer may run at the same
  * time on several streams as long as no call writes what another reads (give
- * each its own workspace), and all may be captured in CUDA graphs. */
+ * each its own workspace), and all may be captured in CUDA graphs, which the
+ * layer and the pool must outlive. Outputs may not overlap inputs (a gate may
+ * be the output itself). */
 typedef struct tla_page_pool {
   void* key;               /* device; element (page, kv_head, slot, d) at key + page*page_stride + */
   void* value;             /* kv_head*head_stride + slot*slot_stride + d, strides in elements      */

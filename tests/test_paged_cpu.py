@@ -53,6 +53,7 @@ def create(pkg, flags=0, head_dim=64, heads=4, kv_heads=2, key=1 << 20, value=1 
     (dict(strides=(-2048, 1024, 64)), INVALID),
     (dict(strides=(1 << 62, 1024, 64)), INVALID),
     (dict(heads=5), UNSUPPORTED),                          # heads do not divide
+    (dict(heads=65536), UNSUPPORTED),
     (dict(head_dim=257), UNSUPPORTED),
     (dict(kv_heads=8), INVALID),                           # more kv heads than heads
     (dict(flags=(1 << 2) | (1 << 4)), INVALID),            # two I/O types

@@ -4,6 +4,10 @@ sequence is NaN, and the tables' unused entries name no page, so a read of
 either shows. Error bounds come with the reference's outputs; they count each
 rounding, and are derived there."""
 import ctypes
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -539,6 +543,8 @@ def test_python_refuses(pkg, cuda):
         (lambda: layer(key_bounds=None).select(q, pos, table, 2), pkg.TlaError),
         (lambda: layer(options={"attnScale": -1.0}).select(q, pos, table, 2), pkg.TlaError),
         (lambda: layer(options={"maxBatch": 1}).decode(q, pos, table), pkg.TlaError),
+        (lambda: a.decode(q, pos, table, out=q), pkg.TlaError),                              # outputs over inputs
+        (lambda: a.append(qkv, pos, table, query=qkv.view(-1)[512:1536].view(2, 512)), pkg.TlaError),
     ]
     for call, err in bad:
         with pytest.raises(err):
@@ -555,6 +561,24 @@ def test_python_refuses(pkg, cuda):
     for at, size in ((None, 0), (work.data_ptr(), need.value - 1), (work.data_ptr() + 8, need.value)):
         assert pkg.lib().tla_paged_decode(long.handle, q.data_ptr(), pos.data_ptr(), wide.data_ptr(), 4096, None, 0,
                                           None, q.data_ptr(), 2, at, size, None) == -1
+
+
+def test_append_refuses_rows_that_do_not_fit(pkg, cuda):
+    """A head_dim that goes through shared memory row by row, with more heads than it holds."""
+    k, v = (torch.zeros(2, 64, 4, 80, dtype=torch.float16, device=cuda) for _ in range(2))
+    a = pkg.PagedAttention(640 * 80, 640, 8, k, v, {"headDim": 80, "kvHeadCount": 64})
+    with pytest.raises(pkg.TlaError, match="UNSUPPORTED"):
+        a.append(torch.zeros(1, 768 * 80, dtype=torch.float16, device=cuda), ints([0], cuda), ints([[0]], cuda))
+    torch.zeros(1, device=cuda)  # no CUDA error is left behind
+
+
+def test_decode_gate_as_output(pkg, cuda):
+    w = World([70, 40], 2, 64, 16, "fp16")
+    layer, *_ = make(pkg, cuda, w, 8, 2, 64, "fp16")
+    q, gate = (w.normal(2, 512, dtype=torch.float16).to(cuda) for _ in range(2))
+    pos, table = ints([69, 39], cuda), w.device_table(cuda)
+    exp = layer.decode(q, pos, table, gate=gate)
+    assert torch.equal(layer.decode(q, pos, table, gate=gate, out=gate), exp)
 
 
 def test_empty_calls(pkg, cuda):
@@ -720,3 +744,16 @@ def test_repeated_calls_agree_bit_for_bit(pkg, cuda):
     for _ in range(10):
         for a, b in zip(step(layer, qkv, pos, table, 16), first):
             assert torch.equal(a, b)
+
+
+def test_paged_under_bounds_check_build(pkg):
+    """These tests in a fresh process that loads libtla_check.so: no guarded index may leave its buffer."""
+    if os.environ.get("TLA_LIBRARY"):
+        pytest.skip("runs in that process")
+    root = Path(__file__).resolve().parent.parent
+    subprocess.run(["make", "-s", "-j8", "-C", str(root / "three-llm_b200" / "csrc"), "check"], check=True)
+    env = dict(os.environ, TLA_LIBRARY=str(root / "three-llm_b200" / "libtla_check.so"))
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "-p", "no:cacheprovider", "-m", "gpu",
+                        "tests/test_paged_gpu.py"], cwd=root, env=env, capture_output=True, text=True, timeout=900)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
+    assert " passed" in r.stdout

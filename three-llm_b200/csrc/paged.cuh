@@ -6,8 +6,12 @@
 
 namespace tla {
 
-// First element of a (page, kv head, slot) row of the pool.
+// First element of a (page, kv head, slot) row of the pool. (A bounds-check
+// build reports a row outside the pool and hands out row 0.)
 __device__ __forceinline__ int64_t pool_row(const PagedArgs& p, int page, int kvh, int slot) {
+  if (!TLA_IN_BOUNDS(page, p.page_count, p.a.error) || !TLA_IN_BOUNDS(kvh, p.a.Hk, p.a.error) ||
+      !TLA_IN_BOUNDS(slot, 1 << p.page_shift, p.a.error))
+    return 0;
   return page * p.page_stride + kvh * p.head_stride + slot * p.slot_stride;
 }
 

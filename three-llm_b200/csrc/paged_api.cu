@@ -66,6 +66,15 @@ bool rows_apart(const tla_page_pool& pool, int heads, int D) {
   return true;
 }
 
+// Whether [a, a + n) and [b, b + m) share a byte.
+bool overlap(const void* a, size_t n, const void* b, size_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && x < y + m && y < x + n;
+}
+size_t row_bytes(const tla_paged* P, int heads) {
+  return static_cast<size_t>(heads) * P->base.D * (P->io == tla::kFp32 ? 4 : 2);
+}
+
 size_t decode_workspace(const tla_paged* P, const tla::PagedArgs& p, int count) {
   return tla::paged_decode_takes(P, p, count) ? tla::paged_decode_workspace(P, p, count)
                                               : tla::paged_decode_generic_workspace(P, p.batch);
@@ -84,7 +93,8 @@ int tla_paged_create(tla_ctx* ctx, const tla_attn_config* cfg, const tla_page_po
   std::vector<float> inv;
   int rc = tla::layer_params(cfg, &L, &inv);
   if (rc != TLA_OK) return rc;
-  if (L.G == 0) return TLA_ERR_UNSUPPORTED;  // query heads do not divide into the kv heads
+  // query heads that do not divide into the kv heads; more heads than a grid's second dimension
+  if (L.G == 0 || L.Hq > 65535) return TLA_ERR_UNSUPPORTED;
   const uint32_t io_bits = cfg->flags & (TLA_FLAG_IO_FP32 | TLA_FLAG_IO_BF16);
   const uint32_t kept_bits = cfg->flags & (TLA_FLAG_CACHE_FP32 | TLA_FLAG_CACHE_BF16);
   if (io_bits == (TLA_FLAG_IO_FP32 | TLA_FLAG_IO_BF16) || kept_bits == (TLA_FLAG_CACHE_FP32 | TLA_FLAG_CACHE_BF16))
@@ -117,8 +127,9 @@ int tla_paged_create(tla_ctx* ctx, const tla_attn_config* cfg, const tla_page_po
   P->wide = (L.D == 64 || L.D == 128) && aligned16(pool->key) && aligned16(pool->value) &&
             (pool->page_count == 1 || pool->page_stride % vec == 0) && (L.Hk == 1 || pool->head_stride % vec == 0) &&
             (pool->page_size == 1 || pool->slot_stride % vec == 0);
-  tla::paged_decode_configure(P);
-  rc = tla::layer_tables(&P->base, inv, q_norm_weight, k_norm_weight);
+  rc = from_cuda(tla::paged_decode_configure(P));
+  if (rc == TLA_OK && pool->bounds) rc = from_cuda(tla::paged_select_configure(P));
+  if (rc == TLA_OK) rc = tla::layer_tables(&P->base, inv, q_norm_weight, k_norm_weight);
   const int half = L.rotary / 2;
   if (rc == TLA_OK && half > 0) {
     std::vector<float2> turns(static_cast<size_t>(tla::kTurnSteps) * half);
@@ -162,7 +173,10 @@ int tla_paged_append(tla_paged* P, const void* qkv, const int32_t* positions, co
   if (rc != TLA_OK) return rc;
   if (rows < 0 || (rows > 0 && !qkv) || (!row_offsets && rows != batch)) return TLA_ERR_INVALID_ARG;
   if (batch == 0 || rows == 0) return TLA_OK;
-  if (!aligned16(qkv) || !aligned16(query_out)) return TLA_ERR_INVALID_ARG;
+  if (!aligned16(qkv) || !aligned16(query_out) ||
+      overlap(qkv, rows * row_bytes(P, P->base.Hq + 2 * P->base.Hk), query_out, rows * row_bytes(P, P->base.Hq)))
+    return TLA_ERR_INVALID_ARG;
+  if (!tla::paged_append_takes(P)) return TLA_ERR_UNSUPPORTED;
   DeviceGuard g(P->base.ctx->device);
   return from_cuda(tla::launch_paged_append(P, tla::paged_args(P, positions, page_table, table_width, batch), qkv,
                                             row_offsets, rows, query_out, static_cast<cudaStream_t>(stream)));
@@ -184,7 +198,9 @@ int tla_paged_decode(tla_paged* P, const void* query, const int32_t* positions, 
   if (rc != TLA_OK) return rc;
   if (pages ? page_count <= 0 : page_count != 0) return TLA_ERR_INVALID_ARG;
   if (batch == 0) return TLA_OK;
-  if (!query || !out || !aligned16(query) || !aligned16(out) || !aligned16(gate) || !aligned16(workspace))
+  const size_t bytes = batch * row_bytes(P, P->base.Hq);
+  if (!query || !out || !aligned16(query) || !aligned16(out) || !aligned16(gate) || !aligned16(workspace) ||
+      overlap(query, bytes, out, bytes) || (gate != out && overlap(gate, bytes, out, bytes)))
     return TLA_ERR_INVALID_ARG;
   const tla::PagedArgs p = tla::paged_args(P, positions, page_table, table_width, batch);
   const size_t need = decode_workspace(P, p, page_count);

@@ -608,12 +608,19 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+// The layers that append_rows takes.
+bool by_rows(const tla_paged* P) { return P->wide && P->base.rotary % 8 == 0; }
+// Shared memory of the block-per-row kernel: the row in float32, its cosines and sines.
+size_t row_smem(const tla_paged* P) {
+  return sizeof(float) * (static_cast<size_t>(P->base.Hq + 2 * P->base.Hk) * P->base.D + P->base.rotary);
+}
+
 template <typename IO, typename CT>
 cudaError_t append_t(const tla_paged* P, const PagedArgs& p, const void* qkv, const int32_t* offsets, int rows,
                      void* query_out, cudaStream_t stream) {
   const int D = p.a.D;
   const bool by_pages = p.bounds && offsets;
-  if (P->wide && p.a.rotary % 8 == 0) {
+  if (by_rows(P)) {
     // Warps per row: enough for 16 on every SM, at most one per warp-wide load
     // (64 rows of 48 heads: 12 warps per row).
     const int heads = p.a.Hq + (by_pages ? 1 : 2) * p.a.Hk, per = 256 / D, most = (heads + per - 1) / per;
@@ -643,7 +650,7 @@ cudaError_t append_t(const tla_paged* P, const PagedArgs& p, const void* qkv, co
                       static_cast<const IO*>(qkv), offsets, rows, static_cast<IO*>(query_out), static_cast<int>(parts),
                       part_heads, static_cast<int>(blocks), page_heads);
   }
-  const size_t smem = sizeof(float) * (static_cast<size_t>(p.a.Hq + 2 * p.a.Hk) * D + p.a.rotary);
+  const size_t smem = row_smem(P);
   auto k = paged_append_kernel<IO, CT>;
   cudaError_t e = cudaSuccess;
   if (smem > 48 * 1024) e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem));
@@ -655,6 +662,8 @@ cudaError_t append_t(const tla_paged* P, const PagedArgs& p, const void* qkv, co
 }
 
 }  // namespace
+
+bool paged_append_takes(const tla_paged* P) { return by_rows(P) || row_smem(P) <= 227 * 1024; }
 
 cudaError_t launch_paged_append(const tla_paged* P, const PagedArgs& p, const void* qkv, const int32_t* offsets,
                                 int rows, void* query_out, cudaStream_t stream) {

@@ -80,6 +80,7 @@ struct DecodeParams {
   const void* gate;
   void* out;
   float* scratch;  // [grid][2][rows][D + 2]
+  long long scratch_floats;  // its extent (bounds-check builds)
   int count;
   int subs;        // groups of up to 16 query heads per kv head
   int rows;        // query heads per such group, the last one's may be fewer
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const PagedArgs& p = d.p;
   const int Hq = p.a.Hq, G = p.a.G, pairs = p.a.Hk * d.subs, rows = d.rows;
-  const SmemLayout L = smem_layout<D>(rows, p.batch, SPLIT);
+  const SmemLayout L = smem_layout<D>(rows, d.cluster ? 0 : p.batch, SPLIT);
   int* prefix = reinterpret_cast<int*>(smem + L.prefix);
   int* spos = prefix + p.batch + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
@@ -686,7 +687,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
         store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * D + c, v0 * inv);
         store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * D + c + 1, v1 * inv);
-      } else {
+      } else if (d.cluster ||
+                 TLA_IN_BOUNDS(mine - d.scratch + (r + 1) * (D + 2) - 1, d.scratch_floats, p.a.error)) {
         *reinterpret_cast<float2*>(mine + r * (D + 2) + 2 + c) = make_float2(v0, v1);
         if (c == 0) *reinterpret_cast<float2*>(mine + r * (D + 2)) = make_float2(top, sum);
       }
@@ -785,7 +787,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
     float mk[kBatch], lk[kBatch], v[kBatch][kPer];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int at = k + u * warps, slot = at < n ? slot_of[at] : -1;
+      const int at = k + u * warps;
+      int slot = at < n ? slot_of[at] : -1;
+      if (slot >= 0 && !TLA_IN_BOUNDS((static_cast<long long>(slot) + 1) * d.rows * (D + 2) - 1, d.scratch_floats,
+                                      p.a.error))
+        slot = -1;
       mk[u] = -INFINITY;
       lk[u] = 0.f;
 #pragma unroll
@@ -848,14 +854,8 @@ template <int D, typename CT, bool SPLIT, bool TWO>
 cudaError_t launch_t(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   using IO = typename std::conditional<SPLIT, float, CT>::type;
   auto kernel = paged_decode_kernel<D, CT, SPLIT, TWO>;
-  const void* k = reinterpret_cast<const void*>(kernel);
-  const int smem = smem_layout<D>(d.rows, d.p.batch, SPLIT).total;
-  cudaError_t e = raise_smem_limit(k, smem);
-  if (e != cudaSuccess) return e;
+  const int smem = smem_layout<D>(d.rows, d.cluster ? 0 : d.p.batch, SPLIT).total;
   if (d.cluster) {
-    if (d.cluster > 8 &&  // more than the cluster that every kernel may ask for
-        (e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
-      return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(d.p.batch) * P->base.Hk * d.subs * d.cluster);
     cfg.blockDim = dim3(kThreads);
@@ -877,10 +877,35 @@ cudaError_t launch_t(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   per_sm = per_sm < kCtasPerSm ? per_sm : kCtasPerSm;
   const int grid = per_sm * P->base.ctx->sm_count;
   d.small_grid = P->base.ctx->sm_count;
-  e = launch_pdl(kernel, grid, kThreads, smem, stream, d);
+  const cudaError_t e = launch_pdl(kernel, grid, kThreads, smem, stream, d);
   if (e != cudaSuccess) return e;
   return launch_pdl(paged_decode_join_kernel<D, IO>, static_cast<unsigned>(d.p.batch) * P->base.Hq, kJoinWarps * 32, 0,
                     stream, d, grid);
+}
+
+// What launches of an instance need to have been set for it: the shared memory
+// of the layer's largest calls, and clusters of up to 16 (*most: 8 where the
+// device does not run those).
+template <int D, typename CT, bool SPLIT, bool TWO>
+cudaError_t configure_t(int rows, int max_batch, int* most) {
+  const void* k = reinterpret_cast<const void*>(paged_decode_kernel<D, CT, SPLIT, TWO>);
+  const int smem = smem_layout<D>(rows, max_batch < kMaxBatch ? max_batch : kMaxBatch, SPLIT).total;
+  cudaError_t e = raise_smem_limit(k, smem);
+  if (e != cudaSuccess) return e;
+  return large_cluster(k, kThreads, smem_layout<D>(rows, 0, SPLIT).total, most);
+}
+template <int D>
+cudaError_t configure_d(const tla_paged* P, int rows, int* most) {
+  const bool two = rows > 8;
+  const int max_batch = P->base.max_batch;
+  if (P->io == kFp32)
+    return two ? configure_t<D, __half, true, true>(rows, max_batch, most)
+               : configure_t<D, __half, true, false>(rows, max_batch, most);
+  if (P->kept == kBf16)
+    return two ? configure_t<D, __nv_bfloat16, false, true>(rows, max_batch, most)
+               : configure_t<D, __nv_bfloat16, false, false>(rows, max_batch, most);
+  return two ? configure_t<D, __half, false, true>(rows, max_batch, most)
+             : configure_t<D, __half, false, false>(rows, max_batch, most);
 }
 
 template <int D>
@@ -906,9 +931,12 @@ int subgroup_rows(const tla_paged* P) {
 // one page), head_dim 64 or 128 and pools with rows on 16-byte boundaries;
 // float32 activations only over float16 pages (two bfloat16 parts would carry
 // 16 bits).
-void paged_decode_configure(tla_paged* P) {
+cudaError_t paged_decode_configure(tla_paged* P) {
   P->fast = P->wide && P->kept != kFp32 && (P->io != kFp32 || P->kept == kFp16) && P->pool.page_size >= 16 &&
             kCtasPerSm * P->base.ctx->sm_count <= kMaxGrid;
+  if (!P->fast) return cudaSuccess;
+  return P->base.D == 64 ? configure_d<64>(P, subgroup_rows(P), &P->decode_cluster)
+                         : configure_d<128>(P, subgroup_rows(P), &P->decode_cluster);
 }
 
 // The most tiles that a pair of this call can have.
@@ -939,15 +967,17 @@ int cluster_size(const tla_paged* P, const PagedArgs& p, int count) {
   const long long tiles = most_tiles(p, count), pairs = static_cast<long long>(p.batch) * p.a.Hk * subgroups(P);
   const int sms = P->base.ctx->sm_count;
   int n = 1;
-  while (n < kMaxCluster && tiles > 4 * n && pairs * n * 2 <= kCtasPerSm * sms) n *= 2;
+  while (n < P->decode_cluster && tiles > 4 * n && pairs * n * 2 <= kCtasPerSm * sms) n *= 2;
   return tiles <= (pairs * n > sms ? 40 : 20) * n ? n : 0;
 }
 
-// Whether a call's shares can be cut: the batch's table fits shared memory and
-// its tiles are counted in 32 bits.
+// Whether a call's pairs make a grid, or its shares can be cut: the batch's
+// table fits shared memory and its tiles are counted in 32 bits.
 bool paged_decode_takes(const tla_paged* P, const PagedArgs& p, int count) {
-  return P->fast && p.batch <= kMaxBatch &&
-         (most_tiles(p, count) + 16) * p.a.Hk * subgroups(P) * p.batch < (1LL << 31);
+  if (!P->fast) return false;
+  const long long pairs = static_cast<long long>(p.a.Hk) * subgroups(P) * p.batch;
+  if (cluster_size(P, p, count) > 0) return pairs < (1LL << 26);
+  return p.batch <= kMaxBatch && (most_tiles(p, count) + 16) * pairs < (1LL << 31);
 }
 
 size_t paged_decode_workspace(const tla_paged* P, const PagedArgs& p, int count) {
@@ -965,6 +995,7 @@ cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const vo
   d.gate = gate;
   d.out = out;
   d.scratch = static_cast<float*>(workspace);
+  d.scratch_floats = static_cast<long long>(paged_decode_workspace(P, p, count) / sizeof(float));
   d.count = count;
   d.subs = subgroups(P);
   d.rows = subgroup_rows(P);

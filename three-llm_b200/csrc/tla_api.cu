@@ -76,6 +76,30 @@ cudaError_t raise_smem_limit(const void* kernel, int bytes) {
   return e;
 }
 
+cudaError_t large_cluster(const void* kernel, int threads, int smem, int* most) {
+  *most = 8;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(16);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 16;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // (asked too much: not a fault of the caller's)
+    return cudaSuccess;
+  }
+  if (n > 0) *most = 16;
+  return cudaSuccess;
+}
+
 cudaError_t ensure_proj_workspace(tla_ctx* ctx, size_t floats, size_t tiles) {
   if (floats <= ctx->proj_ws_floats && tiles <= ctx->proj_cnt_count) return cudaSuccess;
   cudaError_t e = cudaSuccess;

@@ -13,12 +13,16 @@ namespace tla {
 
 struct DeviceGuard {
   int prev = -1;
+  bool moved = false;
   explicit DeviceGuard(int dev) {
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != dev) cudaSetDevice(dev);
+    if (prev != dev) {
+      cudaSetDevice(dev);
+      moved = true;
+    }
   }
   ~DeviceGuard() {
-    if (prev >= 0) cudaSetDevice(prev);
+    if (moved && prev >= 0) cudaSetDevice(prev);
   }
 };
 

@@ -66,6 +66,7 @@ struct tla_paged {
   int page_shift = 0;       // log2(page_size)
   bool wide = false;        // head_dim 64 or 128, rows of the pool on 16-byte boundaries
   float2* d_turns = nullptr;  // [kTurnSteps][rotary / 2]: cos and sin of 0, 1, .. steps of each pair
+  int decode_cluster = 1, select_cluster = 1;  // largest clusters of the kernels
   bool fast = false;        // tensor-core decode path (paged_decode_configure)
 };
 
@@ -118,6 +119,10 @@ cudaError_t raise_smem_limit(const void* kernel, int bytes);
 // Resident blocks per SM of a kernel instance at (threads, dynamic smem) on
 // the current device, cached per (device, kernel, threads, smem).
 cudaError_t cached_occupancy(const void* kernel, int threads, int smem, int* blocks);
+
+// Lets a kernel run in clusters of more than the portable 8 blocks and asks
+// whether the device holds one of 16 at (threads, dynamic smem): *most is 16 or 8.
+cudaError_t large_cluster(const void* kernel, int threads, int smem, int* most);
 
 // Generic path (any head_dim <= 256, any GQA ratio, fp16 or fp32 cache).
 // rope_append: per (b, t) token at pos = start[b] + t: QK-norm + RoPE of Q into
@@ -209,10 +214,13 @@ struct PagedArgs {
 };
 PagedArgs paged_args(const tla_paged* P, const int32_t* positions, const int32_t* table, int width, int batch);
 
+// Whether a row of the layer's heads fits the append kernels.
+bool paged_append_takes(const tla_paged* P);
 cudaError_t launch_paged_append(const tla_paged* P, const PagedArgs& p, const void* qkv, const int32_t* offsets,
                                 int rows, void* query_out, cudaStream_t stream);
 cudaError_t launch_paged_select(const tla_paged* P, const PagedArgs& p, const void* query, int first, int last,
                                 int32_t* pages_out, int count, void* workspace, cudaStream_t stream);
+cudaError_t paged_select_configure(tla_paged* P);
 size_t paged_select_workspace(const tla_paged* P, int batch, int width);
 // pages: null, or the listed pages [batch][Hk][count].
 cudaError_t launch_paged_decode_generic(const tla_paged* P, const PagedArgs& p, const void* query,
@@ -220,7 +228,7 @@ cudaError_t launch_paged_decode_generic(const tla_paged* P, const PagedArgs& p, 
                                         cudaStream_t stream);
 size_t paged_decode_generic_workspace(const tla_paged* P, int batch);
 // Tensor-core path: set up at creation, and whether it takes a call (count: listed pages, 0 for all).
-void paged_decode_configure(tla_paged* P);
+cudaError_t paged_decode_configure(tla_paged* P);
 bool paged_decode_takes(const tla_paged* P, const PagedArgs& p, int count);
 size_t paged_decode_workspace(const tla_paged* P, const PagedArgs& p, int count);
 cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const void* query, const int32_t* pages,

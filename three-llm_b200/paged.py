@@ -167,6 +167,8 @@ class PagedAttention:
             d, s = ctypes.c_size_t(), ctypes.c_size_t()
             check(self._lib.tla_paged_workspace(self.handle, batch, width, count, ctypes.byref(d), ctypes.byref(s)),
                   "workspace")
+            if len(self._workspace_bytes) >= 4096:
+                self._workspace_bytes.clear()
             sizes = self._workspace_bytes[batch, width, count] = (d.value, s.value)
         size = sizes[which]
         if size == 0:
