@@ -146,6 +146,66 @@ def test_decode_split_over_length_and_empty_rows(pkg, cuda, io, kept, lengths, d
     check_decode(pkg, cuda, lengths, 8, 2, d, 32, io, kept, seed=1)
 
 
+WIDE = 40000  # table entries past the sequences' own: their capacity has the pairs' tiles cut into shares
+
+
+@pytest.mark.parametrize("io,kept", PAIRS)
+@pytest.mark.parametrize("hq,hk,d", SHAPES)
+def test_decode_in_shares_shapes_and_types(pkg, cuda, hq, hk, d, io, kept):
+    check_decode(pkg, cuda, LENGTHS + [0, 900], hq, hk, d, 16, io, kept, extra_width=WIDE)
+
+
+@pytest.mark.parametrize("io,kept", [("fp16", "fp16"), ("bf16", "bf16"), ("fp32", "fp16")])
+@pytest.mark.parametrize("lengths", [[5000], [1], [0], [0, 0], [1, 2999, 700], [0, 5, 0, 900, 0], [64] * 40,
+                                     [1 + (i * 37) % 90 for i in range(301)]])
+@pytest.mark.parametrize("d", [64, 128])
+def test_decode_in_shares(pkg, cuda, io, kept, lengths, d):
+    """Pairs held by one CTA and by many, empty rows, more pairs than CTAs and fewer; then with gates."""
+    check_decode(pkg, cuda, lengths, 8, 2, d, 32, io, kept, seed=2, extra_width=WIDE // 2)
+    check_decode(pkg, cuda, lengths[:40], 8, 2, d, 128, io, kept, layout="NHD", gated=True, extra_width=WIDE // 8)
+
+
+def test_decode_listed_pages_in_shares(pkg, cuda):
+    """Lists long enough for shares, most of them ending early."""
+    lengths = [700, 16, 5000, 90]
+    listed = [[list(range(0, 44, 3)), [43]], [[0], []], [list(range(1, 313)), [5, 6, 7, 100]], [[0, 2], [1, 5]]]
+    count = 3000
+    w = World(lengths, 2, 64, 16, "fp16", extra_width=WIDE)
+    layer, *_ = make(pkg, cuda, w, 8, 2, 64, "fp16")
+    q = w.normal(4, 8, 64, dtype=torch.float16)
+    pages = ints([[x + [-1] * (count - len(x)) for x in seq] for seq in listed], cuda)
+    out = layer.decode(q.view(4, -1).to(cuda), ints([n - 1 for n in lengths], cuda), w.device_table(cuda), pages=pages)
+    assert layer.context.error() == 0
+    for i, n in enumerate(lengths):
+        exp, tol = ref.attend(q[i], w.keys, w.values, w.table[i], n - 1, 16, 0.125, listed=listed[i])
+        close(out[i], exp, tol)
+
+
+@pytest.mark.parametrize("wide", [0, WIDE])
+def test_decode_faults_leave_the_other_rows(pkg, cuda, wide):
+    """A page outside the pool in the middle of a long sequence, a position past the capacity, a row without
+    a sequence and a good one, in one call."""
+    w = World([3000, 3000, 0, 2000], 2, 128, 16, "fp16", extra_width=wide)
+    layer, *_ = make(pkg, cuda, w, 8, 2, 128, "fp16")
+    q = w.normal(4, 8, 128, dtype=torch.float16)
+    table = [list(r) for r in w.table]
+    table[0][77] = -5
+    positions = [2999, w.width * 16, -1, 1999]
+    out = layer.decode(q.view(4, -1).to(cuda), ints(positions, cuda), ints(table, cuda))
+    assert layer.context.error() in (-12, -18)
+    assert not out[1].any() and not out[2].any()
+    for i in (0, 3):
+        exp, tol = ref.attend(q[i], w.keys, w.values, table[i], positions[i], 16, 128 ** -0.5)
+        close(out[i], exp, tol)
+
+
+@pytest.mark.parametrize("hq,hk", [(1, 1), (3, 1), (16, 16), (64, 8), (8, 8), (33, 1), (128, 2)])
+@pytest.mark.parametrize("wide", [0, WIDE])
+def test_decode_head_groups(pkg, cuda, hq, hk, wide):
+    check_decode(pkg, cuda, [1, 100, 333], hq, hk, 64, 16, "fp16", "fp16", extra_width=wide)
+    check_decode(pkg, cuda, [77, 10], hq, hk, 128, 16, "fp32", "fp16", extra_width=wide)
+
+
 def test_decode_many_sequences(pkg, cuda):
     check_decode(pkg, cuda, [1 + (i * 37) % 90 for i in range(301)], 4, 2, 64, 16, "fp16", "fp16")
 
@@ -480,6 +540,24 @@ def test_select_many_pages(pkg, cuda):
     check_select(pkg, cuda, w, 4, 1, 64, "fp16", 100)
 
 
+@pytest.mark.parametrize("io,kept", PAIRS)
+@pytest.mark.parametrize("d", [64, 80, 128])
+def test_select_from_more_pages_than_shared_memory_ranks(pkg, cuda, io, kept, d):
+    """Tables so wide that the ranks go through the workspace."""
+    w = World([20000, 0, 16, 9000, 640], 1, d, 8 if d == 64 else 16, kept, extra_width=60000)
+    check_select(pkg, cuda, w, 4, 1, d, io, 100)
+    check_select(pkg, cuda, w, 4, 1, d, io, 7, 2, 3, window=5000)
+
+
+@pytest.mark.parametrize("n", [5, 65, 200, 257, 300, 1024, 1025, 1500, 4000])
+@pytest.mark.parametrize("batch", [1, 3, 40])
+def test_select_block_and_cluster_sizes(pkg, cuda, n, batch):
+    """Around the sizes where the blocks and the clusters change."""
+    batch = min(batch, 6000 // n)  # (the 64-bit form on the host is slow)
+    w = World([max(1, n * 8 - 3 * i) for i in range(batch)], 2, 64, 8, "fp16")
+    check_select(pkg, cuda, w, 8, 2, 64, "fp16", max(2, n // 5))
+
+
 def test_select_tiny_and_huge_keys(pkg, cuda):
     """Subnormal bounds and the type's largest values."""
     for kept, tiny in (("fp16", 2.0 ** -24), ("bf16", 2.0 ** -130)):
@@ -661,8 +739,8 @@ def step(layer, qkv, pos, table, count):
     return q, layer.decode(q, pos, table), pages, layer.decode(q, pos, table, pages=pages)
 
 
-def serving(pkg, cuda, seed, hq=8, hk=2, d=64, lengths=(300, 17, 650), context=None):
-    w = World(list(lengths), hk, d, 16, "fp16", seed=seed, room=1)
+def serving(pkg, cuda, seed, hq=8, hk=2, d=64, lengths=(300, 17, 650), context=None, extra_width=1):
+    w = World(list(lengths), hk, d, 16, "fp16", seed=seed, room=1, extra_width=extra_width)
     k, v, bd = w.device_pool(cuda)
     layer = pkg.PagedAttention(hq * d, hq, w.width * 16, k, v, {"headDim": d, "kvHeadCount": hk, "ropeTheta": 1e4},
                                key_bounds=bd, context=context)
@@ -673,7 +751,8 @@ def serving(pkg, cuda, seed, hq=8, hk=2, d=64, lengths=(300, 17, 650), context=N
 def test_two_graphs_and_an_eager_call_at_once(pkg, cuda):
     """Steps of two layers of one context captured into two graphs, replayed on two streams at the same time
     beside eager steps of a third: each equals its own eager step, bit for bit."""
-    worlds = [serving(pkg, cuda, s, lengths=n) for s, n in enumerate([(300, 17, 650), (2000,), (40, 999)])]
+    worlds = [serving(pkg, cuda, s, lengths=n, extra_width=x)
+              for s, (n, x) in enumerate([((300, 17, 650), 1), ((2000,), WIDE), ((40, 999), WIDE)])]
     exp = [[t.clone() for t in step(*w, 8)] for w in worlds]
     graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in worlds]
     for w in worlds[:2]:
@@ -738,8 +817,9 @@ def test_given_stream(pkg, cuda):
     assert torch.equal(q, exp[0]) and torch.equal(pages, exp[2]) and torch.equal(out, exp[3])
 
 
-def test_repeated_calls_agree_bit_for_bit(pkg, cuda):
-    layer, qkv, pos, table = serving(pkg, cuda, 6, 32, 8, 128, (4000, 3, 777, 0, 129))
+@pytest.mark.parametrize("wide", [1, WIDE])
+def test_repeated_calls_agree_bit_for_bit(pkg, cuda, wide):
+    layer, qkv, pos, table = serving(pkg, cuda, 6, 32, 8, 128, (4000, 3, 777, 0, 129), extra_width=wide)
     first = [t.clone() for t in step(layer, qkv, pos, table, 16)]
     for _ in range(10):
         for a, b in zip(step(layer, qkv, pos, table, 16), first):
