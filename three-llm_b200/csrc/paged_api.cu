@@ -128,7 +128,6 @@ int tla_paged_create(tla_ctx* ctx, const tla_attn_config* cfg, const tla_page_po
             (pool->page_count == 1 || pool->page_stride % vec == 0) && (L.Hk == 1 || pool->head_stride % vec == 0) &&
             (pool->page_size == 1 || pool->slot_stride % vec == 0);
   rc = from_cuda(tla::paged_decode_configure(P));
-  if (rc == TLA_OK && pool->bounds) rc = from_cuda(tla::paged_select_configure(P));
   if (rc == TLA_OK) rc = tla::layer_tables(&P->base, inv, q_norm_weight, k_norm_weight);
   const int half = L.rotary / 2;
   if (rc == TLA_OK && half > 0) {

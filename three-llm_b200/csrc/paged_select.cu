@@ -22,6 +22,7 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kMaxWarps = 16;
+constexpr int kMaxCluster = 8;
 constexpr int kMaxHeld = 48 * 1024;  // ranks that one block's shared memory holds
 constexpr int kScorePages = 32 * kMaxWarps;  // pages per block of the scoring kernel for longer sequences
 
@@ -447,19 +448,6 @@ int most_pages(int width, int shift, int capacity) {
 }
 
 template <typename IO, typename CT>
-cudaError_t configure_t(int* most) {
-  cudaError_t e = large_cluster(reinterpret_cast<const void*>(paged_select_kernel<IO, CT, 128>), 128, 40 * 1024, most);
-  int m = 8;
-  if (e == cudaSuccess)
-    e = large_cluster(reinterpret_cast<const void*>(paged_select_kernel<IO, CT, 256>), 256, 40 * 1024, &m);
-  if (m < *most) *most = m;
-  if (e == cudaSuccess)
-    e = large_cluster(reinterpret_cast<const void*>(paged_select_kernel<IO, CT, 512>), 512, 40 * 1024, &m);
-  if (m < *most) *most = m;
-  return e;
-}
-
-template <typename IO, typename CT>
 cudaError_t select_t(const tla_paged* P, const PagedArgs& p, const void* query, int first, int last,
                      int32_t* pages_out, int count, uint32_t* ranks, cudaStream_t stream) {
   const int most = most_pages(p.width, p.page_shift, p.capacity);
@@ -481,8 +469,10 @@ cudaError_t select_t(const tla_paged* P, const PagedArgs& p, const void* query, 
     if (most > 256) k = paged_select_kernel<IO, CT, 256>, warps = 8;
     if (most > 1024) k = paged_select_kernel<IO, CT, 512>, warps = 16;
     // Blocks per pair: up to eight per SM in all, at least two pages per warp.
+    // (Clusters of 16 leave a GPC's other SMs idle: 8 of them with 512 threads
+    // each ran in two waves, 28 us for a sparse step at 131072 tokens.)
     int shares = 1;
-    while (shares < P->select_cluster && pairs * shares * 2 <= 8 * P->base.ctx->sm_count && most > 2 * warps * shares)
+    while (shares < kMaxCluster && pairs * shares * 2 <= 8 * P->base.ctx->sm_count && most > 2 * warps * shares)
       shares *= 2;
     const size_t smem = vec + (most > count ? most * sizeof(uint32_t) : 0);
     if (smem > 48 * 1024) {
@@ -513,15 +503,6 @@ size_t paged_select_workspace(const tla_paged* P, int batch, int width) {
   const PagedArgs p = paged_args(P, nullptr, nullptr, width, batch);
   if (!P->pool.bounds || most_pages(width, P->page_shift, p.capacity) <= kMaxHeld) return 0;
   return static_cast<size_t>(batch) * P->base.Hk * width * sizeof(uint32_t);
-}
-
-cudaError_t paged_select_configure(tla_paged* P) {
-  int* most = &P->select_cluster;
-  if (P->io == kFp16) return configure_t<__half, __half>(most);
-  if (P->io == kBf16) return configure_t<__nv_bfloat16, __nv_bfloat16>(most);
-  if (P->kept == kFp16) return configure_t<float, __half>(most);
-  if (P->kept == kBf16) return configure_t<float, __nv_bfloat16>(most);
-  return configure_t<float, float>(most);
 }
 
 cudaError_t launch_paged_select(const tla_paged* P, const PagedArgs& p, const void* query, int first, int last,

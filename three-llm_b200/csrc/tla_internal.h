@@ -66,7 +66,7 @@ struct tla_paged {
   int page_shift = 0;       // log2(page_size)
   bool wide = false;        // head_dim 64 or 128, rows of the pool on 16-byte boundaries
   float2* d_turns = nullptr;  // [kTurnSteps][rotary / 2]: cos and sin of 0, 1, .. steps of each pair
-  int decode_cluster = 1, select_cluster = 1;  // largest clusters of the kernels
+  int decode_cluster = 1;   // largest cluster of the decode kernel
   bool fast = false;        // tensor-core decode path (paged_decode_configure)
 };
 
@@ -220,7 +220,6 @@ cudaError_t launch_paged_append(const tla_paged* P, const PagedArgs& p, const vo
                                 int rows, void* query_out, cudaStream_t stream);
 cudaError_t launch_paged_select(const tla_paged* P, const PagedArgs& p, const void* query, int first, int last,
                                 int32_t* pages_out, int count, void* workspace, cudaStream_t stream);
-cudaError_t paged_select_configure(tla_paged* P);
 size_t paged_select_workspace(const tla_paged* P, int batch, int width);
 // pages: null, or the listed pages [batch][Hk][count].
 cudaError_t launch_paged_decode_generic(const tla_paged* P, const PagedArgs& p, const void* query,
