@@ -154,7 +154,7 @@ class PagedAttention:
 
     @staticmethod
     def _new(like, shape, stream, dtype=None):
-        """A tensor on `like`'s device that belongs to the call's stream."""
+        """A dense tensor on `like`'s device that belongs to the call's stream."""
         if stream is None:
             return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
         with torch.cuda.stream(stream):
@@ -194,7 +194,8 @@ class PagedAttention:
         elif rows != batch:
             raise ValueError(f"{rows} rows for {batch} sequences need row_offsets")
         if query is None:
-            query = self._new(qkv, (rows, self.qSize), stream)
+            n = self.qSize  # (the strides given: a quicker call)
+            query = qkv.new_empty_strided((rows, n), (n, 1)) if stream is None else self._new(qkv, (rows, n), stream)
         else:
             self._rows(query, "query", rows, self.qSize)
         rc = self._lib.tla_paged_append(self.handle, qkv.data_ptr(), positions.data_ptr(), offsets,
@@ -239,7 +240,9 @@ class PagedAttention:
         self._rows(query, "query", batch, self.qSize)
         count = int(count)
         if pages is None:
-            pages = self._new(query, (batch, self.kvHeadCount, max(count, 0)), stream, torch.int32)
+            h, n = self.kvHeadCount, max(count, 0)
+            pages = (query.new_empty_strided((batch, h, n), (h * n, n, 1), dtype=torch.int32) if stream is None
+                     else self._new(query, (batch, h, n), stream, torch.int32))
         else:
             self._ints(pages, "pages", (batch, self.kvHeadCount, count))
         work, at, size = self._workspace(query, batch, width, 0, 1, stream)
