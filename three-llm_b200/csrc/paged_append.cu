@@ -168,29 +168,71 @@ __device__ __forceinline__ float4 floats(const Raw4<__nv_bfloat16>& r) {
                      __uint_as_float(u.y & 0xffff0000u));
 }
 template <typename T>
-__device__ __forceinline__ float4 load4(const T* p) {
-  return floats(raw4(p));
+__device__ __forceinline__ void put4(T* p, Raw4<T> v) {
+  *reinterpret_cast<Raw4<T>*>(p) = v;
 }
-__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
-__device__ __forceinline__ void store4(__half* p, float4 v) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w));
+// Four floats rounded to T.
+template <typename T>
+__device__ __forceinline__ Raw4<T> pack4(float4 v) {
+  if constexpr (sizeof(T) == 4) {
+    return {v};
+  } else if constexpr (std::is_same<T, __half>::value) {
+    return {make_uint2(pack_half2(v.x, v.y), pack_half2(v.z, v.w))};
+  } else {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    return {make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b))};
+  }
 }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
-  const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
-  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 v) {
+  put4(p, pack4<T>(v));
 }
-// A rounding to the pages' type, as a float.
-template <typename CT>
-__device__ __forceinline__ float4 as_stored(float4 v) {
-  return make_float4(to_f32(from_f32<CT>(v.x)), to_f32(from_f32<CT>(v.y)), to_f32(from_f32<CT>(v.z)),
-                     to_f32(from_f32<CT>(v.w)));
+// What was loaded, stored without a detour where the types are the same.
+template <typename T>
+__device__ __forceinline__ void put_same(T* p, Raw4<T> v) {
+  put4(p, v);
 }
-// (the comparison's order keeps what is there when either is NaN, as low_of and high_of do)
-__device__ __forceinline__ float4 low4(float4 a, float4 b) {
-  return make_float4(b.x < a.x ? b.x : a.x, b.y < a.y ? b.y : a.y, b.z < a.z ? b.z : a.z, b.w < a.w ? b.w : a.w);
+template <typename T, typename U>
+__device__ __forceinline__ void put_same(T* p, Raw4<U> v) {
+  store4(p, floats(v));
 }
-__device__ __forceinline__ float4 high4(float4 a, float4 b) {
-  return make_float4(b.x > a.x ? b.x : a.x, b.y > a.y ? b.y : a.y, b.z > a.z ? b.z : a.z, b.w > a.w ? b.w : a.w);
+
+// The smaller and the larger of two, element by element (a NaN gives way to a number).
+template <typename P>
+__device__ __forceinline__ uint32_t low_pair(uint32_t a, uint32_t b) {
+  const P v = __hmin2(*reinterpret_cast<P*>(&a), *reinterpret_cast<P*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename P>
+__device__ __forceinline__ uint32_t high_pair(uint32_t a, uint32_t b) {
+  const P v = __hmax2(*reinterpret_cast<P*>(&a), *reinterpret_cast<P*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ Raw4<T> low4(Raw4<T> a, Raw4<T> b) {
+  if constexpr (sizeof(T) == 4) {
+    return {make_float4(fminf(a.u.x, b.u.x), fminf(a.u.y, b.u.y), fminf(a.u.z, b.u.z), fminf(a.u.w, b.u.w))};
+  } else {
+    using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    return {make_uint2(low_pair<P>(a.u.x, b.u.x), low_pair<P>(a.u.y, b.u.y))};
+  }
+}
+template <typename T>
+__device__ __forceinline__ Raw4<T> high4(Raw4<T> a, Raw4<T> b) {
+  if constexpr (sizeof(T) == 4) {
+    return {make_float4(fmaxf(a.u.x, b.u.x), fmaxf(a.u.y, b.u.y), fmaxf(a.u.z, b.u.z), fmaxf(a.u.w, b.u.w))};
+  } else {
+    using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    return {make_uint2(high_pair<P>(a.u.x, b.u.x), high_pair<P>(a.u.y, b.u.y))};
+  }
+}
+template <typename T>
+__device__ __forceinline__ Raw4<T> lane_xor(Raw4<T> v, int o) {
+  if constexpr (sizeof(T) == 4)
+    return {make_float4(__shfl_xor_sync(0xffffffffu, v.u.x, o), __shfl_xor_sync(0xffffffffu, v.u.y, o),
+                        __shfl_xor_sync(0xffffffffu, v.u.z, o), __shfl_xor_sync(0xffffffffu, v.u.w, o))};
+  else
+    return {make_uint2(__shfl_xor_sync(0xffffffffu, v.u.x, o), __shfl_xor_sync(0xffffffffu, v.u.y, o))};
 }
 
 // head_dim 64 or 128, rotary dimensions a multiple of 8: D / 8 lanes hold a
@@ -323,16 +365,21 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
         } else {
           const int kvh = h - Hq - (kKind == 1 ? 0 : Hk);
           CT* at = kv + kvh * p.head_stride;
-          store4(at + d0, x);
-          store4(at + d1, y);
+          if (kKind == 2 && !norm) {  // values stay as they are
+            put_same(at + d0, lo[c]);
+            put_same(at + d1, hi[c]);
+          } else {
+            store4(at + d0, x);
+            store4(at + d1, y);
+          }
           if (kKind == 1 && p.bounds && !offsets) {  // one new token: its page's bounds right here
             CT* low = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D;
             CT* high = low + D;
-            const float4 k0 = as_stored<CT>(x), k1 = as_stored<CT>(y);
-            store4(low + d0, slot == 0 ? k0 : low4(load4(low + d0), k0));
-            store4(low + d1, slot == 0 ? k1 : low4(load4(low + d1), k1));
-            store4(high + d0, slot == 0 ? k0 : high4(load4(high + d0), k0));
-            store4(high + d1, slot == 0 ? k1 : high4(load4(high + d1), k1));
+            const Raw4<CT> k0 = pack4<CT>(x), k1 = pack4<CT>(y);
+            put4(low + d0, slot == 0 ? k0 : low4<CT>(raw4(low + d0), k0));
+            put4(low + d1, slot == 0 ? k1 : low4<CT>(raw4(low + d1), k1));
+            put4(high + d0, slot == 0 ? k0 : high4<CT>(raw4(high + d0), k0));
+            put4(high + d1, slot == 0 ? k1 : high4<CT>(raw4(high + d1), k1));
           }
         }
       }
@@ -436,8 +483,8 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
   const int shares = kWarps / heads, share = warp / heads;  // warps per head, and this one's place
   const int kvh = unit % groups * heads + warp % heads;
   const int row_size = (a.Hq + 2 * Hk) * D;
-  float4 low0 = make_float4(INFINITY, INFINITY, INFINITY, INFINITY), low1 = low0;
-  float4 high0 = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), high1 = high0;
+  Raw4<CT> low0 = pack4<CT>(make_float4(INFINITY, INFINITY, INFINITY, INFINITY)), low1 = low0;
+  Raw4<CT> high0 = pack4<CT>(make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY)), high1 = high0;
   for (int s0 = begin; s0 < end; s0 += kPageSlots) {
     const int slots = min(kPageSlots, end - s0);
     __syncthreads();
@@ -471,7 +518,7 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
 #pragma unroll
       for (int k = 0; k < kLoads; ++k) {
         const int s = s1 + k * shares * kPer;
-        float4 xf = floats(lo[k]), yf = floats(hi[k]);
+        const float4 xf = floats(lo[k]), yf = floats(hi[k]);
         float x[4] = {xf.x, xf.y, xf.z, xf.w}, y[4] = {yf.x, yf.y, yf.z, yf.w};
         if (a.k_norm) {  // math.ts:78-97
           float ss = 0.f;
@@ -497,34 +544,30 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
             x[e] = u;
           }
         }
-        xf = as_stored<CT>(make_float4(x[0], x[1], x[2], x[3]));
-        yf = as_stored<CT>(make_float4(y[0], y[1], y[2], y[3]));
-        store4(out + s * p.slot_stride + d0, xf);
-        store4(out + s * p.slot_stride + d1, yf);
-        low0 = low4(low0, xf);
-        low1 = low4(low1, yf);
-        high0 = high4(high0, xf);
-        high1 = high4(high1, yf);
+        const Raw4<CT> k0 = pack4<CT>(make_float4(x[0], x[1], x[2], x[3]));
+        const Raw4<CT> k1 = pack4<CT>(make_float4(y[0], y[1], y[2], y[3]));
+        put4(out + s * p.slot_stride + d0, k0);
+        put4(out + s * p.slot_stride + d1, k1);
+        low0 = low4<CT>(low0, k0);
+        low1 = low4<CT>(low1, k1);
+        high0 = high4<CT>(high0, k0);
+        high1 = high4<CT>(high1, k1);
       }
     }
   }
   // across the lanes' slots, then the warps of a head
 #pragma unroll
   for (int o = kLanes; o < 32; o <<= 1) {
-    auto from_lane = [&](float4 v) {
-      return make_float4(__shfl_xor_sync(full, v.x, o), __shfl_xor_sync(full, v.y, o), __shfl_xor_sync(full, v.z, o),
-                         __shfl_xor_sync(full, v.w, o));
-    };
-    low0 = low4(low0, from_lane(low0));
-    low1 = low4(low1, from_lane(low1));
-    high0 = high4(high0, from_lane(high0));
-    high1 = high4(high1, from_lane(high1));
+    low0 = low4<CT>(low0, lane_xor<CT>(low0, o));
+    low1 = low4<CT>(low1, lane_xor<CT>(low1, o));
+    high0 = high4<CT>(high0, lane_xor<CT>(high0, o));
+    high1 = high4<CT>(high1, lane_xor<CT>(high1, o));
   }
   if (group == 0) {
-    *reinterpret_cast<float4*>(&join_s[warp][0][d0]) = low0;
-    *reinterpret_cast<float4*>(&join_s[warp][0][d1]) = low1;
-    *reinterpret_cast<float4*>(&join_s[warp][1][d0]) = high0;
-    *reinterpret_cast<float4*>(&join_s[warp][1][d1]) = high1;
+    *reinterpret_cast<float4*>(&join_s[warp][0][d0]) = floats(low0);
+    *reinterpret_cast<float4*>(&join_s[warp][0][d1]) = floats(low1);
+    *reinterpret_cast<float4*>(&join_s[warp][1][d0]) = floats(high0);
+    *reinterpret_cast<float4*>(&join_s[warp][1][d1]) = floats(high1);
   }
   __syncthreads();
   for (int i = tid; i < heads * 2 * D; i += kPageThreads) {  // [head][low, high][d]
