@@ -131,6 +131,15 @@ def test_decode_other_head_dims(pkg, cuda, d, io, kept):
     check_decode(pkg, cuda, [1, 33, 130], 6, 2, d, 16, io, kept)
 
 
+@pytest.mark.parametrize("d", [8, 24, 72, 80, 96, 136, 200, 256])
+@pytest.mark.parametrize("io,kept", [("fp16", "fp16"), ("bf16", "bf16"), ("fp32", "fp16")])
+@pytest.mark.parametrize("wide", [1, 9000])
+def test_decode_widths_between(pkg, cuda, d, io, kept, wide):
+    """head_dims that the kernels built for 64, 128 and 256 take with zero columns, in clusters and in shares."""
+    check_decode(pkg, cuda, [1, 17, 64, 300, 0, 1000], 6, 2, d, 32, io, kept, gated=True, extra_width=wide)
+    check_decode(pkg, cuda, [77, 500], 20, 2, d, 16, io, kept, layout="NHD", window=90, extra_width=wide)
+
+
 @pytest.mark.parametrize("window", [1, 5, 16, 64, 100, 10000])
 @pytest.mark.parametrize("page", [16, 64])
 @pytest.mark.parametrize("io,kept", [("fp16", "fp16"), ("bf16", "bf16"), ("fp32", "fp16")])

@@ -124,7 +124,7 @@ int tla_paged_create(tla_ctx* ctx, const tla_attn_config* cfg, const tla_page_po
   while ((1 << P->page_shift) < pool->page_size) ++P->page_shift;
   // a dimension of one entry may carry any stride
   const int vec = static_cast<int>(16 / elem);
-  P->wide = (L.D == 64 || L.D == 128) && aligned16(pool->key) && aligned16(pool->value) &&
+  P->wide = L.D % 8 == 0 && aligned16(pool->key) && aligned16(pool->value) &&
             (pool->page_count == 1 || pool->page_stride % vec == 0) && (L.Hk == 1 || pool->head_stride % vec == 0) &&
             (pool->page_size == 1 || pool->slot_stride % vec == 0);
   rc = from_cuda(tla::paged_decode_configure(P));

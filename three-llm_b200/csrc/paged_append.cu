@@ -652,7 +652,9 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // The layers that append_rows takes.
-bool by_rows(const tla_paged* P) { return P->wide && P->base.rotary % 8 == 0; }
+bool by_rows(const tla_paged* P) {
+  return P->wide && (P->base.D == 64 || P->base.D == 128) && P->base.rotary % 8 == 0;
+}
 // Shared memory of the block-per-row kernel: the row in float32, its cosines and sines.
 size_t row_smem(const tla_paged* P) {
   return sizeof(float) * (static_cast<size_t>(P->base.Hq + 2 * P->base.Hk) * P->base.D + P->base.rotary);

@@ -1,12 +1,13 @@
-// Persistent split-KV decode over a paged cache (sm_100a): 16-bit pages,
-// head_dim 64 or 128, pages of 16 tokens and up.
+// Split-KV decode over a paged cache (sm_100a): 16-bit pages of 16 tokens and
+// up, head_dim a multiple of 8 up to 256 (the kernel is built for 64, 128 and
+// 256, whose columns past head_dim stay zero in shared memory).
 //
 //   o = sum_t 2^(x_t - m) v_t / sum_t 2^(x_t - m),  x_t = log2(e) scale q.k_t
 //
 // Each K and V element is read once and used by the group's query heads, about
 // 2 G operations per byte: memory bounds it, so the kernel's shape follows the
-// reads. A (sequence, kv head) pair's tokens are cut into tiles (8 KB of K and
-// V: 32 tokens at head_dim 64, 16 at 128), and the tiles of all pairs into
+// reads. A (sequence, kv head) pair's tokens are cut into tiles (32 tokens at
+// head_dim 64, 16 above: 8 KB of K and V at 64 and 128), and the tiles of all pairs into
 // equal contiguous shares, one per resident CTA, whatever the sequences'
 // lengths; a share may begin and end inside a pair. Four warps take a share's
 // tiles in turn, each by itself: a warp keeps a ring of tiles of its own, which
@@ -64,14 +65,21 @@ struct Cfg {
   static constexpr int kTile = D == 64 ? 32 : 16;
   static constexpr int kGroups = kTile / 16;
   static constexpr int kStages = 2;
-  static constexpr int kHalves = D / 64;  // 128-byte rows per cache row
-  static constexpr int kTileBytes = kTile * kHalves * 128;
+  static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kQPitch = D * 2 + 16;
   // A pair costs its query set-up and its epilogue besides its tiles: counted
   // as this many tiles when the shares are cut.
   static constexpr int kSetup = 14;
 };
+
+// Byte offset of 16-byte piece `chunk` of token `tok` in a tile: the piece's
+// place among its row's eighths turns with the token, so that the eight rows of
+// a matrix operand lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t tile_at(int tok, int chunk) {
+  return static_cast<uint32_t>(tok * D * 2 + ((chunk ^ (tok & 7)) << 4));
+}
 
 struct DecodeParams {
   PagedArgs p;
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const PagedArgs& p = d.p;
-  const int Hq = p.a.Hq, G = p.a.G, pairs = p.a.Hk * d.subs, rows = d.rows;
+  const int Hq = p.a.Hq, G = p.a.G, pairs = p.a.Hk * d.subs, rows = d.rows, hd = p.a.D;
   const SmemLayout L = smem_layout<D>(rows, d.cluster ? 0 : p.batch, SPLIT);
   int* prefix = reinterpret_cast<int*>(smem + L.prefix);
   int* spos = prefix + p.batch + 1;
@@ -266,6 +274,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   const uint32_t ring = smem_u32(smem + L.stages) + warp * C::kStages * C::kStageBytes;
   int* meta = reinterpret_cast<int*>(smem + L.meta) + warp * C::kStages * C::kGroups;  // first position of each 16 tokens
   if (tid == 0) prefix[0] = 0;
+  if (hd < D)  // columns that no copy goes to
+    for (int i = lane; i < C::kStages * C::kStageBytes / 16; i += 32)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + i * 16), "r"(0) : "memory");
+  __syncwarp();
   griddep_wait();
   griddep_launch_dependents();
   int tb = 0, te = 1;  // the share's units; one segment with a cluster per pair
@@ -285,8 +297,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     if (only.tiles == 0) {  // (the same for the whole cluster) no sequence: zeros
       const int kvh = only.pair / d.subs, sub = only.pair - kvh * d.subs;
       const int h0 = kvh * G + sub * rows, heads = min(rows, (kvh + 1) * G - h0);
-      for (int i = tid; rank == 0 && i < heads * D; i += kThreads)
-        static_cast<IO*>(d.out)[(static_cast<int64_t>(only_b) * Hq + h0) * D + i] = from_f32<IO>(0.f);
+      for (int i = tid; rank == 0 && i < heads * hd; i += kThreads)
+        static_cast<IO*>(d.out)[(static_cast<int64_t>(only_b) * Hq + h0) * hd + i] = from_f32<IO>(0.f);
       return;
     }
   } else {
@@ -303,8 +315,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     // rows without a sequence, spread over the whole launch
     for (int b = cta; b < p.batch; b += gridDim.x)
       if (prefix[b + 1] == prefix[b])
-        for (int i = tid; i < Hq * D; i += kThreads)
-          static_cast<IO*>(d.out)[static_cast<int64_t>(b) * Hq * D + i] = from_f32<IO>(0.f);
+        for (int i = tid; i < Hq * hd; i += kThreads)
+          static_cast<IO*>(d.out)[static_cast<int64_t>(b) * Hq * hd + i] = from_f32<IO>(0.f);
     const int grid = effective_grid(total, gridDim.x, d.small_grid);
     if (total == 0 || cta >= grid) return;
     tb = cta_begin(cta, total, grid);
@@ -349,11 +361,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   };
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;  // lanes per row, rows per copy
   const int r0 = lane / kLanes, chunk = lane % kLanes;
-  // where a lane's 16 bytes go: two places in turn, 1024 bytes on every second copy
-  const uint32_t place0 = sw128(r0 * C::kHalves + (chunk >> 3), chunk & 7);
-  const uint32_t place1 = sw128((r0 + kRows) * C::kHalves + (chunk >> 3), chunk & 7);
+  // Where a lane's 16 bytes go: 512 bytes on with every copy, the place in the
+  // row turned by the rows passed (r0 and the steps share no bits).
+  const uint32_t place = static_cast<uint32_t>(r0 * D * 2), turned = static_cast<uint32_t>((chunk ^ r0) << 4);
+  auto place_of = [&](int i) { return place + i * 512 + (turned ^ (((i * kRows) & 7) << 4)); };
+  const bool lane_on = chunk * 8 < hd;
   const int64_t lane_from = r0 * p.slot_stride + chunk * 8;
-  const bool dense = p.slot_stride == D;  // a page's rows of a head are one block
+  const bool dense = p.slot_stride == D && hd == D;  // a page's rows of a head are one block
   const int64_t apart = static_cast<const CT*>(p.value) - static_cast<const CT*>(p.key);
   auto load_next = [&](int stage) {
     while (ld.it >= ld.end && ld.g < te) {  // on to the segment that holds the tile
@@ -401,32 +415,29 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         const int at = page < 0 ? kNowhere : (index << shift) + slot;
         if (lane == 0) meta[stage * C::kGroups + u] = at;
         const CT* k = static_cast<const CT*>(p.key) + (page * p.page_stride + slot * p.slot_stride + ld.head);
-        const uint32_t dst = kst + u * 16 * C::kHalves * 128;
+        const uint32_t dst = kst + u * 16 * D * 2;
         if (at >= ld.lo && at + 15 <= ld.hi) {  // (the same for the whole warp)
           if (dense) {
 #pragma unroll
             for (int i = 0; i < 16 / kRows; ++i) {
-              const uint32_t to = dst + (i / 2) * 1024 + (i % 2 ? place1 : place0);
-              copy16(to, k + i * kRows * D);
-              copy16(to + C::kTileBytes, k + apart + i * kRows * D);
+              copy16(dst + place_of(i), k + i * kRows * D);
+              copy16(dst + place_of(i) + C::kTileBytes, k + apart + i * kRows * D);
             }
-          } else {
+          } else if (lane_on) {
 #pragma unroll
             for (int i = 0; i < 16 / kRows; ++i) {
-              const uint32_t to = dst + (i / 2) * 1024 + (i % 2 ? place1 : place0);
-              copy16(to, k);
-              copy16(to + C::kTileBytes, k + apart);
+              copy16(dst + place_of(i), k);
+              copy16(dst + place_of(i) + C::kTileBytes, k + apart);
               k += kRows * p.slot_stride;
             }
           }
-        } else {  // rows outside the range, and pages that are not there, as zeros
+        } else if (lane_on) {  // rows outside the range, and pages that are not there, as zeros
 #pragma unroll 1
           for (int i = 0; i < 16 / kRows; ++i) {
             const int tok = at + r0 + i * kRows, bytes = tok >= ld.lo && tok <= ld.hi ? 16 : 0;
             const CT* from = bytes ? k + i * kRows * p.slot_stride : static_cast<const CT*>(p.key);
-            const uint32_t to = dst + (i / 2) * 1024 + (i % 2 ? place1 : place0);
-            copy16_or_zeros(to, from, bytes);
-            copy16_or_zeros(to + C::kTileBytes, bytes ? from + apart : from, bytes);
+            copy16_or_zeros(dst + place_of(i), from, bytes);
+            copy16_or_zeros(dst + place_of(i) + C::kTileBytes, bytes ? from + apart : from, bytes);
           }
         }
       }
@@ -456,14 +467,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     const int kvh = sg.pair / d.subs, sub = sg.pair - kvh * d.subs;
     const int h0 = kvh * G + sub * rows, heads = min(rows, (kvh + 1) * G - h0);
     const Walk w = walk(b);
-    const IO* q = static_cast<const IO*>(d.query) + (static_cast<int64_t>(b) * Hq + h0) * D;
+    const IO* q = static_cast<const IO*>(d.query) + (static_cast<int64_t>(b) * Hq + h0) * hd;
     // ---- the group's queries, 8 elements per thread and trip; rows past the group are zeros
     if constexpr (SPLIT) {
       for (int r = warp; r < 8 * kNt; r += kWarps) {
         float x[D / 32], top = 0.f;
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) {
-          x[e] = r < heads ? q[r * D + lane + 32 * e] : 0.f;
+          x[e] = r < heads && lane + 32 * e < hd ? q[r * hd + lane + 32 * e] : 0.f;
           top = fmaxf(top, fabsf(x[e]));
         }
 #pragma unroll
@@ -485,7 +496,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     } else {
       for (int i = tid; i < 8 * kNt * D / 8; i += 128) {
         const int r = i / (D / 8), c = i - r * (D / 8);
-        const uint4 v = r < heads ? reinterpret_cast<const uint4*>(q)[i] : make_uint4(0, 0, 0, 0);
+        const uint4 v = r < heads && c * 8 < hd ? *reinterpret_cast<const uint4*>(q + r * hd + c * 8)
+                                                : make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(q_s + r * (C::kQPitch / 2) + c * 8) = v;
       }
     }
@@ -549,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
           for (int u = 0; u < kGroups; ++u) {
             const int tok = u * 16 + frag_row;
             uint32_t a[4];
-            ldsm_x4(kbase + sw128(tok * C::kHalves + (chunk >> 3), chunk & 7), a[0], a[1], a[2], a[3]);
+            ldsm_x4(kbase + tile_at<D>(tok, chunk), a[0], a[1], a[2], a[3]);
 #pragma unroll
             for (int nt = 0; nt < kNt; ++nt) {
               mma_t<CT>(x[u][nt], a, qb[nt][kk][0], qb[nt][kk][1]);
@@ -625,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
           for (int i = 0; i < D / 16; ++i) {
             const int chunk = 2 * i + ((lane >> 3) & 1);
             uint32_t a[4];
-            ldsm_x4_t(vbase + sw128(tok * C::kHalves + (chunk >> 3), chunk & 7), a[0], a[1], a[2], a[3]);
+            ldsm_x4_t(vbase + tile_at<D>(tok, chunk), a[0], a[1], a[2], a[3]);
 #pragma unroll
             for (int nt = 0; nt < kNt; ++nt) {
               mma_t<CT>(o[nt][i], a, pb[u][nt][0], pb[u][nt][1]);
@@ -685,8 +697,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       }
       if (whole) {
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * D + c, v0 * inv);
-        store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * D + c + 1, v1 * inv);
+        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c, v0 * inv);
+        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c + 1, v1 * inv);
       } else if (d.cluster ||
                  TLA_IN_BOUNDS(mine - d.scratch + (r + 1) * (D + 2) - 1, d.scratch_floats, p.a.error)) {
         *reinterpret_cast<float2*>(mine + r * (D + 2) + 2 + c) = make_float2(v0, v1);
@@ -705,6 +717,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     float* part = reinterpret_cast<float*>(smem + L.part);
     for (int i = cluster.block_rank() * kThreads + tid; i < heads * (D / 2); i += d.cluster * kThreads) {
       const int r = i / (D / 2), c = i % (D / 2) * 2;
+      if (c >= hd) continue;
       float2 ml[kMaxCluster], x[kMaxCluster];
       float top = -INFINITY;
 #pragma unroll
@@ -729,8 +742,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         v1 += x[k].y * f;
       }
       const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * D + c, v0 * inv);
-      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * D + c + 1, v1 * inv);
+      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c, v0 * inv);
+      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c + 1, v1 * inv);
     }
     cluster.sync();  // the others may still read this CTA's triple
   }
@@ -824,7 +837,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
   if (alone) {
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
-      store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * D + lane + 32 * e, sum > 0.f ? acc[e] / sum : 0.f);
+      if (lane + 32 * e < p.a.D)
+        store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + lane + 32 * e, sum > 0.f ? acc[e] / sum : 0.f);
     return;
   }
   if (lane == 0) {
@@ -837,17 +851,25 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
   float high = red[0][0];
 #pragma unroll
   for (int w = 1; w < kJoinWarps; ++w) high = fmaxf(high, red[0][w]);
-  if (tid >= D) return;
-  float all = 0.f, v = 0.f;
-  if (high != -INFINITY) {
+  for (int c = tid; c < p.a.D; c += kJoinWarps * 32) {
+    float all = 0.f, v = 0.f;
+    if (high != -INFINITY) {
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      const float f = ex2(red[0][w] - high);
-      all += red[1][w] * f;
-      v += row_s[w][tid] * f;
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = ex2(red[0][w] - high);
+        all += red[1][w] * f;
+        v += row_s[w][c] * f;
+      }
     }
+    store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + c, all > 0.f ? v / all : 0.f);
   }
-  store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * D + tid, all > 0.f ? v / all : 0.f);
+}
+
+// Two CTAs per SM by registers (the launch bounds), if shared memory holds two
+// (228 KB, 1 KB of it reserved per CTA).
+int ctas_per_sm(int smem) {
+  const int n = 228 * 1024 / (smem + 1024);
+  return n < kCtasPerSm ? n : kCtasPerSm;
 }
 
 template <int D, typename CT, bool SPLIT, bool TWO>
@@ -871,16 +893,20 @@ cudaError_t launch_t(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
     cfg.numAttrs = d.cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, d);
   }
-  // two CTAs per SM by registers (the launch bounds), if shared memory holds
-  // two (228 KB, 1 KB of it reserved per CTA)
-  int per_sm = 228 * 1024 / (smem + 1024);
-  per_sm = per_sm < kCtasPerSm ? per_sm : kCtasPerSm;
-  const int grid = per_sm * P->base.ctx->sm_count;
+  const int grid = ctas_per_sm(smem) * P->base.ctx->sm_count;
   d.small_grid = P->base.ctx->sm_count;
   const cudaError_t e = launch_pdl(kernel, grid, kThreads, smem, stream, d);
   if (e != cudaSuccess) return e;
   return launch_pdl(paged_decode_join_kernel<D, IO>, static_cast<unsigned>(d.p.batch) * P->base.Hq, kJoinWarps * 32, 0,
                     stream, d, grid);
+}
+
+template <typename F>
+auto by_width(const tla_paged* P, F f) {
+  const int D = P->base.D;
+  if (D <= 64) return f(std::integral_constant<int, 64>());
+  if (D <= 128) return f(std::integral_constant<int, 128>());
+  return f(std::integral_constant<int, 256>());
 }
 
 // What launches of an instance need to have been set for it: the shared memory
@@ -898,6 +924,11 @@ template <int D>
 cudaError_t configure_d(const tla_paged* P, int rows, int* most) {
   const bool two = rows > 8;
   const int max_batch = P->base.max_batch;
+  if constexpr (D == 256) {  // (groups of at most 8 heads: two column tiles of O would not fit the registers)
+    if (P->io == kFp32) return configure_t<D, __half, true, false>(rows, max_batch, most);
+    if (P->kept == kBf16) return configure_t<D, __nv_bfloat16, false, false>(rows, max_batch, most);
+    return configure_t<D, __half, false, false>(rows, max_batch, most);
+  }
   if (P->io == kFp32)
     return two ? configure_t<D, __half, true, true>(rows, max_batch, most)
                : configure_t<D, __half, true, false>(rows, max_batch, most);
@@ -911,6 +942,11 @@ cudaError_t configure_d(const tla_paged* P, int rows, int* most) {
 template <int D>
 cudaError_t launch_d(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   const bool two = d.rows > 8;
+  if constexpr (D == 256) {
+    if (P->io == kFp32) return launch_t<D, __half, true, false>(P, d, stream);
+    if (P->kept == kBf16) return launch_t<D, __nv_bfloat16, false, false>(P, d, stream);
+    return launch_t<D, __half, false, false>(P, d, stream);
+  }
   if (P->io == kFp32)
     return two ? launch_t<D, __half, true, true>(P, d, stream) : launch_t<D, __half, true, false>(P, d, stream);
   if (P->kept == kBf16)
@@ -919,7 +955,10 @@ cudaError_t launch_d(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
   return two ? launch_t<D, __half, false, true>(P, d, stream) : launch_t<D, __half, false, false>(P, d, stream);
 }
 
-int subgroups(const tla_paged* P) { return (P->base.G + 15) / 16; }
+int subgroups(const tla_paged* P) {
+  const int most = P->base.D > 128 ? 8 : 16;
+  return (P->base.G + most - 1) / most;
+}
 int subgroup_rows(const tla_paged* P) {
   const int s = subgroups(P);
   return (P->base.G + s - 1) / s;
@@ -928,20 +967,19 @@ int subgroup_rows(const tla_paged* P) {
 }  // namespace
 
 // The tensor-core path takes 16-bit pages of 16 tokens and up (16 tokens lie in
-// one page), head_dim 64 or 128 and pools with rows on 16-byte boundaries;
+// one page), head_dim a multiple of 8 and pools with rows on 16-byte boundaries;
 // float32 activations only over float16 pages (two bfloat16 parts would carry
 // 16 bits).
 cudaError_t paged_decode_configure(tla_paged* P) {
   P->fast = P->wide && P->kept != kFp32 && (P->io != kFp32 || P->kept == kFp16) && P->pool.page_size >= 16 &&
             kCtasPerSm * P->base.ctx->sm_count <= kMaxGrid;
   if (!P->fast) return cudaSuccess;
-  return P->base.D == 64 ? configure_d<64>(P, subgroup_rows(P), &P->decode_cluster)
-                         : configure_d<128>(P, subgroup_rows(P), &P->decode_cluster);
+  return by_width(P, [&](auto w) { return configure_d<decltype(w)::value>(P, subgroup_rows(P), &P->decode_cluster); });
 }
 
 // The most tiles that a pair of this call can have.
 long long most_tiles(const PagedArgs& p, int count) {
-  const int kTile = p.a.D == 64 ? Cfg<64>::kTile : Cfg<128>::kTile;
+  const int kTile = p.a.D <= 64 ? Cfg<64>::kTile : Cfg<128>::kTile;
   long long tokens = p.capacity, tiles = (tokens + kTile - 1) / kTile;
   if (count > 0) {
     const long long listed = ((static_cast<long long>(count) << p.page_shift) + kTile - 1) / kTile;
@@ -966,8 +1004,9 @@ long long most_tiles(const PagedArgs& p, int count) {
 int cluster_size(const tla_paged* P, const PagedArgs& p, int count) {
   const long long tiles = most_tiles(p, count), pairs = static_cast<long long>(p.batch) * p.a.Hk * subgroups(P);
   const int sms = P->base.ctx->sm_count;
+  const int per_sm = p.a.D > 128 ? 1 : kCtasPerSm;
   int n = 1;
-  while (n < P->decode_cluster && tiles > 4 * n && pairs * n * 2 <= kCtasPerSm * sms) n *= 2;
+  while (n < P->decode_cluster && tiles > 4 * n && pairs * n * 2 <= per_sm * sms) n *= 2;
   return tiles <= (pairs * n > sms ? 40 : 20) * n ? n : 0;
 }
 
@@ -982,8 +1021,8 @@ bool paged_decode_takes(const tla_paged* P, const PagedArgs& p, int count) {
 
 size_t paged_decode_workspace(const tla_paged* P, const PagedArgs& p, int count) {
   if (cluster_size(P, p, count) > 0) return 0;
-  return static_cast<size_t>(kCtasPerSm) * P->base.ctx->sm_count * 2 * subgroup_rows(P) * (P->base.D + 2) *
-         sizeof(float);
+  const int width = by_width(P, [](auto w) { return decltype(w)::value; });
+  return static_cast<size_t>(kCtasPerSm) * P->base.ctx->sm_count * 2 * subgroup_rows(P) * (width + 2) * sizeof(float);
 }
 
 cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const void* query, const int32_t* pages,
@@ -1001,7 +1040,7 @@ cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const vo
   d.rows = subgroup_rows(P);
   d.small_grid = 0;
   d.cluster = cluster_size(P, p, count);
-  return P->base.D == 64 ? launch_d<64>(P, d, stream) : launch_d<128>(P, d, stream);
+  return by_width(P, [&](auto w) { return launch_d<decltype(w)::value>(P, d, stream); });
 }
 
 }  // namespace tla

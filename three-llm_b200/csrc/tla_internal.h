@@ -64,7 +64,7 @@ struct tla_paged {
   tla_page_pool pool{};
   int io = 0, kept = 0;     // tla::Type of the activations and of the pages
   int page_shift = 0;       // log2(page_size)
-  bool wide = false;        // head_dim 64 or 128, rows of the pool on 16-byte boundaries
+  bool wide = false;        // head_dim a multiple of 8, rows of the pool on 16-byte boundaries
   float2* d_turns = nullptr;  // [kTurnSteps][rotary / 2]: cos and sin of 0, 1, .. steps of each pair
   int decode_cluster = 1;   // largest cluster of the decode kernel
   bool fast = false;        // tensor-core decode path (paged_decode_configure)
