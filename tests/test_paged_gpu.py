@@ -445,6 +445,23 @@ def test_append_other_head_dims(pkg, cuda, d, chunks):
     check_append(pkg, cuda, 4, 2, d, 8, "fp32", "fp32", [3, 12], chunks)
 
 
+@pytest.mark.parametrize("d", [8, 24, 72, 80, 100, 136, 200, 256])
+@pytest.mark.parametrize("chunks", [None, [70, 5]])
+def test_append_head_dims_normed(pkg, cuda, d, chunks):
+    g = torch.Generator().manual_seed(1)
+    norms = {k: torch.randn(d, generator=g).mul(0.3).add(1).numpy() for k in ("qNormWeight", "kNormWeight")}
+    check_append(pkg, cuda, 4, 2, d, 32, "bf16", "bf16", [3, 12], chunks, vNorm=True, **norms)
+    check_append(pkg, cuda, 13, 13, d, 64, "fp32", "fp32", [3, 12], chunks, "NHD", **norms)
+    if d >= 24:
+        check_append(pkg, cuda, 4, 2, d, 16, "fp32", "fp16", [3, 12], chunks, rotaryDim=16, offsetRMSNorm=True, **norms)
+
+
+@pytest.mark.parametrize("io,kept", PAIRS)
+def test_select_256_wide(pkg, cuda, io, kept):
+    w = World([1, 640, 333, 0, 1500], 2, 256, 16, kept)
+    check_select(pkg, cuda, w, 8, 2, 256, io, 9)
+
+
 def test_append_far_positions(pkg, cuda):
     """Angles of far positions are reduced in 64 bits."""
     hq, hk, d, page = 4, 2, 128, 16
@@ -652,11 +669,15 @@ def test_python_refuses(pkg, cuda):
 
 def test_append_refuses_rows_that_do_not_fit(pkg, cuda):
     """A head_dim that goes through shared memory row by row, with more heads than it holds."""
-    k, v = (torch.zeros(2, 64, 4, 80, dtype=torch.float16, device=cuda) for _ in range(2))
-    a = pkg.PagedAttention(640 * 80, 640, 8, k, v, {"headDim": 80, "kvHeadCount": 64})
+    k, v = (torch.zeros(2, 64, 4, 84, dtype=torch.float16, device=cuda) for _ in range(2))
+    a = pkg.PagedAttention(640 * 84, 640, 8, k, v, {"headDim": 84, "kvHeadCount": 64})
     with pytest.raises(pkg.TlaError, match="UNSUPPORTED"):
-        a.append(torch.zeros(1, 768 * 80, dtype=torch.float16, device=cuda), ints([0], cuda), ints([[0]], cuda))
+        a.append(torch.zeros(1, 768 * 84, dtype=torch.float16, device=cuda), ints([0], cuda), ints([[0]], cuda))
     torch.zeros(1, device=cuda)  # no CUDA error is left behind
+
+
+def test_append_many_heads(pkg, cuda):
+    check_append(pkg, cuda, 640, 64, 80, 4, "fp16", "fp16", [0, 5])
 
 
 def test_decode_gate_as_output(pkg, cuda):

@@ -235,14 +235,15 @@ __device__ __forceinline__ Raw4<T> lane_xor(Raw4<T> v, int o) {
     return {make_uint2(__shfl_xor_sync(0xffffffffu, v.u.x, o), __shfl_xor_sync(0xffffffffu, v.u.y, o))};
 }
 
-// head_dim 64 or 128, rotary dimensions a multiple of 8: D / 8 lanes hold a
-// head, each the four rotation pairs 4 l .. 4 l + 3 (both elements, so that no
-// lane needs another's; dimensions past the rotary ones pair up among
-// themselves and stay). `parts` warps share a row's heads, so that few rows
-// still fill the GPU; a warp forms the row's cosines and sines once, one or
-// two per lane, and hands them out by shuffles. Without `keys` the row's keys
-// are left to the blocks that go by pages. `unit`: the warp's (row, part).
-template <typename IO, typename CT, int D>
+// head_dim and the rotary dimensions multiples of 8: D / 8 lanes hold a head (D
+// is head_dim, or where !EXACT 128 or 256, its last lanes idle), each the four
+// rotation pairs 4 l .. 4 l + 3 (both elements, so that no lane needs another's;
+// dimensions past the rotary ones pair up among themselves and stay). `parts`
+// warps share a row's heads, so that few rows still fill the GPU; a warp forms
+// the row's cosines and sines once, one or two per lane, and hands them out by
+// shuffles (at 256 each lane its own four). Without `keys` the row's keys are
+// left to the blocks that go by pages. `unit`: the warp's (row, part).
+template <typename IO, typename CT, int D, bool EXACT>
 __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __restrict__ qkv,
                                             const int32_t* __restrict__ offsets, int rows,
                                             IO* __restrict__ query_out, int parts, int part_heads, bool keys,
@@ -253,15 +254,17 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
   const LayerArgs& a = p.a;
   const int Hq = a.Hq, Hk = a.Hk, heads = Hq + 2 * Hk, half = a.rotary / 2;
   const int lane = threadIdx.x & 31, group = lane / kLanes, i0 = 4 * (lane % kLanes);
+  const int hd = EXACT ? D : a.D;
+  const bool on = EXACT || 2 * i0 < hd;
   const int row = static_cast<int>(unit / parts), part = static_cast<int>(unit % parts);
   // the first elements of the lane's four pairs, and their partners
   const int d0 = i0 < half ? i0 : a.rotary + i0 - half;
-  const int d1 = d0 + (i0 < half ? half : (D - a.rotary) / 2);
+  const int d1 = d0 + (i0 < half ? half : (hd - a.rotary) / 2);
   if (row >= rows) return;
   // the part's heads: queries, keys (or none), values
   const int k_heads = keys ? Hk : 0, h_begin = part * part_heads;
   const int h_end = min(Hq + k_heads + Hk, h_begin + part_heads);
-  const IO* src = qkv + static_cast<int64_t>(row) * heads * D;
+  const IO* src = qkv + static_cast<int64_t>(row) * heads * hd;
   const int b = sequence_of_warp(offsets, p.batch, row, lane);
   if (b < 0) return;
   const int start = p.positions[b];
@@ -271,7 +274,8 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
     if (pos >= 0 && lane == 0) report_error(a.error, TLA_ERR_POSITION);
     if (query_out)
       for (int h = h_begin + group; h < min(h_end, Hq); h += kPer) {
-        IO* q = query_out + (static_cast<int64_t>(row) * Hq + h) * D;
+        IO* q = query_out + (static_cast<int64_t>(row) * Hq + h) * hd;
+        if (!on) continue;
         store4(q + d0, make_float4(0.f, 0.f, 0.f, 0.f));
         store4(q + d1, make_float4(0.f, 0.f, 0.f, 0.f));
       }
@@ -283,13 +287,19 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
   float cos4[4], sin4[4];
   if (h_begin < Hq + k_heads) {
     float c0 = 1.f, s0 = 0.f, c1 = 1.f, s1 = 0.f;
-    if (lane < min(a.pair_count, half)) rope_cos_sin(pos, a.inv_freq[lane], &c0, &s0);
+    if (D < 256 && lane < min(a.pair_count, half)) rope_cos_sin(pos, a.inv_freq[lane], &c0, &s0);
     if (D == 128 && lane + 32 < min(a.pair_count, half)) rope_cos_sin(pos, a.inv_freq[lane + 32], &c1, &s1);
     const int turned = i0 < half ? min(a.pair_count, half) - i0 : 0;  // of this lane's pairs, those before this one
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int src_lane = (i0 + e) & 31;
-      float c = __shfl_sync(full, c0, src_lane), s = __shfl_sync(full, s0, src_lane);
+      float c = 1.f, s = 0.f;
+      if (D == 256) {
+        if (e < turned) rope_cos_sin(pos, a.inv_freq[i0 + e], &c, &s);
+      } else {
+        c = __shfl_sync(full, c0, src_lane);
+        s = __shfl_sync(full, s0, src_lane);
+      }
       if (D == 128) {
         const float ch = __shfl_sync(full, c1, src_lane), sh = __shfl_sync(full, s1, src_lane);
         if (i0 + e >= 32) {
@@ -312,22 +322,22 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float add = a.offset_rms ? 1.f : 0.f;
-      const float wx = w == nullptr ? 1.f : add + w[d0 + e], wy = w == nullptr ? 1.f : add + w[d1 + e];
+      const float wx = w == nullptr || !on ? 1.f : add + w[d0 + e], wy = w == nullptr || !on ? 1.f : add + w[d1 + e];
       xc[e] = kKind == 2 ? 1.f : wx * cos4[e];
       xs[e] = kKind == 2 ? 0.f : wx * sin4[e];
       yc[e] = kKind == 2 ? 1.f : wy * cos4[e];
       ys[e] = kKind == 2 ? 0.f : wy * sin4[e];
     }
-    const IO* in = src + (from + group) * D;
-    IO* q = kKind == 0 ? query_out + (static_cast<int64_t>(row) * Hq + from + group) * D : nullptr;
+    const IO* in = src + (from + group) * hd;
+    IO* q = kKind == 0 ? query_out + (static_cast<int64_t>(row) * Hq + from + group) * hd : nullptr;
     CT* kv = kKind == 0 ? nullptr : static_cast<CT*>(kKind == 1 ? p.key : p.value) + pool_row(p, page, 0, slot);
-    for (int h0 = from + group; h0 - group < to; h0 += kLoads * kPer, in += kLoads * kPer * D, q += kLoads * kPer * D) {
+    for (int h0 = from + group; h0 - group < to; h0 += kLoads * kPer, in += kLoads * kPer * hd, q += kLoads * kPer * hd) {
       Raw4<IO> lo[kLoads], hi[kLoads];
 #pragma unroll
       for (int c = 0; c < kLoads; ++c) {
-        const bool on = h0 + c * kPer < to;
-        lo[c] = on ? raw4(in + c * kPer * D + d0) : Raw4<IO>{};
-        hi[c] = on ? raw4(in + c * kPer * D + d1) : Raw4<IO>{};
+        const bool in_part = on && h0 + c * kPer < to;
+        lo[c] = in_part ? raw4(in + c * kPer * hd + d0) : Raw4<IO>{};
+        hi[c] = in_part ? raw4(in + c * kPer * hd + d1) : Raw4<IO>{};
       }
       float r[kLoads];
       if (norm) {  // math.ts:78-97; the loads' sums go through the shuffles side by side
@@ -341,7 +351,7 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
 #pragma unroll
           for (int c = 0; c < kLoads; ++c) r[c] += __shfl_xor_sync(full, r[c], o);
 #pragma unroll
-        for (int c = 0; c < kLoads; ++c) r[c] = rsqrtf(r[c] * (1.f / D) + a.rms_eps);  // (2 ulp)
+        for (int c = 0; c < kLoads; ++c) r[c] = rsqrtf(r[c] * (1.f / hd) + a.rms_eps);  // (2 ulp)
       }
 #pragma unroll
       for (int c = 0; c < kLoads; ++c) {
@@ -358,10 +368,10 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
                           y.w * yc[3] + u.w * xs[3]);
         }
         const int h = h0 + c * kPer;
-        if (h >= to) continue;
+        if (h >= to || !on) continue;
         if (kKind == 0) {
-          store4(q + c * kPer * D + d0, x);
-          store4(q + c * kPer * D + d1, y);
+          store4(q + c * kPer * hd + d0, x);
+          store4(q + c * kPer * hd + d1, y);
         } else {
           const int kvh = h - Hq - (kKind == 1 ? 0 : Hk);
           CT* at = kv + kvh * p.head_stride;
@@ -373,8 +383,8 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
             store4(at + d1, y);
           }
           if (kKind == 1 && p.bounds && !offsets) {  // one new token: its page's bounds right here
-            CT* low = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * D;
-            CT* high = low + D;
+            CT* low = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * hd;
+            CT* high = low + hd;
             const Raw4<CT> k0 = pack4<CT>(x), k1 = pack4<CT>(y);
             put4(low + d0, slot == 0 ? k0 : low4<CT>(raw4(low + d0), k0));
             put4(low + d1, slot == 0 ? k1 : low4<CT>(raw4(low + d1), k1));
@@ -454,12 +464,13 @@ __device__ __forceinline__ bool find_page(const PagedArgs& p, const int32_t* off
 // of the first slot and a table of those of 0 .. kPageSlots - 1 steps:
 // cos(a + b) = cos a cos b - sin a sin b and its like add three roundings and
 // spare 31 of 32 evaluations, which with few rows per block would bound it.
-constexpr int kPageThreads = 256, kPageSlots = kTurnSteps;
-template <typename IO, typename CT, int D>
+constexpr int kPageThreads = 256;
+template <typename IO, typename CT, int D, bool EXACT>
 __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __restrict__ qkv,
                                             const int32_t* __restrict__ offsets, int rows, int heads, int unit) {
   constexpr int kLanes = D / 8, kPer = 32 / kLanes, kWarps = kPageThreads / 32;
   constexpr int kLoads = 4;  // warp-wide loads in flight
+  constexpr int kPageSlots = D == 256 ? kTurnSteps / 2 : kTurnSteps;
   const unsigned full = 0xffffffffu;
   __shared__ float2 base_s[D / 2];
   __shared__ float2 turn_s[kPageSlots][D / 2];
@@ -467,6 +478,8 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
   const LayerArgs& a = p.a;
   const int Hk = a.Hk, half = a.rotary / 2, pairs = min(a.pair_count, half);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = lane / kLanes, i0 = 4 * (lane % kLanes);
+  const int hd = EXACT ? D : a.D;
+  const bool on = EXACT || 2 * i0 < hd;
   const int groups = (Hk + heads - 1) / heads;
   int b, nth;
   if (!find_page<kPageThreads>(p, offsets, rows, unit / groups, &b, &nth)) return;
@@ -479,10 +492,10 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
   const int end = static_cast<int>(min(static_cast<int64_t>(size), c.start + static_cast<int64_t>(c.n) - from));
   const int64_t row0 = c.row + from - c.start;  // the row of slot 0 (of slots >= begin)
   const int d0 = i0 < half ? i0 : a.rotary + i0 - half;
-  const int d1 = d0 + (i0 < half ? half : (D - a.rotary) / 2);
+  const int d1 = d0 + (i0 < half ? half : (hd - a.rotary) / 2);
   const int shares = kWarps / heads, share = warp / heads;  // warps per head, and this one's place
   const int kvh = unit % groups * heads + warp % heads;
-  const int row_size = (a.Hq + 2 * Hk) * D;
+  const int row_size = (a.Hq + 2 * Hk) * hd;
   Raw4<CT> low0 = pack4<CT>(make_float4(INFINITY, INFINITY, INFINITY, INFINITY)), low1 = low0;
   Raw4<CT> high0 = pack4<CT>(make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY)), high1 = high0;
   for (int s0 = begin; s0 < end; s0 += kPageSlots) {
@@ -505,15 +518,15 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
     }
     __syncthreads();
     if (kvh >= Hk) continue;
-    const IO* in = qkv + (row0 + s0) * row_size + (a.Hq + kvh) * D;
+    const IO* in = qkv + (row0 + s0) * row_size + (a.Hq + kvh) * hd;
     CT* out = static_cast<CT*>(p.key) + pool_row(p, page, kvh, s0);
     for (int s1 = share * kPer + group; s1 - group < slots; s1 += shares * kPer * kLoads) {
       Raw4<IO> lo[kLoads], hi[kLoads];
 #pragma unroll
       for (int k = 0; k < kLoads; ++k) {
         const int s = s1 + k * shares * kPer;
-        lo[k] = s < slots ? raw4(in + static_cast<int64_t>(s) * row_size + d0) : Raw4<IO>{};
-        hi[k] = s < slots ? raw4(in + static_cast<int64_t>(s) * row_size + d1) : Raw4<IO>{};
+        lo[k] = on && s < slots ? raw4(in + static_cast<int64_t>(s) * row_size + d0) : Raw4<IO>{};
+        hi[k] = on && s < slots ? raw4(in + static_cast<int64_t>(s) * row_size + d1) : Raw4<IO>{};
       }
 #pragma unroll
       for (int k = 0; k < kLoads; ++k) {
@@ -526,15 +539,15 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
           for (int e = 0; e < 4; ++e) ss += x[e] * x[e] + y[e] * y[e];
 #pragma unroll
           for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(full, ss, o);
-          const float r = rsqrtf(ss * (1.f / D) + a.rms_eps);  // (2 ulp)
+          const float r = rsqrtf(ss * (1.f / hd) + a.rms_eps);  // (2 ulp)
           const float add = a.offset_rms ? 1.f : 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[e] *= r * (add + __ldg(a.k_norm + d0 + e));
-            y[e] *= r * (add + __ldg(a.k_norm + d1 + e));
+            x[e] *= r * (on ? add + __ldg(a.k_norm + d0 + e) : 0.f);
+            y[e] *= r * (on ? add + __ldg(a.k_norm + d1 + e) : 0.f);
           }
         }
-        if (s >= slots) continue;
+        if (s >= slots || !on) continue;
         if (i0 < half) {  // RoPE, math.ts:134-147
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -563,24 +576,24 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
     high0 = high4<CT>(high0, lane_xor<CT>(high0, o));
     high1 = high4<CT>(high1, lane_xor<CT>(high1, o));
   }
-  if (group == 0) {
+  if (group == 0 && on) {
     *reinterpret_cast<float4*>(&join_s[warp][0][d0]) = floats(low0);
     *reinterpret_cast<float4*>(&join_s[warp][0][d1]) = floats(low1);
     *reinterpret_cast<float4*>(&join_s[warp][1][d0]) = floats(high0);
     *reinterpret_cast<float4*>(&join_s[warp][1][d1]) = floats(high1);
   }
   __syncthreads();
-  for (int i = tid; i < heads * 2 * D; i += kPageThreads) {  // [head][low, high][d]
-    const int h = i / (2 * D), at = i - h * 2 * D, head = unit % groups * heads + h;
-    const bool is_low = at < D;
-    const int e = is_low ? at : at - D;
+  for (int i = tid; i < heads * 2 * hd; i += kPageThreads) {  // [head][low, high][d]
+    const int h = i / (2 * hd), at = i - h * 2 * hd, head = unit % groups * heads + h;
+    const bool is_low = at < hd;
+    const int e = is_low ? at : at - hd;
     if (head >= Hk) continue;
     float v = join_s[h][is_low ? 0 : 1][e];
     for (int k = 1; k < shares; ++k) {
       const float u = join_s[h + k * heads][is_low ? 0 : 1][e];
       v = (is_low ? u < v : u > v) ? u : v;
     }
-    CT* to = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + head) * 2 * D + at;
+    CT* to = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + head) * 2 * hd + at;
     if (begin > 0) {
       const float u = to_f32(to[0]);
       v = (is_low ? v < u : v > u) ? v : u;
@@ -590,29 +603,29 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
 }
 
 // Rows only.
-template <typename IO, typename CT, int D>
+template <typename IO, typename CT, int D, bool EXACT>
 __global__ void __launch_bounds__(kThreads, 5)
     paged_append_rows_kernel(PagedArgs p, const IO* __restrict__ qkv, const int32_t* __restrict__ offsets, int rows,
                              IO* __restrict__ query_out, int parts, int part_heads) {
   griddep_wait();
   griddep_launch_dependents();
-  append_rows<IO, CT, D>(p, qkv, offsets, rows, query_out, parts, part_heads, true,
-                         static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5));
+  append_rows<IO, CT, D, EXACT>(p, qkv, offsets, rows, query_out, parts, part_heads, true,
+                                static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5));
 }
 
 // Chunks into a pool with bounds: the first blocks take the touched pages'
 // keys, the others the rows' queries and values.
-template <typename IO, typename CT, int D, int kBlocks>
+template <typename IO, typename CT, int D, bool EXACT, int kBlocks>
 __global__ void __launch_bounds__(kPageThreads, kBlocks)
     paged_append_chunks_kernel(PagedArgs p, const IO* __restrict__ qkv, const int32_t* __restrict__ offsets, int rows,
                                IO* __restrict__ query_out, int parts, int part_heads, int page_blocks, int page_heads) {
   griddep_wait();
   griddep_launch_dependents();
   if (static_cast<int>(blockIdx.x) < page_blocks)
-    append_page<IO, CT, D>(p, qkv, offsets, rows, page_heads, blockIdx.x);
+    append_page<IO, CT, D, EXACT>(p, qkv, offsets, rows, page_heads, blockIdx.x);
   else
-    append_rows<IO, CT, D>(p, qkv, offsets, rows, query_out, parts, part_heads, false,
-                           static_cast<int64_t>(blockIdx.x - page_blocks) * (kPageThreads / 32) + (threadIdx.x >> 5));
+    append_rows<IO, CT, D, EXACT>(p, qkv, offsets, rows, query_out, parts, part_heads, false,
+                                  static_cast<int64_t>(blockIdx.x - page_blocks) * (kPageThreads / 32) + (threadIdx.x >> 5));
 }
 
 // Bounds of the pages that a chunk touched, any shape: the block of a page's
@@ -653,7 +666,7 @@ __global__ void __launch_bounds__(kThreads)
 
 // The layers that append_rows takes.
 bool by_rows(const tla_paged* P) {
-  return P->wide && (P->base.D == 64 || P->base.D == 128) && P->base.rotary % 8 == 0;
+  return P->wide && P->base.rotary % 8 == 0;
 }
 // Shared memory of the block-per-row kernel: the row in float32, its cosines and sines.
 size_t row_smem(const tla_paged* P) {
@@ -668,13 +681,16 @@ cudaError_t append_t(const tla_paged* P, const PagedArgs& p, const void* qkv, co
   if (by_rows(P)) {
     // Warps per row: enough for 16 on every SM, at most one per warp-wide load
     // (64 rows of 48 heads: 12 warps per row).
-    const int heads = p.a.Hq + (by_pages ? 1 : 2) * p.a.Hk, per = 256 / D, most = (heads + per - 1) / per;
+    const int heads = p.a.Hq + (by_pages ? 1 : 2) * p.a.Hk, per = 256 / (D == 64 ? 64 : D <= 128 ? 128 : 256), most = (heads + per - 1) / per;
     long long parts = (16LL * P->base.ctx->sm_count + rows - 1) / rows;
     parts = parts < 1 ? 1 : parts > most ? most : parts;
     const int part_heads = (most + static_cast<int>(parts) - 1) / static_cast<int>(parts) * per;
     parts = (heads + part_heads - 1) / part_heads;
     if (!by_pages) {
-      auto k = D == 64 ? paged_append_rows_kernel<IO, CT, 64> : paged_append_rows_kernel<IO, CT, 128>;
+      auto k = D == 64    ? paged_append_rows_kernel<IO, CT, 64, true>
+               : D == 128 ? paged_append_rows_kernel<IO, CT, 128, true>
+               : D < 128  ? paged_append_rows_kernel<IO, CT, 128, false>
+                          : paged_append_rows_kernel<IO, CT, 256, false>;
       return launch_pdl(k, static_cast<unsigned>((rows * parts + 3) / 4), kThreads, 0, stream, p,
                         static_cast<const IO*>(qkv), offsets, rows, static_cast<IO*>(query_out),
                         static_cast<int>(parts), part_heads);
@@ -695,8 +711,11 @@ cudaError_t append_t(const tla_paged* P, const PagedArgs& p, const void* qkv, co
     const int warps = kPageThreads / 32;
     const long long grid = blocks + (rows * parts + warps - 1) / warps;
     const bool many = grid > 6LL * P->base.ctx->sm_count;
-    auto k = D == 64 ? (many ? paged_append_chunks_kernel<IO, CT, 64, 4> : paged_append_chunks_kernel<IO, CT, 64, 3>)
-                     : (many ? paged_append_chunks_kernel<IO, CT, 128, 4> : paged_append_chunks_kernel<IO, CT, 128, 3>);
+    auto k = D < 128 ? paged_append_chunks_kernel<IO, CT, 128, false, 3> : paged_append_chunks_kernel<IO, CT, 256, false, 3>;
+    if (D == 64)
+      k = many ? paged_append_chunks_kernel<IO, CT, 64, true, 4> : paged_append_chunks_kernel<IO, CT, 64, true, 3>;
+    if (D == 128)
+      k = many ? paged_append_chunks_kernel<IO, CT, 128, true, 4> : paged_append_chunks_kernel<IO, CT, 128, true, 3>;
     return launch_pdl(k, static_cast<unsigned>(grid), kPageThreads, 0, stream, p, static_cast<const IO*>(qkv), offsets, rows, static_cast<IO*>(query_out), static_cast<int>(parts),
                       part_heads, static_cast<int>(blocks), page_heads);
   }

@@ -213,7 +213,7 @@ __device__ __forceinline__ void score_32(const PagedArgs& p, const double* vec, 
 template <typename CT>
 __device__ __forceinline__ int piece_lanes(int D) {
   const int reads = 2 * D * static_cast<int>(sizeof(CT)) / 16;
-  return D == 64 || D == 128 ? min(reads, 32) : 0;
+  return D == 64 || D == 128 || D == 256 ? min(reads, 32) : 0;
 }
 template <typename CT, typename Put>
 __device__ __forceinline__ void score_any(const PagedArgs& p, const double* vec, int kvh, PageRange r, int first,
@@ -222,6 +222,8 @@ __device__ __forceinline__ void score_any(const PagedArgs& p, const double* vec,
     score_32<CT, 128>(p, vec, kvh, r, first, last, from, step, raw, put);
   else if (p.a.D == 64)
     score_32<CT, 64>(p, vec, kvh, r, first, last, from, step, raw, put);
+  else if (p.a.D == 256)
+    score_32<CT, 256>(p, vec, kvh, r, first, last, from, step, raw, put);
   else
     score_32<CT, 0>(p, vec, kvh, r, first, last, from, step, raw, put);
 }
