@@ -131,6 +131,18 @@ def test_decode_other_head_dims(pkg, cuda, d, io, kept):
     check_decode(pkg, cuda, [1, 33, 130], 6, 2, d, 16, io, kept)
 
 
+@pytest.mark.parametrize("d", [8, 24, 64, 80, 128, 200, 256])
+@pytest.mark.parametrize("io,kept,page", [("fp32", "fp32", 16), ("fp32", "fp32", 1), ("fp32", "bf16", 64),
+                                          ("bf16", "bf16", 4), ("fp16", "fp16", 8)])
+def test_decode_rows(pkg, cuda, d, io, kept, page):
+    """What goes row by row: float32 pages, float32 over bfloat16 pages, small pages."""
+    check_decode(pkg, cuda, [1, 17, 64, 300, 0, 1000], 6, 2, d, page, io, kept, gated=True)
+    check_decode(pkg, cuda, [77, 500], 10, 1, d, page, io, kept, layout="NHD", window=90)
+    if page > 1:
+        check_decode(pkg, cuda, [70, 200], 4, 2, d, page, io, kept,
+                     listed=[[[0, 1], [0, 2, 3]], [[1], [0, 2, 199 // page]]] if page < 64 else [[[0, 1], [1]], [[0, 3], [2]]])
+
+
 @pytest.mark.parametrize("d", [8, 24, 72, 80, 96, 136, 200, 256])
 @pytest.mark.parametrize("io,kept", [("fp16", "fp16"), ("bf16", "bf16"), ("fp32", "fp16")])
 @pytest.mark.parametrize("wide", [1, 9000])
