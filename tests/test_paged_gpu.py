@@ -143,6 +143,24 @@ def test_decode_rows(pkg, cuda, d, io, kept, page):
                      listed=[[[0, 1], [0, 2, 3]], [[1], [0, 2, 199 // page]]] if page < 64 else [[[0, 1], [1]], [[0, 3], [2]]])
 
 
+@pytest.mark.parametrize("d,io,kept,page,wide", [
+    (64, "fp16", "fp16", 16, 1), (128, "bf16", "bf16", 64, 1), (256, "fp32", "fp16", 16, 1), (64, "fp16", "fp16", 16, 9000),
+    (128, "fp32", "fp16", 16, 9000), (64, "fp32", "fp32", 16, 1), (100, "fp16", "fp16", 16, 1)])
+def test_decode_nan_among_the_tokens(pkg, cuda, d, io, kept, page, wide):
+    """A NaN in a key or value that takes part shows in the heads that read it, also where it is the only token."""
+    lengths = [1, 40, 700, 1, 700]
+    w = World(lengths, 2, d, page, kept, extra_width=wide)
+    at = [w.table[i][n] for i, n in ((0, 0), (1, 37 // page), (2, 650 // page))]
+    w.keys[at[0], 0, 0, d - 1] = float("nan")
+    w.keys[at[1], 1, 37 % page, 0] = float("nan")
+    w.values[at[2], 1, 650 % page] = float("nan")
+    layer, *_ = make(pkg, cuda, w, 6, 2, d, io)
+    out = layer.decode(w.normal(5, 6 * d, dtype=TYPES[io]).to(cuda), ints([n - 1 for n in lengths], cuda),
+                       w.device_table(cuda))
+    bad = out.view(5, 2, 3 * d).isnan().cpu()
+    assert bad[0, 0].all() and bad[1, 1].all() and bad[2, 1].all() and int(bad.sum()) == 9 * d
+
+
 @pytest.mark.parametrize("d", [8, 24, 72, 80, 96, 136, 200, 256])
 @pytest.mark.parametrize("io,kept", [("fp16", "fp16"), ("bf16", "bf16"), ("fp32", "fp16")])
 @pytest.mark.parametrize("wide", [1, 9000])

@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         v1 += x.y * f;
       }
       if (whole) {
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
         if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c, v0 * inv);
         if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c + 1, v1 * inv);
       } else if (d.cluster ||
@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         v0 += x[k].x * f;
         v1 += x[k].y * f;
       }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
       store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c, v0 * inv);
       store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c + 1, v1 * inv);
     }
@@ -820,14 +820,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
     float high = top;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) high = fmaxf(high, mk[u]);
-    if (high == -INFINITY) continue;
-    const float keep = ex2(top - high);
+    const float base = high == -INFINITY ? 0.f : high, keep = ex2(top - base);
     sum *= keep;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) acc[e] *= keep;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const float f = ex2(mk[u] - high);
+      const float f = ex2(mk[u] - base);
       sum += lk[u] * f;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) acc[e] += v[u][e] * f;
@@ -838,7 +837,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
       if (lane + 32 * e < p.a.D)
-        store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + lane + 32 * e, sum > 0.f ? acc[e] / sum : 0.f);
+        store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + lane + 32 * e, sum != 0.f ? acc[e] / sum : 0.f);
     return;
   }
   if (lane == 0) {
@@ -851,17 +850,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
   float high = red[0][0];
 #pragma unroll
   for (int w = 1; w < kJoinWarps; ++w) high = fmaxf(high, red[0][w]);
+  const float base = high == -INFINITY ? 0.f : high;
   for (int c = tid; c < p.a.D; c += kJoinWarps * 32) {
     float all = 0.f, v = 0.f;
-    if (high != -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) {
-        const float f = ex2(red[0][w] - high);
-        all += red[1][w] * f;
-        v += row_s[w][c] * f;
-      }
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const float f = ex2(red[0][w] - base);
+      all += red[1][w] * f;
+      v += row_s[w][c] * f;
     }
-    store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + c, all > 0.f ? v / all : 0.f);
+    store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + c, all != 0.f ? v / all : 0.f);
   }
 }
 
