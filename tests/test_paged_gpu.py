@@ -697,6 +697,34 @@ def test_python_refuses(pkg, cuda):
                                           None, q.data_ptr(), 2, at, size, None) == -1
 
 
+def test_overlaps_and_short_workspaces_are_refused(pkg, cuda):
+    k, v = (torch.zeros(4, 2, 16, 64, dtype=torch.float16, device=cuda) for _ in range(2))
+    bounds = torch.zeros(4, 2, 2, 64, dtype=torch.float16, device=cuda)
+    a = pkg.PagedAttention(512, 8, 1 << 16, k, v, {"headDim": 64, "kvHeadCount": 2}, key_bounds=bounds)
+    lib, pos, table = pkg.lib(), ints([3, 3], cuda), torch.zeros(2, 4096, dtype=torch.int32, device=cuda)
+    buf = torch.zeros(2 * 768 + 4096, dtype=torch.float16, device=cuda)
+    at, end = buf.data_ptr(), buf.data_ptr() + 2 * 768 * 2
+    need, choose = ctypes.c_size_t(), ctypes.c_size_t()
+    assert lib.tla_paged_workspace(a.handle, 2, 4096, 0, ctypes.byref(need), ctypes.byref(choose)) == 0 and need.value
+    work = torch.empty(need.value + choose.value + 16, dtype=torch.uint8, device=cuda)
+
+    def decode(out, w=work.data_ptr(), size=need.value, gate=None):
+        return lib.tla_paged_decode(a.handle, at, pos.data_ptr(), table.data_ptr(), 4096, None, 0, gate, out, 2, w, size,
+                                    None)
+
+    def select(out):
+        return lib.tla_paged_select(a.handle, at, pos.data_ptr(), table.data_ptr(), 4096, 1, 1, out, 4, 2,
+                                    work.data_ptr(), choose.value, None)
+
+    assert decode(end) == 0 and decode(end, gate=end) == 0 and select(end) == 0
+    assert decode(end, None, 0) == decode(end, size=need.value - 1) == decode(end, work.data_ptr() + 8) == -1
+    assert decode(at) == decode(at + 2 * 512 * 2 - 16) == decode(end, gate=end + 16) == -1
+    assert select(at) == select(at + 2 * 512 * 2 - 16) == -1
+    for out in (at, end - 16):
+        assert lib.tla_paged_append(a.handle, at, pos.data_ptr(), None, table.data_ptr(), 4096, 2, 2, out, None) == -1
+    torch.cuda.synchronize()
+
+
 def test_append_refuses_rows_that_do_not_fit(pkg, cuda):
     """A head_dim that goes through shared memory row by row, with more heads than it holds."""
     k, v = (torch.zeros(2, 64, 4, 84, dtype=torch.float16, device=cuda) for _ in range(2))

@@ -3,6 +3,7 @@
 // tla_paged_create or keeps anything between calls.
 #include <math.h>
 
+#include <memory>
 #include <new>
 #include <utility>
 
@@ -112,7 +113,9 @@ int tla_paged_create(tla_ctx* ctx, const tla_attn_config* cfg, const tla_page_po
       !aligned16(pool->bounds))
     return TLA_ERR_INVALID_ARG;
   DeviceGuard g(ctx->device);
-  tla_paged* P = new tla_paged();
+  std::unique_ptr<tla_paged, int (*)(tla_paged*)> owner(new tla_paged(), tla_paged_destroy);
+  tla_paged* P = owner.get();
+  P->base.ctx = ctx;
   L.ctx = ctx;
   L.k_cache = pool->key;
   L.v_cache = pool->value;
@@ -142,11 +145,8 @@ int tla_paged_create(tla_ctx* ctx, const tla_attn_config* cfg, const tla_page_po
     if (rc == TLA_OK)
       rc = from_cuda(cudaMemcpy(P->d_turns, turns.data(), turns.size() * sizeof(float2), cudaMemcpyHostToDevice));
   }
-  if (rc != TLA_OK) {
-    tla_paged_destroy(P);
-    return rc;
-  }
-  *out = P;
+  if (rc != TLA_OK) return rc;
+  *out = owner.release();
   return TLA_OK;
 } catch (const std::bad_alloc&) {
   return TLA_ERR_OUT_OF_MEMORY;
@@ -222,7 +222,10 @@ int tla_paged_select(tla_paged* P, const void* query, const int32_t* positions, 
     return TLA_ERR_INVALID_ARG;
   if (!P->pool.bounds || !(P->base.attn_scale > 0)) return TLA_ERR_UNSUPPORTED;
   if (batch == 0) return TLA_OK;
-  if (!query || !pages_out || !aligned16(query) || !aligned16(workspace)) return TLA_ERR_INVALID_ARG;
+  if (!query || !pages_out || !aligned16(query) || !aligned16(workspace) ||
+      overlap(query, batch * row_bytes(P, P->base.Hq), pages_out,
+              static_cast<size_t>(batch) * P->base.Hk * page_count * sizeof(int32_t)))
+    return TLA_ERR_INVALID_ARG;
   const size_t need = tla::paged_select_workspace(P, batch, table_width);
   if (need > 0 && (!workspace || workspace_bytes < need)) return TLA_ERR_INVALID_ARG;
   DeviceGuard g(P->base.ctx->device);
