@@ -7,6 +7,11 @@
 //
 // with angle position * inv_freq[j], reduced in 64 bits. Q goes to query_out,
 // K and V to their slots, K as stored into its page's bounds.
+//
+// Every value is read and written once, so memory bounds long calls: 20,500 rows
+// of 16 ragged chunks with bounds, 48 heads of 128, bfloat16, QK-norm, in 93 us
+// (0.86 of a copy's rate, issue slots 64% busy); one new token each of 64
+// sequences takes 2.6 us, a chain of offsets, position, table entry and row.
 #include <math.h>
 
 #include <type_traits>
