@@ -614,6 +614,14 @@ def test_select_block_and_cluster_sizes(pkg, cuda, n, batch):
     check_select(pkg, cuda, w, 8, 2, 64, "fp16", max(2, n // 5))
 
 
+@pytest.mark.parametrize("wide", [1, 300, 1200, 2000])
+@pytest.mark.parametrize("batch", [30, 74, 90, 200])
+def test_select_many_sequences(pkg, cuda, wide, batch):
+    """Blocks and clusters by the number of sequences, few of them as long as the table."""
+    w = World([(900, 8, 70, 0, 1)[i % 5] + i % 3 for i in range(batch)], 2, 64, 8, "bf16", extra_width=wide)
+    check_select(pkg, cuda, w, 4, 2, 64, "bf16", 7)
+
+
 def test_select_tiny_and_huge_keys(pkg, cuda):
     """Subnormal bounds and the type's largest values."""
     for kept, tiny in (("fp16", 2.0 ** -24), ("bf16", 2.0 ** -130)):

@@ -464,18 +464,26 @@ cudaError_t select_t(const tla_paged* P, const PagedArgs& p, const void* query, 
   cfg.numAttrs = 1;
   cfg.blockDim = dim3(kMaxWarps * 32);
   if (most <= kMaxHeld) {
-    // Larger blocks for longer sequences: their first one picks alone, and its
-    // rounds and the list's writing go over all pages.
-    auto k = paged_select_kernel<IO, CT, 128>;
-    int warps = 4;
-    if (most > 256) k = paged_select_kernel<IO, CT, 256>, warps = 8;
-    if (most > 1024) k = paged_select_kernel<IO, CT, 512>, warps = 16;
-    // Blocks per pair: up to eight per SM in all, at least two pages per warp.
+    // Larger blocks for longer sequences, whose first one picks alone, its rounds
+    // and the list's writing going over all pages; small ones, of which an SM
+    // runs more threads, where the pairs alone give every SM something to do
+    // while another picks. A cluster's blocks share the scores out, up to eight,
+    // at least two pages per warp, as long as all blocks run at once (five per
+    // SM of 128 threads, two of 256, one of 512; the longest ones up to 1.6
+    // times that). Measured (threads x blocks per pair, us): 512 pairs of 64
+    // pages 128 x 1 7.5, x 2 13.2; 160 of 1250 (128 wide) 128 x 4 36.7, 256 x 1
+    // 53, 512 x 2 52; 256 of 4000 256 x 1 91, 128 x 2 109, 512 x 2 111; 64 of 500
+    // (128 wide) 256 x 4 9.3, x 8 15.2; 114 of up to 5562 512 x 2 46, x 8 60; 32
+    // of 1875 512 x 4 13.8, x 8 22.2.
     // (Clusters of 16 leave a GPC's other SMs idle: 8 of them with 512 threads
     // each ran in two waves, 28 us for a sparse step at 131072 tokens.)
+    const int sms = P->base.ctx->sm_count;
+    auto k = paged_select_kernel<IO, CT, 128>;
+    int warps = 4, blocks = 5 * sms;
+    if (most > (pairs <= sms ? 256 : 1536)) k = paged_select_kernel<IO, CT, 256>, warps = 8, blocks = 2 * sms;
+    if (most > 1024 && pairs <= sms) k = paged_select_kernel<IO, CT, 512>, warps = 16, blocks = sms * 8 / 5;
     int shares = 1;
-    while (shares < kMaxCluster && pairs * shares * 2 <= 8 * P->base.ctx->sm_count && most > 2 * warps * shares)
-      shares *= 2;
+    while (shares < kMaxCluster && pairs * shares * 2 <= blocks && most > 2 * warps * shares) shares *= 2;
     const size_t smem = vec + (most > count ? most * sizeof(uint32_t) : 0);
     if (smem > 48 * 1024) {
       const cudaError_t e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem));
