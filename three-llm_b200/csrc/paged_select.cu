@@ -25,6 +25,9 @@ constexpr int kMaxWarps = 16;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxHeld = 48 * 1024;  // ranks that one block's shared memory holds
 constexpr int kScorePages = 32 * kMaxWarps;  // pages per block of the scoring kernel for longer sequences
+// What a block gets without asking, its own variables counted in: 48 KB (and 1
+// KB left over here for their padding).
+constexpr size_t kDefaultSmem = 47 * 1024;
 
 // Larger scores have larger keys, and every score a key above 0.
 __device__ __forceinline__ uint32_t rank_of(float s) {
@@ -485,7 +488,7 @@ cudaError_t select_t(const tla_paged* P, const PagedArgs& p, const void* query, 
     int shares = 1;
     while (shares < kMaxCluster && pairs * shares * 2 <= blocks && most > 2 * warps * shares) shares *= 2;
     const size_t smem = vec + (most > count ? most * sizeof(uint32_t) : 0);
-    if (smem > 48 * 1024) {
+    if (smem + sizeof(PickSmem) > kDefaultSmem) {
       const cudaError_t e = raise_smem_limit(reinterpret_cast<const void*>(k), static_cast<int>(smem));
       if (e != cudaSuccess) return e;
     }
