@@ -6,6 +6,9 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
+
+from tests.test_paged_gpu import ints
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +41,14 @@ def test_select_from_tables_near_the_default_shared_memory(pkg, cuda, d, batch):
     r = subprocess.run([sys.executable, "-c", SELECT_TABLES.format(root=str(ROOT), d=d, batch=batch)], cwd=ROOT,
                        capture_output=True, text=True, timeout=600)
     assert r.returncode == 0 and "all tables done" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+# ---------------------------------------------------------------- errors
+def test_a_failed_call_leaves_no_error_for_the_next(pkg, cuda):
+    """A refused allocation is reported by its own call and not by a later launch."""
+    small = pkg.CUDAAttention(None, 160, 2, 16, {"headDim": 80, "ropeTheta": 1e4})
+    qkv, pos = torch.ones(1, 480, dtype=torch.float16, device=cuda), ints([0], cuda)
+    exp = small.decode(qkv, pos)
+    with pytest.raises(pkg.TlaError, match="OUT_OF_MEMORY"):
+        pkg.CUDAAttention(None, 64 * 256, 64, (1 << 31) - 1, {"headDim": 256, "maxBatch": 1024})
+    assert torch.equal(small.decode(qkv, pos), exp)

@@ -28,6 +28,7 @@
 
 #include "exchange.cuh"
 #include "tla_device.cuh"
+#include "tla_host.h"
 #include "tla_internal.h"
 
 namespace tla {
@@ -1522,10 +1523,9 @@ extern "C" int tla_decode_noalloc(const tla_attn_config* cfg, void* key_cache, v
   // zero the completion counters this launch uses.
   store_inv_freq_kernel<<<1, 64, 0, st>>>(L.d_inv_freq, inv);
   if (cudaGetLastError() != cudaSuccess) return TLA_ERR_CUDA;
-  if (cudaMemsetAsync(ctx.d_counters, 0, sizeof(int32_t) * batch * Hk, st) != cudaSuccess) return TLA_ERR_CUDA;
-  const cudaError_t e =
-      launch_decode_fast(&L, qkv, positions, gate, out, nullptr, batch, 0, cfg->max_tokens, 1, st);
-  return e == cudaSuccess ? TLA_OK : TLA_ERR_CUDA;
+  const cudaError_t e = cudaMemsetAsync(ctx.d_counters, 0, sizeof(int32_t) * batch * Hk, st);
+  if (e != cudaSuccess) return from_cuda(e);
+  return from_cuda(launch_decode_fast(&L, qkv, positions, gate, out, nullptr, batch, 0, cfg->max_tokens, 1, st));
 }
 
 #ifdef TLA_DECODE_TRACE

@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "exchange.cuh"
+#include "tla_host.h"
 #include "tla_internal.h"
 
 struct tla_exchange {
@@ -99,7 +100,7 @@ int tla_exchange_create(tla_ctx* ctx, int32_t rank, int32_t ranks, size_t slot_b
   if (prev >= 0) cudaSetDevice(prev);
   if (e != cudaSuccess) {
     tla_exchange_destroy(ex);
-    return e == cudaErrorMemoryAllocation ? TLA_ERR_OUT_OF_MEMORY : TLA_ERR_CUDA;
+    return tla::from_cuda(e);
   }
   ex->peers.assign(ranks, nullptr);
   ex->opened.assign(ranks, 0);
@@ -126,7 +127,7 @@ int tla_exchange_connect(tla_exchange* ex, const void* handles) {
   if (e == cudaSuccess)
     e = cudaMemcpy(ex->d_peers, ex->peers.data(), sizeof(uint8_t*) * ex->ranks, cudaMemcpyHostToDevice);
   if (prev >= 0) cudaSetDevice(prev);
-  if (e != cudaSuccess) return TLA_ERR_CUDA;
+  if (e != cudaSuccess) return tla::from_cuda(e);
   ex->connected = 1;
   return TLA_OK;
 }
@@ -148,7 +149,7 @@ int tla_exchange_connect_buffers(tla_exchange* ex, void* const* buffers) {
   const cudaError_t e =
       cudaMemcpy(ex->d_peers, ex->peers.data(), sizeof(uint8_t*) * ex->ranks, cudaMemcpyHostToDevice);
   if (prev >= 0) cudaSetDevice(prev);
-  if (e != cudaSuccess) return TLA_ERR_CUDA;
+  if (e != cudaSuccess) return tla::from_cuda(e);
   ex->connected = 1;
   return TLA_OK;
 }
@@ -180,7 +181,7 @@ int tla_exchange_combine(tla_exchange* ex, const float* partial, int32_t batch, 
                                                                   static_cast<__half*>(out), ex->ctx->d_error);
   const cudaError_t e = cudaGetLastError();
   if (prev >= 0) cudaSetDevice(prev);
-  return e == cudaSuccess ? TLA_OK : TLA_ERR_CUDA;
+  return tla::from_cuda(e);
 }
 
 int tla_out_proj_allreduce(tla_exchange* ex, const void* attn, const void* weight, const float* bias,
@@ -202,7 +203,7 @@ int tla_out_proj_allreduce(tla_exchange* ex, const void* attn, const void* weigh
       tla::launch_out_proj_allreduce(ex->ctx, x, attn, weight, bias, residual, (io_flags & TLA_FLAG_IO_FP32) != 0, y,
                                      rows, in_features, hidden, static_cast<cudaStream_t>(stream));
   if (prev >= 0) cudaSetDevice(prev);
-  return e == cudaSuccess ? TLA_OK : TLA_ERR_CUDA;
+  return tla::from_cuda(e);
 }
 
 int tla_exchange_destroy(tla_exchange* ex) {

@@ -26,8 +26,11 @@ struct DeviceGuard {
   }
 };
 
+// The status of a runtime call. A failed call's error is taken off the runtime's
+// record, where a later launch's check would find it and report it as its own.
 inline int from_cuda(cudaError_t e) {
   if (e == cudaSuccess) return TLA_OK;
+  cudaGetLastError();
   if (getenv("TLA_DEBUG")) fprintf(stderr, "tla: CUDA error %d: %s\n", static_cast<int>(e), cudaGetErrorString(e));
   if (e == cudaErrorMemoryAllocation) return TLA_ERR_OUT_OF_MEMORY;
   return TLA_ERR_CUDA;
