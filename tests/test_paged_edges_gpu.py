@@ -1,6 +1,7 @@
 """Edges of the paged cache on the GPU, at sizes and values where a rounding, a
 limit or an address goes wrong. Worlds and 64-bit forms are those of
 test_paged_gpu.py and paged_ref.py."""
+import math
 import subprocess
 import sys
 from pathlib import Path
@@ -8,7 +9,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from tests.test_paged_gpu import ints
+from tests.test_paged_gpu import TYPES, WIDE, World, ints, make
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +53,39 @@ def test_a_failed_call_leaves_no_error_for_the_next(pkg, cuda):
     with pytest.raises(pkg.TlaError, match="OUT_OF_MEMORY"):
         pkg.CUDAAttention(None, 64 * 256, 64, (1 << 31) - 1, {"headDim": 256, "maxBatch": 1024})
     assert torch.equal(small.decode(qkv, pos), exp)
+
+
+# ---------------------------------------------------------------- decode: the weights' roundings
+def places(w, n):
+    """(pages, slots) of the first sequence's n tokens."""
+    t = torch.arange(n)
+    return torch.tensor(w.table[0])[t // w.page], t % w.page
+
+
+def worst_gap(dtype, low, high):
+    """The number of the type between low and high whose weight 2^-gap is furthest from the type's own, relative to it."""
+    gap = torch.arange(low, high, torch.finfo(dtype).eps, dtype=torch.float64).to(dtype).double().unique()
+    weight = torch.exp2(-gap)
+    return float(gap[((weight.to(dtype).double() - weight).abs() / weight).argmax()])
+
+
+@pytest.mark.parametrize("io,kept", [("fp32", "fp16"), ("fp16", "fp16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("wide", [1, WIDE])
+@pytest.mark.parametrize("low", [0.5, 1.5, 4.5])
+def test_decode_gives_a_constant_back(pkg, cuda, io, kept, wide, low):
+    """Where all values are one number, the output is that number whatever the weights are rounded to: the sum is of
+    the weights that the values are multiplied with."""
+    n, d, page = 700, 64, 16
+    w = World([n], 1, d, page, kept, extra_width=wide)
+    p, s = places(w, n)
+    c = 2 - 2 * torch.finfo(w.kept).eps  # of all numbers the one whose half step is the smallest part of it, or nearly
+    w.keys[p, 0, s] = 0
+    w.keys[p[5::16], 0, s[5::16], 0] = worst_gap(w.kept, low, low + 0.5)
+    w.values[p, 0, s] = c
+    layer, *_ = make(pkg, cuda, w, 8, 1, d, io, attnScale=math.log(2.0))
+    q = torch.zeros(1, 8, d, dtype=TYPES[io])
+    q[..., 0] = 1
+    out = layer.decode(q.view(1, -1).to(cuda), ints([n - 1], cuda), w.device_table(cuda)).double().cpu()
+    # float32: weights in two parts against their 32-bit sum, and at most 40 additions of either, 2^-23 each; the
+    # 16-bit types have the constant's neighbours further off than that
+    assert (out - c).abs().max() <= (2.0 ** -17 * c if io == "fp32" else 0.0)

@@ -239,6 +239,15 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
 }
+// The two values of a packed pair.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {  // a float's upper half
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
 // What pack_half2 rounded away of (lo, hi), as a pair of its own.
 __device__ __forceinline__ uint32_t pack_rest(uint32_t packed, float lo, float hi) {
   const float2 f = __half22float2(*reinterpret_cast<__half2*>(&packed));
@@ -607,13 +616,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
           for (int u = 0; u < kGroups; ++u) {
             float pr[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              pr[e] = ex2(x[u][nt][e] - base[e & 1]);
-              l[nt][e & 1] += pr[e];
-            }
+            for (int e = 0; e < 4; ++e) pr[e] = ex2(x[u][nt][e] - base[e & 1]);
             // P rounded to the pages' type: its products with V then run on
-            // the tensor cores (SPLIT keeps the rest as a second operand)
+            // the tensor cores (SPLIT keeps the rest as a second operand). The
+            // sum is of the weights that V is multiplied with, so that the
+            // output stays a mean of the values: what all weights lose or gain
+            // alike cancels.
             const uint32_t p0 = pack2<CT>(pr[0], pr[1]), p1 = pack2<CT>(pr[2], pr[3]);
+            if constexpr (SPLIT) {
+              l[nt][0] += pr[0] + pr[2];
+              l[nt][1] += pr[1] + pr[3];
+            } else {
+              const float2 r0 = unpack2<CT>(p0), r1 = unpack2<CT>(p1);
+              l[nt][0] += r0.x + r1.x;
+              l[nt][1] += r0.y + r1.y;
+            }
             pb[u][nt][0] = transpose8(p0);
             pb[u][nt][1] = transpose8(p1);
             if constexpr (SPLIT) {
