@@ -9,7 +9,8 @@ from pathlib import Path
 import pytest
 import torch
 
-from tests.test_paged_gpu import TYPES, WIDE, World, ints, make
+from tests import paged_ref as ref
+from tests.test_paged_gpu import TYPES, WIDE, World, close, ints, make
 
 pytestmark = pytest.mark.gpu
 
@@ -60,6 +61,84 @@ def places(w, n):
     """(pages, slots) of the first sequence's n tokens."""
     t = torch.arange(n)
     return torch.tensor(w.table[0])[t // w.page], t % w.page
+
+
+def dominated(n, d, page, kept, gaps, wide, every):
+    """One sequence, one kv head: token 5 and each `every`-th after it have the top score and values of zeros, the
+    others lie `gaps` below it in powers of two (given attnScale = ln 2 and the query (1, 0, ...)), so that the output
+    is what they sum up to."""
+    w = World([n], 1, d, page, kept, extra_width=wide)
+    p, s = places(w, n)
+    below = torch.tensor(gaps, dtype=torch.float64)[torch.arange(n) % len(gaps)]
+    top = torch.arange(5, n, every)
+    below[top] = 0
+    w.keys[p, 0, s] = 0
+    w.keys[p, 0, s, 0] = (8.0 - below).to(w.kept)
+    w.values[p, 0, s] = (w.values[p, 0, s].abs() + 0.5) * 4096
+    w.values[p[top], 0, s[top]] = 0
+    return w
+
+
+def check_dominated(pkg, cuda, w, n, hq, d, io, kept):
+    layer, *_ = make(pkg, cuda, w, hq, 1, d, io, attnScale=math.log(2.0))
+    q = torch.zeros(1, hq, d, dtype=TYPES[io])
+    q[..., 0] = 1
+    out = layer.decode(q.view(1, -1).to(cuda), ints([n - 1], cuda), w.device_table(cuda))
+    assert layer.context.error() == 0
+    p, s = places(w, n)
+    k, v = w.keys[p, 0, s].double(), w.values[p, 0, s].double()
+    weight = torch.softmax(k[:, 0] * math.log(2.0), 0)
+    exp = weight @ v
+    # A score carries the roundings of its product, the scale and log2(e), 2^-22 of at most 32 powers of two; the sums
+    # run in 32 bits over n / 16 steps spread over 32 warps at least, then 24 joins, 2^-22 each (the tensor cores cut
+    # off). A weight is kept in 22 bits (two fp16 parts), 11 or 8, and its smallest part no finer than 2^-39 of the
+    # largest (fp16: half of 2^-24 under a top of 2^14).
+    share = 32 * 2.0 ** -22 * 2 + (n / 16 / 32 + 24) * 2.0 ** -22
+    share += {"fp32": 2.0 ** -21, "fp16": 2 * 2.0 ** -11, "bf16": 2 * 2.0 ** -8}[io]
+    tol = share * exp + (0 if io == "bf16" else n * 2.0 ** -39 * v.max() / (weight / weight.max()).sum())
+    tol = tol + ref.half_step(TYPES[io]) * exp + ref.smallest(TYPES[io])
+    for h in range(hq):
+        close(out[0].view(hq, d)[h], exp, tol, f"head {h}")
+
+
+@pytest.mark.parametrize("io,kept", [("fp32", "fp16"), ("fp16", "fp16"), ("bf16", "bf16"), ("fp32", "fp32")])
+@pytest.mark.parametrize("gap", [12.0, 20.0, 24.40625, 25.203125, 26.0])
+@pytest.mark.parametrize("d,wide", [(64, 1), (64, WIDE), (128, 1), (256, 1)])
+@pytest.mark.parametrize("every", [16, 10000])
+def test_decode_many_small_weights(pkg, cuda, io, kept, gap, d, wide, every):
+    """Thousands of equal weights far below one, among few large ones or beside a single one: together they count, and
+    equal roundings add up."""
+    w = dominated(8193, d, 16, kept, [gap], wide, every)
+    check_dominated(pkg, cuda, w, 8193, 8, d, io, kept)
+
+
+@pytest.mark.parametrize("io,kept", [("fp32", "fp16"), ("fp16", "fp16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("hq", [3, 16])
+def test_decode_weights_of_every_size(pkg, cuda, io, kept, hq):
+    w = dominated(4097, 64, 32, kept, [1.0 + 0.25 * i for i in range(107)], 1, 16)
+    check_dominated(pkg, cuda, w, 4097, hq, 64, io, kept)
+
+
+@pytest.mark.parametrize("io,kept", [("fp32", "fp16"), ("fp16", "fp16"), ("bf16", "bf16"), ("fp32", "bf16"), ("fp32", "fp32")])
+@pytest.mark.parametrize("top", [2.0 ** e for e in (0, 10, 20, 24, 25, 26, 27, 28, 29, 30)])
+def test_decode_equal_scores_of_any_size(pkg, cuda, io, kept, top):
+    """The same key everywhere, its score up to where a float's step is larger than any weight's exponent: the mean of
+    the values."""
+    n, d, page = 333, 64, 16
+    w = World([n], 1, d, page, kept)
+    p, s = places(w, n)
+    w.keys[p, 0, s] = 0
+    w.keys[p, 0, s, 0] = 2.0 ** 15
+    layer, *_ = make(pkg, cuda, w, 4, 1, d, io, attnScale=1.0)
+    q = torch.zeros(1, 4, d, dtype=TYPES[io])
+    q[..., 0] = top / 2 ** 15
+    out = layer.decode(q.view(1, -1).to(cuda), ints([n - 1], cuda), w.device_table(cuda))
+    v = w.values[p, 0, s].double()
+    size = v.abs().mean(0)
+    # equal weights: what they are rounded to cancels; sums in 32 bits, then the output's own rounding
+    tol = 64 * 2.0 ** -22 * size + ref.half_step(TYPES[io]) * v.mean(0).abs() + ref.smallest(TYPES[io])
+    for h in range(4):
+        close(out.view(4, d)[h], v.mean(0), tol)
 
 
 def worst_gap(dtype, low, high):

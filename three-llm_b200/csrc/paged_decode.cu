@@ -35,8 +35,9 @@
 // prepared or survives the call.
 //
 // float32 activations over float16 pages: each query row is scaled by a power
-// of two and split into two float16 parts, and so is each weight; with both
-// parts multiplied the products carry 22 bits, and the output keeps float32's
+// of two and split into two float16 parts, and so is each weight. With both
+// parts multiplied a weight keeps 22 bits down to 2^-17 of the largest and
+// below that 2^-39 of the largest (see kLiftOf), and the output keeps float32's
 // use for its caller. K and V are exact as stored.
 #include <cooperative_groups.h>
 #include <math.h>
@@ -267,6 +268,17 @@ __device__ __forceinline__ void store_out(const DecodeParams& d, int64_t i, floa
   static_cast<IO*>(d.out)[i] = from_f32<IO>(v);
 }
 
+// Weights are formed as powers of two over a base that lies this far below the
+// running maximum, the largest being 2^14: float16 keeps a weight's 11 bits down
+// to 2^-28 of the largest, and rounds by 2^-39 of it at most below, where
+// weights of up to 1 would be cut to ever fewer bits from 2^-14 on and vanish
+// under 2^-25 (8192 of them together were lost or a third too heavy). The sum
+// and the output carry the same factor. The base is rounded upwards, so that no
+// weight passes 2^14 where scores are so large that a float's step is (there the
+// base is the maximum itself). bfloat16 has float32's exponents.
+template <typename CT>
+constexpr float kLiftOf = std::is_same<CT, __half>::value ? 14.f : 0.f;
+
 // SPLIT: float32 activations over float16 pages. TWO: more than 8 query heads per group.
 template <int D, typename CT, bool SPLIT, bool TWO>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(const __grid_constant__ DecodeParams d) {
@@ -461,6 +473,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   CT* q_s = reinterpret_cast<CT*>(smem + L.q);
   float* red = reinterpret_cast<float*>(smem + L.red);
   constexpr int kNt = TWO ? 2 : 1;  // column tiles of 8 query heads
+  constexpr float kLift = kLiftOf<CT>;
   constexpr int kGroups = C::kGroups;
   const int g8 = lane >> 2, t4 = lane & 3;
   const int frag_row = (lane & 7) + ((lane >> 3) & 1) * 8;   // K as the left operand: token rows, then dimensions
@@ -531,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       }
     }
 
-    // this thread's columns: heads nt * 8 + 2 * t4 + e
+    // this thread's columns: heads nt * 8 + 2 * t4 + e; m is the weights' base
     float o[kNt][D / 16][4], m[kNt][2], l[kNt][2];
 #pragma unroll
     for (int nt = 0; nt < kNt; ++nt) {
@@ -606,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
             top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 4));
             top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 8));
             top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 16));
-            top[e] = fmaxf(top[e], m[nt][e]);
+            top[e] = fmaxf(kLift > 0.f ? __fsub_ru(top[e], kLift) : top[e], m[nt][e]);
             base[e] = top[e] == -INFINITY ? 0.f : top[e];
             keep[e] = ex2(m[nt][e] - base[e]);
             m[nt][e] = top[e];
