@@ -948,39 +948,25 @@ cudaError_t configure_t(int rows, int max_batch, int* most) {
   if (e != cudaSuccess) return e;
   return large_cluster(k, kThreads, smem_layout<D>(rows, 0, SPLIT).total, most);
 }
-template <int D>
-cudaError_t configure_d(const tla_paged* P, int rows, int* most) {
-  const bool two = rows > 8;
-  const int max_batch = P->base.max_batch;
-  if constexpr (D == 256) {  // (groups of at most 8 heads: two column tiles of O would not fit the registers)
-    if (P->io == kFp32) return configure_t<D, __half, true, false>(rows, max_batch, most);
-    if (P->kept == kBf16) return configure_t<D, __nv_bfloat16, false, false>(rows, max_batch, most);
-    return configure_t<D, __half, false, false>(rows, max_batch, most);
-  }
-  if (P->io == kFp32)
-    return two ? configure_t<D, __half, true, true>(rows, max_batch, most)
-               : configure_t<D, __half, true, false>(rows, max_batch, most);
-  if (P->kept == kBf16)
-    return two ? configure_t<D, __nv_bfloat16, false, true>(rows, max_batch, most)
-               : configure_t<D, __nv_bfloat16, false, false>(rows, max_batch, most);
-  return two ? configure_t<D, __half, false, true>(rows, max_batch, most)
-             : configure_t<D, __half, false, false>(rows, max_batch, most);
-}
-
-template <int D>
-cudaError_t launch_d(const tla_paged* P, DecodeParams& d, cudaStream_t stream) {
-  const bool two = d.rows > 8;
-  if constexpr (D == 256) {
-    if (P->io == kFp32) return launch_t<D, __half, true, false>(P, d, stream);
-    if (P->kept == kBf16) return launch_t<D, __nv_bfloat16, false, false>(P, d, stream);
-    return launch_t<D, __half, false, false>(P, d, stream);
-  }
-  if (P->io == kFp32)
-    return two ? launch_t<D, __half, true, true>(P, d, stream) : launch_t<D, __half, true, false>(P, d, stream);
-  if (P->kept == kBf16)
-    return two ? launch_t<D, __nv_bfloat16, false, true>(P, d, stream)
-               : launch_t<D, __nv_bfloat16, false, false>(P, d, stream);
-  return two ? launch_t<D, __half, false, true>(P, d, stream) : launch_t<D, __half, false, false>(P, d, stream);
+// f(an instance of the kernel) for the layer's types and `rows` query heads per
+// group (256 wide there are groups of at most 8: two column tiles of O would not
+// fit the registers).
+template <typename CT, bool SPLIT, bool TWO>
+struct Instance {
+  using Type = CT;
+  static constexpr bool kSplit = SPLIT, kTwo = TWO;
+};
+template <int D, typename F>
+cudaError_t by_instance(const tla_paged* P, int rows, F f) {
+  if constexpr (D < 256)
+    if (rows > 8) {
+      if (P->io == kFp32) return f(Instance<__half, true, true>());
+      if (P->kept == kBf16) return f(Instance<__nv_bfloat16, false, true>());
+      return f(Instance<__half, false, true>());
+    }
+  if (P->io == kFp32) return f(Instance<__half, true, false>());
+  if (P->kept == kBf16) return f(Instance<__nv_bfloat16, false, false>());
+  return f(Instance<__half, false, false>());
 }
 
 int subgroups(const tla_paged* P) {
@@ -1002,7 +988,14 @@ cudaError_t paged_decode_configure(tla_paged* P) {
   P->fast = P->wide && P->kept != kFp32 && (P->io != kFp32 || P->kept == kFp16) && P->pool.page_size >= 16 &&
             kCtasPerSm * P->base.ctx->sm_count <= kMaxGrid;
   if (!P->fast) return cudaSuccess;
-  return by_width(P, [&](auto w) { return configure_d<decltype(w)::value>(P, subgroup_rows(P), &P->decode_cluster); });
+  const int rows = subgroup_rows(P);
+  return by_width(P, [&](auto w) {
+    constexpr int D = decltype(w)::value;
+    return by_instance<D>(P, rows, [&](auto i) {
+      using I = decltype(i);
+      return configure_t<D, typename I::Type, I::kSplit, I::kTwo>(rows, P->base.max_batch, &P->decode_cluster);
+    });
+  });
 }
 
 // The most tiles that a pair of this call can have.
@@ -1068,7 +1061,13 @@ cudaError_t launch_paged_decode(const tla_paged* P, const PagedArgs& p, const vo
   d.rows = subgroup_rows(P);
   d.small_grid = 0;
   d.cluster = cluster_size(P, p, count);
-  return by_width(P, [&](auto w) { return launch_d<decltype(w)::value>(P, d, stream); });
+  return by_width(P, [&](auto w) {
+    constexpr int D = decltype(w)::value;
+    return by_instance<D>(P, d.rows, [&](auto i) {
+      using I = decltype(i);
+      return launch_t<D, typename I::Type, I::kSplit, I::kTwo>(P, d, stream);
+    });
+  });
 }
 
 }  // namespace tla
