@@ -168,3 +168,17 @@ def test_decode_gives_a_constant_back(pkg, cuda, io, kept, wide, low):
     # float32: weights in two parts against their 32-bit sum, and at most 40 additions of either, 2^-23 each; the
     # 16-bit types have the constant's neighbours further off than that
     assert (out - c).abs().max() <= (2.0 ** -17 * c if io == "fp32" else 0.0)
+
+
+# ---------------------------------------------------------------- gates, alignment, empty calls
+@pytest.mark.parametrize("d,io,kept,page", [(64, "fp32", "fp32", 16), (128, "fp32", "bf16", 16), (64, "fp16", "fp16", 4),
+                                            (100, "fp16", "fp16", 16), (256, "fp32", "fp16", 16)])
+@pytest.mark.parametrize("wide", [1, WIDE])
+def test_decode_gate_as_output_everywhere(pkg, cuda, d, io, kept, page, wide):
+    """The gate's own memory as the output, for the kernels that join many shares and those that do not."""
+    w = World([700, 40, 0], 2, d, page, kept, extra_width=wide)
+    layer, *_ = make(pkg, cuda, w, 8, 2, d, io)
+    q, gate = (w.normal(3, 8 * d, dtype=TYPES[io]).to(cuda) for _ in range(2))
+    pos, table = ints([699, 39, -1], cuda), w.device_table(cuda)
+    exp = layer.decode(q, pos, table, gate=gate)
+    assert torch.equal(layer.decode(q, pos, table, gate=gate, out=gate), exp)

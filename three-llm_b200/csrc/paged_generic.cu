@@ -39,6 +39,7 @@ int shares_of(const tla_paged* P, int batch) {
   return static_cast<int>(n < 1 ? 1 : n > kMaxShares ? kMaxShares : n);
 }
 
+// (gate and out may be the same memory: neither is declared __restrict__ in this file.)
 template <typename IO>
 __device__ __forceinline__ void store_out(IO* out, const IO* gate, int64_t i, float v) {
   if (gate) v = v * (1.f / (1.f + expf(-to_f32(gate[i]))));  // math.ts:271-273
@@ -49,7 +50,7 @@ __device__ __forceinline__ void store_out(IO* out, const IO* gate, int64_t i, fl
 // workspace, or where one block has all the tokens to the call's output.
 template <typename IO>
 __device__ __forceinline__ void join_warps(const float* red, int D, int heads, int64_t first_row, int share, int shares,
-                                           const IO* __restrict__ gate, IO* __restrict__ out,
+                                           const IO* gate, IO* out,
                                            float* __restrict__ partial) {
   for (int i = threadIdx.x; i < heads * D; i += kThreads) {
     const int h = i / D, d = i - h * D;
@@ -81,7 +82,7 @@ __device__ __forceinline__ void join_warps(const float* red, int D, int heads, i
 template <typename IO, typename CT>
 __global__ void __launch_bounds__(kThreads)
     paged_attend_kernel(PagedArgs p, const IO* __restrict__ query, const int32_t* __restrict__ pages, int count,
-                        const IO* __restrict__ gate, IO* __restrict__ out, float* __restrict__ partial) {
+                        const IO* gate, IO* out, float* __restrict__ partial) {
   extern __shared__ float red[];  // [kWarps][kHeads][D + 2]
   griddep_wait();
   griddep_launch_dependents();
@@ -222,7 +223,7 @@ constexpr int kStages = 4;
 template <typename IO, typename CT, int LANES>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
     paged_rows_kernel(PagedArgs p, const IO* __restrict__ query, const int32_t* __restrict__ pages, int count,
-                      const IO* __restrict__ gate, IO* __restrict__ out, float* __restrict__ partial) {
+                      const IO* gate, IO* out, float* __restrict__ partial) {
   constexpr int kPiece = 16 / sizeof(CT), kPieces = 16 / kPiece, kTokens = 32 / LANES, kStep = kWarps * kTokens;
   extern __shared__ float4 ring[];  // [kWarps][kStages][K, V][kPieces][32], then the warps' triples
   float* red = reinterpret_cast<float*>(ring);
@@ -428,8 +429,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 // Joins the shares' triples; a block per output row.
 template <typename IO>
 __global__ void __launch_bounds__(kThreads)
-    paged_join_kernel(const float* __restrict__ partial, int shares, int D, const IO* __restrict__ gate,
-                      IO* __restrict__ out) {
+    paged_join_kernel(const float* __restrict__ partial, int shares, int D, const IO* gate,
+                      IO* out) {
   griddep_wait();
   griddep_launch_dependents();
   const int64_t row = blockIdx.x;
