@@ -342,7 +342,9 @@ int tla_decode_noalloc(const tla_attn_config* config, void* key_cache, void* val
  * time on several streams as long as no call writes what another reads (give
  * each its own workspace), and all may be captured in CUDA graphs, which the
  * layer and the pool must outlive. Outputs may not overlap inputs (a gate may
- * be the output itself). */
+ * be the output itself). qkv, query, gate and outputs start on 16-byte
+ * boundaries where head_dim is a multiple of 8 (as every row of a dense tensor
+ * then does), else on their elements'. */
 typedef struct tla_page_pool {
   void* key;               /* device; element (page, kv_head, slot, d) at key + page*page_stride + */
   void* value;             /* kv_head*head_stride + slot*slot_stride + d, strides in elements      */

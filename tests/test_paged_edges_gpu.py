@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from tests import paged_ref as ref
-from tests.test_paged_gpu import TYPES, WIDE, World, close, ints, make
+from tests.test_paged_gpu import PAIRS, TYPES, WIDE, World, close, ints, make
 
 pytestmark = pytest.mark.gpu
 
@@ -182,3 +182,43 @@ def test_decode_gate_as_output_everywhere(pkg, cuda, d, io, kept, page, wide):
     pos, table = ints([699, 39, -1], cuda), w.device_table(cuda)
     exp = layer.decode(q, pos, table, gate=gate)
     assert torch.equal(layer.decode(q, pos, table, gate=gate, out=gate), exp)
+
+
+@pytest.mark.parametrize("io,kept", PAIRS)
+def test_rows_off_the_16_byte_boundaries(pkg, cuda, io, kept):
+    """A head_dim that is no multiple of 8: any row of a tensor may be the first one."""
+    d, page = 101, 8
+    w = World([30, 77], 1, d, page, kept, room=1)
+    layer, k, v, bd = make(pkg, cuda, w, 1, 1, d, io, rotaryDim=0)
+    q, gate, qkv = (w.normal(3, n * d, dtype=TYPES[io]).to(cuda) for n in (1, 1, 3))
+    pos, table = ints([29, 76], cuda), w.device_table(cuda)
+    out = torch.full((3, d), 7.0, dtype=TYPES[io], device=cuda)
+    layer.decode(q[1:], pos, table, gate=gate[1:], out=out[1:])
+    assert torch.equal(out[1:], layer.decode(q[1:].clone(), pos, table, gate=gate[1:].clone()))
+    assert (out[0] == 7).all()
+    assert torch.equal(layer.select(q[1:], pos, table, 3), layer.select(q[1:].clone(), pos, table, 3))
+    query = torch.full((3, d), 7.0, dtype=TYPES[io], device=cuda)
+    layer.append(qkv[1:], pos + 1, table, query=query[1:])
+    assert layer.context.error() == 0
+    assert torch.equal(query[1:], qkv[1:, :d]) and (query[0] == 7).all()
+    for b, n in enumerate((30, 77)):
+        at = w.table[b][n // page], 0, n % page
+        assert torch.equal(k[at], qkv[1 + b, d:2 * d].to(w.kept)) and torch.equal(v[at], qkv[1 + b, 2 * d:].to(w.kept))
+
+
+def test_unaligned_addresses_of_vector_kernels_are_refused(pkg, cuda):
+    w = World([30], 1, 64, 16, "fp16")
+    layer, *_ = make(pkg, cuda, w, 1, 1, 64, "fp16")
+    buf = torch.zeros(1024, dtype=torch.float16, device=cuda)
+    pos, table, row = ints([29], cuda), w.device_table(cuda), torch.zeros(1, 64, dtype=torch.float16, device=cuda)
+    off, whole = buf[4:68].view(1, 64), buf[4:196].view(1, 192)
+    for call in (lambda: layer.decode(off, pos, table), lambda: layer.decode(row, pos, table, out=off),
+                 lambda: layer.decode(row, pos, table, gate=off), lambda: layer.append(whole, pos, table),
+                 lambda: layer.select(off, pos, table, 2),
+                 lambda: layer.append(buf[:192].view(1, 192), pos, table, query=buf[260:324].view(1, 64))):
+        with pytest.raises(pkg.TlaError, match="INVALID_ARG"):
+            call()
+    # half an element, through the C ABI
+    odd = make(pkg, cuda, World([30], 1, 101, 16, "fp16"), 1, 1, 101, "fp16", rotaryDim=0)[0]
+    assert pkg.lib().tla_paged_decode(odd.handle, buf.data_ptr() + 1, pos.data_ptr(), table.data_ptr(), w.width, None, 0,
+                                      None, buf.data_ptr() + 512, 1, None, 0, None) == -1

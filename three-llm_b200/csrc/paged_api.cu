@@ -50,6 +50,14 @@ int check_call(const tla_paged* P, const void* positions, const void* table, int
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Whether rows of activations may start there: on 16 bytes where head_dim is a
+// multiple of 8 (the kernels then read and write several elements at a time;
+// every row of a dense tensor does), else on an element.
+bool row_start(const tla_paged* P, const void* p) {
+  const int step = P->base.D % 8 == 0 ? 16 : P->io == tla::kFp32 ? 4 : 2;
+  return reinterpret_cast<uintptr_t>(p) % step == 0;
+}
+
 // Whether every (page, head, slot) row of D elements has memory of its own:
 // sorted by stride, each dimension must step over all that the smaller span.
 bool rows_apart(const tla_page_pool& pool, int heads, int D) {
@@ -172,7 +180,7 @@ int tla_paged_append(tla_paged* P, const void* qkv, const int32_t* positions, co
   if (rc != TLA_OK) return rc;
   if (rows < 0 || (rows > 0 && !qkv) || (!row_offsets && rows != batch)) return TLA_ERR_INVALID_ARG;
   if (batch == 0 || rows == 0) return TLA_OK;
-  if (!aligned16(qkv) || !aligned16(query_out) ||
+  if (!row_start(P, qkv) || !row_start(P, query_out) ||
       overlap(qkv, rows * row_bytes(P, P->base.Hq + 2 * P->base.Hk), query_out, rows * row_bytes(P, P->base.Hq)))
     return TLA_ERR_INVALID_ARG;
   if (!tla::paged_append_takes(P)) return TLA_ERR_UNSUPPORTED;
@@ -198,7 +206,7 @@ int tla_paged_decode(tla_paged* P, const void* query, const int32_t* positions, 
   if (pages ? page_count <= 0 : page_count != 0) return TLA_ERR_INVALID_ARG;
   if (batch == 0) return TLA_OK;
   const size_t bytes = batch * row_bytes(P, P->base.Hq);
-  if (!query || !out || !aligned16(query) || !aligned16(out) || !aligned16(gate) || !aligned16(workspace) ||
+  if (!query || !out || !row_start(P, query) || !row_start(P, out) || !row_start(P, gate) || !aligned16(workspace) ||
       overlap(query, bytes, out, bytes) || (gate != out && overlap(gate, bytes, out, bytes)))
     return TLA_ERR_INVALID_ARG;
   const tla::PagedArgs p = tla::paged_args(P, positions, page_table, table_width, batch);
@@ -222,7 +230,7 @@ int tla_paged_select(tla_paged* P, const void* query, const int32_t* positions, 
     return TLA_ERR_INVALID_ARG;
   if (!P->pool.bounds || !(P->base.attn_scale > 0)) return TLA_ERR_UNSUPPORTED;
   if (batch == 0) return TLA_OK;
-  if (!query || !pages_out || !aligned16(query) || !aligned16(workspace) ||
+  if (!query || !pages_out || !row_start(P, query) || !aligned16(workspace) ||
       overlap(query, batch * row_bytes(P, P->base.Hq), pages_out,
               static_cast<size_t>(batch) * P->base.Hk * page_count * sizeof(int32_t)))
     return TLA_ERR_INVALID_ARG;
