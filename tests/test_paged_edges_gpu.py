@@ -222,3 +222,13 @@ def test_unaligned_addresses_of_vector_kernels_are_refused(pkg, cuda):
     odd = make(pkg, cuda, World([30], 1, 101, 16, "fp16"), 1, 1, 101, "fp16", rotaryDim=0)[0]
     assert pkg.lib().tla_paged_decode(odd.handle, buf.data_ptr() + 1, pos.data_ptr(), table.data_ptr(), w.width, None, 0,
                                       None, buf.data_ptr() + 512, 1, None, 0, None) == -1
+
+
+def test_an_empty_batch_with_a_page_list(pkg, cuda):
+    """No sequences: nothing to do, with or without lists."""
+    layer = make(pkg, cuda, World([30], 2, 64, 16, "fp16"), 8, 2, 64, "fp16")[0]
+    q, none = torch.zeros(0, 512, dtype=torch.float16, device=cuda), ints([], cuda)
+    table = torch.zeros(0, 3, dtype=torch.int32, device=cuda)
+    pages = layer.select(q, none, table, 5)
+    assert pages.shape == (0, 2, 5)
+    assert layer.decode(q, none, table, pages=pages).shape == (0, 512)

@@ -203,8 +203,8 @@ int tla_paged_decode(tla_paged* P, const void* query, const int32_t* positions, 
                      int32_t batch, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_call(P, positions, page_table, table_width, batch);
   if (rc != TLA_OK) return rc;
+  if (batch == 0) return page_count < 0 ? TLA_ERR_INVALID_ARG : TLA_OK;  // (an empty list's address may be null)
   if (pages ? page_count <= 0 : page_count != 0) return TLA_ERR_INVALID_ARG;
-  if (batch == 0) return TLA_OK;
   const size_t bytes = batch * row_bytes(P, P->base.Hq);
   if (!query || !out || !row_start(P, query) || !row_start(P, out) || !row_start(P, gate) || !aligned16(workspace) ||
       overlap(query, bytes, out, bytes) || (gate != out && overlap(gate, bytes, out, bytes)))
