@@ -2,6 +2,7 @@
 limit or an address goes wrong. Worlds and 64-bit forms are those of
 test_paged_gpu.py and paged_ref.py."""
 import math
+import os
 import subprocess
 import sys
 from pathlib import Path
@@ -232,3 +233,53 @@ def test_an_empty_batch_with_a_page_list(pkg, cuda):
     pages = layer.select(q, none, table, 5)
     assert pages.shape == (0, 2, 5)
     assert layer.decode(q, none, table, pages=pages).shape == (0, 512)
+
+
+# ---------------------------------------------------------------- append: offsets out of order, inside guarded buffers
+@pytest.mark.parametrize("d,io,kept", [(64, "fp16", "fp16"), (128, "fp32", "bf16"), (100, "fp16", "fp16"), (256, "fp32", "fp32")])
+@pytest.mark.parametrize("bounded", [True, False])
+@pytest.mark.parametrize("offsets", [[0, 30, 5, 20], [5, 3, 1, 0], [0, 0, 0, 1 << 30], [-(1 << 31), 4, 9, 20],
+                                     [-5, -3, 2, 18], [20, 20, 20, 20], [0, 20, 0, 20], [(1 << 31) - 1, 0, -(1 << 31), 7]])
+def test_append_offsets_out_of_order_touch_nothing_else(pkg, cuda, d, io, kept, bounded, offsets):
+    """Rows may move or be lost, but what surrounds the rows is neither read nor written, nor is any page that the
+    table does not name."""
+    w = World([0, 0, 0], 2, d, 16, kept, room=32)
+    guard = 4096
+
+    def inside(shape, dtype, fill):
+        n = math.prod(shape)
+        whole = torch.full((n + 2 * guard,), fill, dtype=dtype, device=cuda)
+        return whole, whole[guard:guard + n].view(shape)
+
+    pages = w.keys.shape[0]
+    kw, k = inside((pages, 2, 16, d), w.kept, 3.0)
+    vw, v = inside((pages, 2, 16, d), w.kept, 3.0)
+    bw, bd = inside((pages, 2, 2, d), w.kept, 3.0)
+    xw, x = inside((20, 8 * d), TYPES[io], float("nan"))
+    qw, query = inside((20, 4 * d), TYPES[io], 3.0)
+    x.copy_(w.normal(20, 8 * d, dtype=TYPES[io]).clamp(-2, 2))
+    layer = pkg.PagedAttention(4 * d, 4, w.width * 16, k, v, {"headDim": d, "kvHeadCount": 2, "dtype": TYPES[io]},
+                               key_bounds=bd if bounded else None)
+    layer.append(x, ints([0, 7, 16], cuda), w.device_table(cuda), row_offsets=ints(offsets, cuda), query=query)
+    assert layer.context.error() != -17
+    named = sorted({p for row in w.table for p in row if p >= 0})
+    spare = [p for p in range(pages) if p not in named]
+    for whole, inner in ((kw, k), (vw, v), (bw, bd), (qw, query)):
+        assert (whole[:guard] == 3).all() and (whole[-guard:] == 3).all()
+        assert inner.isfinite().all()  # (a row from outside would be NaN)
+    for t in (k, v, bd):
+        assert (t[spare] == 3).all()
+    if not bounded:
+        assert (bw == 3).all()
+
+
+def test_edges_under_bounds_check_build(pkg):
+    """These tests in a fresh process that loads libtla_check.so: no guarded index may leave its buffer."""
+    if os.environ.get("TLA_LIBRARY"):
+        pytest.skip("runs in that process")
+    subprocess.run(["make", "-s", "-j8", "-C", str(ROOT / "three-llm_b200" / "csrc"), "check"], check=True)
+    env = dict(os.environ, TLA_LIBRARY=str(ROOT / "three-llm_b200" / "libtla_check.so"))
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "-p", "no:cacheprovider", "-m", "gpu",
+                        "tests/test_paged_edges_gpu.py"], cwd=ROOT, env=env, capture_output=True, text=True, timeout=900)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-2000:]
+    assert " passed" in r.stdout

@@ -15,6 +15,12 @@ __device__ __forceinline__ int64_t pool_row(const PagedArgs& p, int page, int kv
   return page * p.page_stride + kvh * p.head_stride + slot * p.slot_stride;
 }
 
+// First element of a (page, kv head)'s bounds: [low, high][D].
+__device__ __forceinline__ int64_t bounds_row(const PagedArgs& p, int page, int kvh, int D) {
+  if (!TLA_IN_BOUNDS(page, p.page_count, p.a.error) || !TLA_IN_BOUNDS(kvh, p.a.Hk, p.a.error)) return 0;
+  return (static_cast<int64_t>(page) * p.a.Hk + kvh) * 2 * D;
+}
+
 // The page that holds logical page `index` of sequence b, or -1 (reported)
 // when the table's entry is not a page of the pool. index < p.width.
 __device__ __forceinline__ int pool_page(const PagedArgs& p, int b, int index) {

@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads)
       const CT k = from_f32<CT>(val);
       key[pool_row(p, page, h - Hq, slot) + d] = k;
       if (bounds && !offsets) {  // one new token: its page's bounds right here
-        CT* low = bounds + (static_cast<int64_t>(page) * Hk + (h - Hq)) * 2 * D + d;
+        CT* low = bounds + bounds_row(p, page, h - Hq, D) + d;
         low[0] = slot == 0 ? k : low_of(low[0], k);
         low[D] = slot == 0 ? k : high_of(low[D], k);
       }
@@ -388,7 +388,7 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
             store4(at + d1, y);
           }
           if (kKind == 1 && p.bounds && !offsets) {  // one new token: its page's bounds right here
-            CT* low = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + kvh) * 2 * hd;
+            CT* low = static_cast<CT*>(p.bounds) + bounds_row(p, page, kvh, hd);
             CT* high = low + hd;
             const Raw4<CT> k0 = pack4<CT>(x), k1 = pack4<CT>(y);
             put4(low + d0, slot == 0 ? k0 : low4<CT>(raw4(low + d0), k0));
@@ -530,8 +530,9 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
 #pragma unroll
       for (int k = 0; k < kLoads; ++k) {
         const int s = s1 + k * shares * kPer;
-        lo[k] = on && s < slots ? raw4(in + static_cast<int64_t>(s) * row_size + d0) : Raw4<IO>{};
-        hi[k] = on && s < slots ? raw4(in + static_cast<int64_t>(s) * row_size + d1) : Raw4<IO>{};
+        const bool held = on && s < slots && TLA_IN_BOUNDS(row0 + s0 + s, rows, a.error);
+        lo[k] = held ? raw4(in + static_cast<int64_t>(s) * row_size + d0) : Raw4<IO>{};
+        hi[k] = held ? raw4(in + static_cast<int64_t>(s) * row_size + d1) : Raw4<IO>{};
       }
 #pragma unroll
       for (int k = 0; k < kLoads; ++k) {
@@ -598,7 +599,7 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
       const float u = join_s[h + k * heads][is_low ? 0 : 1][e];
       v = (is_low ? u < v : u > v) ? u : v;
     }
-    CT* to = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + head) * 2 * hd + at;
+    CT* to = static_cast<CT*>(p.bounds) + bounds_row(p, page, head, hd) + at;
     if (begin > 0) {
       const float u = to_f32(to[0]);
       v = (is_low ? v < u : v > u) ? v : u;
@@ -656,7 +657,7 @@ __global__ void __launch_bounds__(kThreads)
   const CT* key = static_cast<const CT*>(p.key);
   for (int i = threadIdx.x; i < Hk * D; i += kThreads) {
     const int h = i / D, d = i - h * D;
-    CT* at = static_cast<CT*>(p.bounds) + (static_cast<int64_t>(page) * Hk + h) * 2 * D + d;
+    CT* at = static_cast<CT*>(p.bounds) + bounds_row(p, page, h, D) + d;
     const CT* k = key + pool_row(p, page, h, slot) + d;
     CT low = k[0], high = k[0];
     for (int s = 1; s < n; ++s) {
