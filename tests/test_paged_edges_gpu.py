@@ -10,6 +10,7 @@ from pathlib import Path
 import pytest
 import torch
 
+from oracle import oracle
 from tests import paged_ref as ref
 from tests.test_paged_gpu import PAIRS, TYPES, WIDE, World, close, ints, make
 
@@ -169,6 +170,69 @@ def test_decode_gives_a_constant_back(pkg, cuda, io, kept, wide, low):
     # float32: weights in two parts against their 32-bit sum, and at most 40 additions of either, 2^-23 each; the
     # 16-bit types have the constant's neighbours further off than that
     assert (out - c).abs().max() <= (2.0 ** -17 * c if io == "fp32" else 0.0)
+
+
+# ---------------------------------------------------------------- append: scaled and partial rotations
+YARN = {"type": "yarn", "factor": 4.0, "original_context_length": 256.0, "beta_fast": 32.0, "beta_slow": 1.0}
+ROTATIONS = [
+    {"ropeScaling": YARN},
+    {"ropeScaling": {**YARN, "attention_factor": 0.625}, "rotaryDim": 32},
+    {"ropeScaling": {"type": "linear", "factor": 3.0}, "ropePairCount": 5},
+    {"ropeScaling": {"type": "llama3", "factor": 8.0, "original_context_length": 64.0, "low_freq_factor": 1.0,
+                     "high_freq_factor": 4.0}},
+    {"ropeScaling": YARN, "ropePairCount": 9, "rotaryDim": 48},
+    {"ropePairCount": 0},
+    {"ropeFreqDim": 128, "rotaryDim": 40},
+    {"ropeScaling": YARN, "ropeFreqDim": 512, "ropePairCount": 13, "norms": True},
+]
+
+
+@pytest.mark.parametrize("options", ROTATIONS, ids=lambda o: "-".join(sorted(o)))
+@pytest.mark.parametrize("form", ["one", "chunks", "chunks without bounds"])
+@pytest.mark.parametrize("d,io,kept", [(64, "fp16", "fp16"), (128, "bf16", "bf16"), (96, "fp32", "fp16"),
+                                       (256, "fp32", "fp32"), (100, "fp32", "fp32"), (64, "fp32", "bf16")])
+def test_append_scaled_and_partial_rotations(pkg, cuda, options, form, d, io, kept):
+    """Every form of the append (block per row, rows, pages) turns the pairs below ropePairCount by the scaled
+    frequencies, times the attention factor, and leaves the rest as it is."""
+    o, hq, hk, page, theta = dict(options), 5, 5, 16, 10000.0
+    norm = o.pop("norms", False)
+    g = torch.Generator().manual_seed(1)
+    qn, kn = (torch.randn(d, generator=g).mul(0.3).add(1) for _ in range(2))
+    if norm:
+        o["qNormWeight"], o["kNormWeight"] = qn.numpy(), kn.numpy()
+    starts, chunks = [0, 17, 300], [1, 1, 1] if form == "one" else [40, 1, 33]
+    w = World(starts, hk, d, page, kept, room=max(chunks))
+    layer, k, v, bd = make(pkg, cuda, w, hq, hk, d, io, bounds=form != "chunks without bounds", ropeTheta=theta, **o)
+    qkv = w.normal(sum(chunks), (hq + 2 * hk) * d, dtype=TYPES[io])
+    offsets = None if form == "one" else ints([0, 40, 41, 74], cuda)
+    query = layer.append(qkv.to(cuda), ints(starts, cuda), w.device_table(cuda), row_offsets=offsets).cpu()
+    assert layer.context.error() == 0
+    rotary = o.get("rotaryDim", d)
+    inv, factor = oracle.rope_parameters(o.get("ropeFreqDim", rotary), theta, o.get("ropeScaling"))
+    pairs = min(rotary // 2, o.get("ropePairCount", rotary // 2))
+    turn = torch.as_tensor(inv[:pairs]).double()
+
+    def rotated(x, pos):
+        a, b = x[..., :pairs], x[..., rotary // 2:rotary // 2 + pairs]
+        cos, sin = (pos * turn).cos(), (pos * turn).sin()
+        y = x.clone()
+        y[..., :pairs] = (a * cos - b * sin) * factor
+        y[..., rotary // 2:rotary // 2 + pairs] = (b * cos + a * sin) * factor
+        return y
+
+    got_k, got_v, at = k.cpu(), v.cpu(), 0
+    for b, n in enumerate(chunks):
+        for i in range(n):
+            x, pos = qkv[at].double().view(hq + 2 * hk, d), starts[b] + i
+            q, kk = x[:hq], x[hq:hq + hk]
+            if norm:
+                q, kk = ref.rms(q, qn, 1e-6, False), ref.rms(kk, kn, 1e-6, False)
+            q, kk = rotated(q, pos), rotated(kk, pos)
+            p, slot = w.table[b][pos // page], pos % page
+            close(query[at], q, ref.row_error(q, TYPES[io], d), f"query of sequence {b}, token {i}")
+            close(got_k[p, :, slot], kk, ref.row_error(kk, w.kept, d), f"key of sequence {b}, token {i}")
+            assert torch.equal(got_v[p, :, slot], x[hq + hk:].to(w.kept))
+            at += 1
 
 
 # ---------------------------------------------------------------- gates, alignment, empty calls
