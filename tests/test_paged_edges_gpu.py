@@ -249,6 +249,28 @@ def test_decode_gate_as_output_everywhere(pkg, cuda, d, io, kept, page, wide):
     assert torch.equal(layer.decode(q, pos, table, gate=gate, out=gate), exp)
 
 
+@pytest.mark.parametrize("d,io,kept,page", [(64, "fp16", "fp16", 16), (128, "bf16", "bf16", 16), (64, "fp32", "fp16", 32),
+                                            (64, "fp32", "fp32", 16), (128, "fp32", "bf16", 16), (64, "fp16", "fp16", 4),
+                                            (100, "fp16", "fp16", 16), (256, "fp32", "fp16", 16)])
+@pytest.mark.parametrize("wide", [1, WIDE])
+@pytest.mark.parametrize("held", [0.0, float("inf"), float("-inf"), float("nan")])
+def test_decode_zeros_whatever_the_gate_holds(pkg, cuda, d, io, kept, page, wide, held):
+    """Rows with nothing to attend to (no sequence, a position past the capacity, an empty list, no page that is in
+    the pool) are zeros also where the gate has no number."""
+    w = World([700, 0, 40, 40], 2, d, page, kept, extra_width=wide)
+    layer, *_ = make(pkg, cuda, w, 8, 2, d, io)
+    q, gate = (w.normal(4, 8 * d, dtype=TYPES[io]).to(cuda) for _ in range(2))
+    gate[1:] = held
+    table = w.device_table(cuda)
+    table[3] = -7
+    out = layer.decode(q, ints([699, -1, w.width * page, 39], cuda), table, gate=gate)
+    assert not out[1:].any() and out[0].isfinite().all() and out[0].any()
+    pages = ints([[[0, 1], [1, -1]]] + [[[-1, -1], [-1, -1]]] * 3, cuda)
+    out = layer.decode(q, ints([699, -1, 39, 39], cuda), w.device_table(cuda), pages=pages, gate=gate)
+    assert not out[1:].any() and out[0].isfinite().all() and out[0].any()
+    layer.context.error()
+
+
 @pytest.mark.parametrize("io,kept", PAIRS)
 def test_rows_off_the_16_byte_boundaries(pkg, cuda, io, kept):
     """A head_dim that is no multiple of 8: any row of a tensor may be the first one."""

@@ -262,9 +262,12 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
+// An output acc / sum times its gate; zero, whatever the gate holds, where no
+// token took part.
 template <typename IO>
-__device__ __forceinline__ void store_out(const DecodeParams& d, int64_t i, float v) {
-  if (d.gate) v = v * (1.f / (1.f + expf(-to_f32(static_cast<const IO*>(d.gate)[i]))));  // math.ts:271-273
+__device__ __forceinline__ void store_out(const DecodeParams& d, int64_t i, float acc, float sum) {
+  float v = sum != 0.f ? acc * (1.f / sum) : 0.f;
+  if (d.gate && sum != 0.f) v = v * (1.f / (1.f + expf(-to_f32(static_cast<const IO*>(d.gate)[i]))));  // math.ts:271-273
   static_cast<IO*>(d.out)[i] = from_f32<IO>(v);
 }
 
@@ -726,9 +729,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         v1 += x.y * f;
       }
       if (whole) {
-        const float inv = sum != 0.f ? 1.f / sum : 0.f;
-        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c, v0 * inv);
-        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c + 1, v1 * inv);
+        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c, v0, sum);
+        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c + 1, v1, sum);
       } else if (d.cluster ||
                  TLA_IN_BOUNDS(mine - d.scratch + (r + 1) * (D + 2) - 1, d.scratch_floats, p.a.error)) {
         *reinterpret_cast<float2*>(mine + r * (D + 2) + 2 + c) = make_float2(v0, v1);
@@ -771,9 +773,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         v0 += x[k].x * f;
         v1 += x[k].y * f;
       }
-      const float inv = sum != 0.f ? 1.f / sum : 0.f;
-      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c, v0 * inv);
-      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c + 1, v1 * inv);
+      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c, v0, sum);
+      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c + 1, v1, sum);
     }
     cluster.sync();  // the others may still read this CTA's triple
   }
@@ -867,7 +868,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
       if (lane + 32 * e < p.a.D)
-        store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + lane + 32 * e, sum != 0.f ? acc[e] / sum : 0.f);
+        store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + lane + 32 * e, acc[e], sum);
     return;
   }
   if (lane == 0) {
@@ -889,7 +890,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
       all += red[1][w] * f;
       v += row_s[w][c] * f;
     }
-    store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + c, all != 0.f ? v / all : 0.f);
+    store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + c, v, all);
   }
 }
 

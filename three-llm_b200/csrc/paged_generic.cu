@@ -39,10 +39,13 @@ int shares_of(const tla_paged* P, int batch) {
   return static_cast<int>(n < 1 ? 1 : n > kMaxShares ? kMaxShares : n);
 }
 
-// (gate and out may be the same memory: neither is declared __restrict__ in this file.)
+// An output acc / sum times its gate; zero, whatever the gate holds, where no
+// token took part. (gate and out may be the same memory: neither is declared
+// __restrict__ in this file.)
 template <typename IO>
-__device__ __forceinline__ void store_out(IO* out, const IO* gate, int64_t i, float v) {
-  if (gate) v = v * (1.f / (1.f + expf(-to_f32(gate[i]))));  // math.ts:271-273
+__device__ __forceinline__ void store_out(IO* out, const IO* gate, int64_t i, float acc, float sum) {
+  float v = sum != 0.f ? acc / sum : 0.f;
+  if (gate && sum != 0.f) v = v * (1.f / (1.f + expf(-to_f32(gate[i]))));  // math.ts:271-273
   out[i] = from_f32<IO>(v);
 }
 
@@ -74,7 +77,7 @@ __device__ __forceinline__ void join_warps(const float* red, int D, int heads, i
         t[1] = sum;
       }
     } else {
-      store_out(out, gate, row * D + d, sum != 0.f ? acc / sum : 0.f);
+      store_out(out, gate, row * D + d, acc, sum);
     }
   }
 }
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(kThreads)
       sum += t[s * (D + 2) + 1] * f;
       acc += t[s * (D + 2) + 2 + d] * f;
     }
-    store_out(out, gate, row * D + d, sum != 0.f ? acc / sum : 0.f);
+    store_out(out, gate, row * D + d, acc, sum);
   }
 }
 
