@@ -262,12 +262,14 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   return r;
 }
 
-// An output acc / sum times its gate; zero, whatever the gate holds, where no
-// token took part.
+// 1 / sum, or 0 where no token took part.
+__device__ __forceinline__ float inverse(float sum) { return sum != 0.f ? 1.f / sum : 0.f; }
+// An output v (times inverse(sum)) and its gate; zero, whatever the gate holds,
+// where no token took part.
 template <typename IO>
-__device__ __forceinline__ void store_out(const DecodeParams& d, int64_t i, float acc, float sum) {
-  float v = sum != 0.f ? acc * (1.f / sum) : 0.f;
-  if (d.gate && sum != 0.f) v = v * (1.f / (1.f + expf(-to_f32(static_cast<const IO*>(d.gate)[i]))));  // math.ts:271-273
+__device__ __forceinline__ void store_out(const DecodeParams& d, int64_t i, float v, float inv) {
+  v *= inv;
+  if (d.gate && inv != 0.f) v = v * (1.f / (1.f + expf(-to_f32(static_cast<const IO*>(d.gate)[i]))));  // math.ts:271-273
   static_cast<IO*>(d.out)[i] = from_f32<IO>(v);
 }
 
@@ -729,8 +731,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         v1 += x.y * f;
       }
       if (whole) {
-        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c, v0, sum);
-        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c + 1, v1, sum);
+        const float inv = inverse(sum);
+        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c, v0, inv);
+        if (c < hd) store_out<IO>(d, (static_cast<int64_t>(b) * Hq + h0 + r) * hd + c + 1, v1, inv);
       } else if (d.cluster ||
                  TLA_IN_BOUNDS(mine - d.scratch + (r + 1) * (D + 2) - 1, d.scratch_floats, p.a.error)) {
         *reinterpret_cast<float2*>(mine + r * (D + 2) + 2 + c) = make_float2(v0, v1);
@@ -773,8 +776,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         v0 += x[k].x * f;
         v1 += x[k].y * f;
       }
-      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c, v0, sum);
-      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c + 1, v1, sum);
+      const float inv = inverse(sum);
+      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c, v0, inv);
+      store_out<IO>(d, (static_cast<int64_t>(only_b) * Hq + h0 + r) * hd + c + 1, v1, inv);
     }
     cluster.sync();  // the others may still read this CTA's triple
   }
@@ -868,7 +872,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
       if (lane + 32 * e < p.a.D)
-        store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + lane + 32 * e, acc[e], sum);
+        store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + lane + 32 * e, acc[e], inverse(sum));
     return;
   }
   if (lane == 0) {
@@ -890,7 +894,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_decode_join_kernel(cons
       all += red[1][w] * f;
       v += row_s[w][c] * f;
     }
-    store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + c, v, all);
+    store_out<IO>(d, static_cast<int64_t>(blockIdx.x) * p.a.D + c, v, inverse(all));
   }
 }
 
