@@ -19,6 +19,22 @@ pytestmark = pytest.mark.gpu
 ROOT = Path(__file__).resolve().parent.parent
 
 
+@pytest.mark.parametrize("page", [8, 16])
+@pytest.mark.parametrize("wide", [1, WIDE])
+def test_decode_reports_what_follows_a_full_list(pkg, cuda, page, wide):
+    """A list that names every page of the sequence and goes on with something else than a negative entry."""
+    w = World([3 * page - 2, 3 * page - 2], 1, 64, page, "fp16", extra_width=wide)
+    layer, *_ = make(pkg, cuda, w, 4, 1, 64, "fp16")
+    q, pos, table = w.normal(2, 256, dtype=torch.float16).to(cuda), ints([3 * page - 3] * 2, cuda), w.device_table(cuda)
+    exp = layer.decode(q, pos, table)
+    assert layer.context.error() == 0
+    for tail, code in ((-1, 0), (3, -18), (0, -18), (1 << 30, -18)):
+        out = layer.decode(q, pos, table, pages=ints([[[0, 1, 2, -1]], [[0, 1, 2, tail]]], cuda))
+        assert layer.context.error() == code
+        # (the same tokens, perhaps in other shares: both round weights and output once)
+        assert (out.float() - exp.float()).abs().max() <= 4 * 2.0 ** -10
+
+
 # ---------------------------------------------------------------- select: tables next to the 48 KB default
 SELECT_TABLES = """
 import sys

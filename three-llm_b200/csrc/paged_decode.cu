@@ -415,7 +415,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       ld.base = static_cast<int>((static_cast<int64_t>(ld.first + ld.it - ld.begin) * C::kTile) >> shift);
       look(ld.base + lane, &ld.index, &ld.page);
       look(ld.base + 32 + lane, &ld.index_next, &ld.page_next);
-      if (ld.list) ld.e_end = min(ld.e_end, list_length(p, ld.list, most, last_page, lane));
+      // (one entry past a list of all pages: it has to be a negative one)
+      if (ld.list) ld.e_end = min(ld.e_end, list_length(p, ld.list, min(d.count, last_page + 2), last_page, lane));
     }
     if (ld.it < ld.end) {
       const int64_t token = static_cast<int64_t>(ld.first + ld.it - ld.begin) * C::kTile;
