@@ -251,6 +251,40 @@ def test_append_scaled_and_partial_rotations(pkg, cuda, options, form, d, io, ke
             at += 1
 
 
+@pytest.mark.parametrize("options", [{"rotaryDim": 0}, {"rotaryDim": 16}, {"ropePairCount": 5}, {"rotaryDim": 24, "ropePairCount": 0}],
+                         ids=str)
+@pytest.mark.parametrize("form", ["one", "chunks", "chunks without bounds"])
+@pytest.mark.parametrize("d,io,kept", [(64, "fp16", "fp16"), (128, "bf16", "bf16"), (96, "fp32", "fp16"), (256, "fp32", "fp32"),
+                                       (100, "fp32", "fp32")])
+def test_append_turns_only_the_pairs_it_should(pkg, cuda, options, form, d, io, kept):
+    """An infinity or a NaN reaches its own dimension, and its pair's where that is turned, and no other."""
+    hq, hk, page, starts, chunks = 2, 2, 16, [1, 17], [1, 1] if form == "one" else [40, 20]
+    w = World(starts, hk, d, page, kept, room=40)
+    layer, k, v, _ = make(pkg, cuda, w, hq, hk, d, io, bounds=form != "chunks without bounds", ropeTheta=1e4, **options)
+    x = w.normal(sum(chunks), 3, hk, d, dtype=TYPES[io])
+    for held in (float("inf"), float("-inf"), float("nan")):
+        x[torch.rand(x.shape, generator=w.g) < 0.02] = held
+    offsets = None if form == "one" else ints([0, 40, 60], cuda)
+    query = layer.append(x.view(sum(chunks), -1).to(cuda), ints(starts, cuda), w.device_table(cuda), row_offsets=offsets)
+    half = options.get("rotaryDim", d) // 2
+    pairs = min(half, options.get("ropePairCount", half))
+    hit = ~x.isfinite()
+    both = hit[..., :pairs] | hit[..., half:half + pairs]
+    hit[:, :2, :, :pairs], hit[:, :2, :, half:half + pairs] = both[:, :2], both[:, :2]
+    still = torch.ones(d, dtype=torch.bool)
+    still[:pairs] = still[half:half + pairs] = False
+    assert torch.equal(~query.view(-1, hq, d).isfinite().cpu(), hit[:, 0])
+    at = 0
+    for b, n in enumerate(chunks):
+        for i in range(n):
+            p, slot = w.table[b][(starts[b] + i) // page], (starts[b] + i) % page
+            for pool, part, plain in ((k, 1, still), (v, 2, torch.ones(d, dtype=torch.bool))):
+                got, exp = pool[p, :, slot].cpu(), x[at, part]
+                assert torch.equal(~got.isfinite(), hit[at, part])
+                assert torch.equal(got[:, plain].nan_to_num(nan=77.0), exp[:, plain].to(w.kept).nan_to_num(nan=77.0))
+            at += 1
+
+
 # ---------------------------------------------------------------- gates, alignment, empty calls
 @pytest.mark.parametrize("d,io,kept,page", [(64, "fp32", "fp32", 16), (128, "fp32", "bf16", 16), (64, "fp16", "fp16", 4),
                                             (100, "fp16", "fp16", 16), (256, "fp32", "fp16", 16)])

@@ -248,7 +248,8 @@ __device__ __forceinline__ Raw4<T> lane_xor(Raw4<T> v, int o) {
 // the row's cosines and sines once, one or two per lane, and hands them out by
 // shuffles (at 256 each lane its own four). Without `keys` the row's keys are
 // left to the blocks that go by pages. `unit`: the warp's (row, part).
-template <typename IO, typename CT, int D, bool EXACT>
+// TURNED: the rotation turns every dimension.
+template <typename IO, typename CT, int D, bool EXACT, bool TURNED>
 __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __restrict__ qkv,
                                             const int32_t* __restrict__ offsets, int rows,
                                             IO* __restrict__ query_out, int parts, int part_heads, bool keys,
@@ -289,12 +290,12 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
   const int slot = pos & ((1 << p.page_shift) - 1);
   // (a part with queries only does not need the page)
   const int page = h_end > Hq ? pool_page(p, b, pos >> p.page_shift) : -1;
+  const int turned = i0 < half ? min(a.pair_count, half) - i0 : 0;  // of this lane's pairs, those before this one
   float cos4[4], sin4[4];
   if (h_begin < Hq + k_heads) {
     float c0 = 1.f, s0 = 0.f, c1 = 1.f, s1 = 0.f;
     if (D < 256 && lane < min(a.pair_count, half)) rope_cos_sin(pos, a.inv_freq[lane], &c0, &s0);
     if (D == 128 && lane + 32 < min(a.pair_count, half)) rope_cos_sin(pos, a.inv_freq[lane + 32], &c1, &s1);
-    const int turned = i0 < half ? min(a.pair_count, half) - i0 : 0;  // of this lane's pairs, those before this one
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int src_lane = (i0 + e) & 31;
@@ -366,11 +367,13 @@ __device__ __forceinline__ void append_rows(const PagedArgs& p, const IO* __rest
           y = make_float4(y.x * r[c], y.y * r[c], y.z * r[c], y.w * r[c]);
         }
         if (kKind < 2) {  // RoPE, math.ts:134-147
-          const float4 u = x;
-          x = make_float4(u.x * xc[0] - y.x * ys[0], u.y * xc[1] - y.y * ys[1], u.z * xc[2] - y.z * ys[2],
-                          u.w * xc[3] - y.w * ys[3]);
-          y = make_float4(y.x * yc[0] + u.x * xs[0], y.y * yc[1] + u.y * xs[1], y.z * yc[2] + u.z * xs[2],
-                          y.w * yc[3] + u.w * xs[3]);
+          // (a dimension that stays takes nothing from its partner, not even 0 times an infinity)
+          const float4 u = x, v = y;
+          const auto from = [&](int e, float partner) { return TURNED || e < turned ? partner : 0.f; };
+          x = make_float4(u.x * xc[0] - from(0, v.x) * ys[0], u.y * xc[1] - from(1, v.y) * ys[1],
+                          u.z * xc[2] - from(2, v.z) * ys[2], u.w * xc[3] - from(3, v.w) * ys[3]);
+          y = make_float4(v.x * yc[0] + from(0, u.x) * xs[0], v.y * yc[1] + from(1, u.y) * xs[1],
+                          v.z * yc[2] + from(2, u.z) * xs[2], v.w * yc[3] + from(3, u.w) * xs[3]);
         }
         const int h = h0 + c * kPer;
         if (h >= to || !on) continue;
@@ -470,7 +473,7 @@ __device__ __forceinline__ bool find_page(const PagedArgs& p, const int32_t* off
 // cos(a + b) = cos a cos b - sin a sin b and its like add three roundings and
 // spare 31 of 32 evaluations, which with few rows per block would bound it.
 constexpr int kPageThreads = 256;
-template <typename IO, typename CT, int D, bool EXACT>
+template <typename IO, typename CT, int D, bool EXACT, bool TURNED>
 __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __restrict__ qkv,
                                             const int32_t* __restrict__ offsets, int rows, int heads, int unit) {
   constexpr int kLanes = D / 8, kPer = 32 / kLanes, kWarps = kPageThreads / 32;
@@ -558,8 +561,9 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 t = turn_s[s][i0 + e];
-            const float u = x[e] * t.x - y[e] * t.y;
-            y[e] = y[e] * t.x + x[e] * t.y;
+            const bool turned = TURNED || i0 + e < pairs;  // (else nothing comes over, not even 0 times an infinity)
+            const float u = x[e] * t.x - (turned ? y[e] : 0.f) * t.y;
+            y[e] = y[e] * t.x + (turned ? x[e] : 0.f) * t.y;
             x[e] = u;
           }
         }
@@ -609,29 +613,29 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
 }
 
 // Rows only.
-template <typename IO, typename CT, int D, bool EXACT>
+template <typename IO, typename CT, int D, bool EXACT, bool TURNED>
 __global__ void __launch_bounds__(kThreads, 5)
     paged_append_rows_kernel(PagedArgs p, const IO* __restrict__ qkv, const int32_t* __restrict__ offsets, int rows,
                              IO* __restrict__ query_out, int parts, int part_heads) {
   griddep_wait();
   griddep_launch_dependents();
-  append_rows<IO, CT, D, EXACT>(p, qkv, offsets, rows, query_out, parts, part_heads, true,
+  append_rows<IO, CT, D, EXACT, TURNED>(p, qkv, offsets, rows, query_out, parts, part_heads, true,
                                 static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5));
 }
 
 // Chunks into a pool with bounds: the first blocks take the touched pages'
 // keys, the others the rows' queries and values.
-template <typename IO, typename CT, int D, bool EXACT, int kBlocks>
+template <typename IO, typename CT, int D, bool EXACT, int kBlocks, bool TURNED>
 __global__ void __launch_bounds__(kPageThreads, kBlocks)
     paged_append_chunks_kernel(PagedArgs p, const IO* __restrict__ qkv, const int32_t* __restrict__ offsets, int rows,
                                IO* __restrict__ query_out, int parts, int part_heads, int page_blocks, int page_heads) {
   griddep_wait();
   griddep_launch_dependents();
   if (static_cast<int>(blockIdx.x) < page_blocks)
-    append_page<IO, CT, D, EXACT>(p, qkv, offsets, rows, page_heads, blockIdx.x);
+    append_page<IO, CT, D, EXACT, TURNED>(p, qkv, offsets, rows, page_heads, blockIdx.x);
   else
-    append_rows<IO, CT, D, EXACT>(p, qkv, offsets, rows, query_out, parts, part_heads, false,
-                                  static_cast<int64_t>(blockIdx.x - page_blocks) * (kPageThreads / 32) + (threadIdx.x >> 5));
+    append_rows<IO, CT, D, EXACT, TURNED>(p, qkv, offsets, rows, query_out, parts, part_heads, false,
+                                          static_cast<int64_t>(blockIdx.x - page_blocks) * (kPageThreads / 32) + (threadIdx.x >> 5));
 }
 
 // Bounds of the pages that a chunk touched, any shape: the block of a page's
@@ -679,52 +683,62 @@ size_t row_smem(const tla_paged* P) {
   return sizeof(float) * (static_cast<size_t>(P->base.Hq + 2 * P->base.Hk) * P->base.D + P->base.rotary);
 }
 
+template <typename IO, typename CT, bool TURNED>
+cudaError_t append_by_rows(const tla_paged* P, const PagedArgs& p, const void* qkv, const int32_t* offsets, int rows,
+                           void* query_out, cudaStream_t stream) {
+  const int D = p.a.D;
+  const bool by_pages = p.bounds && offsets;
+  // Warps per row: enough for 16 on every SM, at most one per warp-wide load
+  // (64 rows of 48 heads: 12 warps per row).
+  const int heads = p.a.Hq + (by_pages ? 1 : 2) * p.a.Hk, per = 256 / (D == 64 ? 64 : D <= 128 ? 128 : 256);
+  const int most = (heads + per - 1) / per;
+  long long parts = (16LL * P->base.ctx->sm_count + rows - 1) / rows;
+  parts = parts < 1 ? 1 : parts > most ? most : parts;
+  const int part_heads = (most + static_cast<int>(parts) - 1) / static_cast<int>(parts) * per;
+  parts = (heads + part_heads - 1) / part_heads;
+  if (!by_pages) {
+    auto k = D == 64    ? paged_append_rows_kernel<IO, CT, 64, true, TURNED>
+             : D == 128 ? paged_append_rows_kernel<IO, CT, 128, true, TURNED>
+             : D < 128  ? paged_append_rows_kernel<IO, CT, 128, false, TURNED>
+                        : paged_append_rows_kernel<IO, CT, 256, false, TURNED>;
+    return launch_pdl(k, static_cast<unsigned>((rows * parts + 3) / 4), kThreads, 0, stream, p,
+                      static_cast<const IO*>(qkv), offsets, rows, static_cast<IO*>(query_out),
+                      static_cast<int>(parts), part_heads);
+  }
+  // a chunk of n rows touches at most (n - 1) / page_size + 2 pages, and no more than its rows
+  const long long pages =
+      min(static_cast<long long>(rows), (static_cast<long long>(rows) >> p.page_shift) + 2LL * p.batch);
+  // kv heads per page block: all eight warps on one while that gives no more
+  // than two blocks per SM (one or four: 24 and 23 us for 16 chunks of up to
+  // 500 rows, 48 heads of 64, against 20)
+  int page_heads = 1;
+  while (page_heads < 8 && page_heads < p.a.Hk &&
+         pages * ((p.a.Hk + page_heads - 1) / page_heads) > 2 * P->base.ctx->sm_count)
+    page_heads *= 2;
+  const long long blocks = pages * ((p.a.Hk + page_heads - 1) / page_heads);
+  // Long chunks run at four blocks per SM (64 registers): more reads in
+  // flight, 96 us against 104 for 20,000 rows of 48 heads of 128; short ones
+  // at three, 7.2 us against 8.9 for 2048 rows of 18 heads of 64.
+  const int warps = kPageThreads / 32;
+  const long long grid = blocks + (rows * parts + warps - 1) / warps;
+  const bool many = grid > 6LL * P->base.ctx->sm_count;
+  auto k = D < 128 ? paged_append_chunks_kernel<IO, CT, 128, false, 3, TURNED>
+                   : paged_append_chunks_kernel<IO, CT, 256, false, 3, TURNED>;
+  if (D == 64)
+    k = many ? paged_append_chunks_kernel<IO, CT, 64, true, 4, TURNED> : paged_append_chunks_kernel<IO, CT, 64, true, 3, TURNED>;
+  if (D == 128)
+    k = many ? paged_append_chunks_kernel<IO, CT, 128, true, 4, TURNED> : paged_append_chunks_kernel<IO, CT, 128, true, 3, TURNED>;
+  return launch_pdl(k, static_cast<unsigned>(grid), kPageThreads, 0, stream, p, static_cast<const IO*>(qkv), offsets, rows,
+                    static_cast<IO*>(query_out), static_cast<int>(parts), part_heads, static_cast<int>(blocks), page_heads);
+}
+
 template <typename IO, typename CT>
 cudaError_t append_t(const tla_paged* P, const PagedArgs& p, const void* qkv, const int32_t* offsets, int rows,
                      void* query_out, cudaStream_t stream) {
-  const int D = p.a.D;
-  const bool by_pages = p.bounds && offsets;
-  if (by_rows(P)) {
-    // Warps per row: enough for 16 on every SM, at most one per warp-wide load
-    // (64 rows of 48 heads: 12 warps per row).
-    const int heads = p.a.Hq + (by_pages ? 1 : 2) * p.a.Hk, per = 256 / (D == 64 ? 64 : D <= 128 ? 128 : 256), most = (heads + per - 1) / per;
-    long long parts = (16LL * P->base.ctx->sm_count + rows - 1) / rows;
-    parts = parts < 1 ? 1 : parts > most ? most : parts;
-    const int part_heads = (most + static_cast<int>(parts) - 1) / static_cast<int>(parts) * per;
-    parts = (heads + part_heads - 1) / part_heads;
-    if (!by_pages) {
-      auto k = D == 64    ? paged_append_rows_kernel<IO, CT, 64, true>
-               : D == 128 ? paged_append_rows_kernel<IO, CT, 128, true>
-               : D < 128  ? paged_append_rows_kernel<IO, CT, 128, false>
-                          : paged_append_rows_kernel<IO, CT, 256, false>;
-      return launch_pdl(k, static_cast<unsigned>((rows * parts + 3) / 4), kThreads, 0, stream, p,
-                        static_cast<const IO*>(qkv), offsets, rows, static_cast<IO*>(query_out),
-                        static_cast<int>(parts), part_heads);
-    }
-    // a chunk of n rows touches at most (n - 1) / page_size + 2 pages, and no more than its rows
-    const long long pages =
-        min(static_cast<long long>(rows), (static_cast<long long>(rows) >> p.page_shift) + 2LL * p.batch);
-    // kv heads per page block: all eight warps on one while that gives no more
-    // than two blocks per SM (one or four: 24 and 23 us for 16 chunks of up to
-    // 500 rows, 48 heads of 64, against 20)
-    int page_heads = 1;
-    while (page_heads < 8 && page_heads < p.a.Hk && pages * ((p.a.Hk + page_heads - 1) / page_heads) > 2 * P->base.ctx->sm_count)
-      page_heads *= 2;
-    const long long blocks = pages * ((p.a.Hk + page_heads - 1) / page_heads);
-    // Long chunks run at four blocks per SM (64 registers): more reads in
-    // flight, 96 us against 104 for 20,000 rows of 48 heads of 128; short ones
-    // at three, 7.2 us against 8.9 for 2048 rows of 18 heads of 64.
-    const int warps = kPageThreads / 32;
-    const long long grid = blocks + (rows * parts + warps - 1) / warps;
-    const bool many = grid > 6LL * P->base.ctx->sm_count;
-    auto k = D < 128 ? paged_append_chunks_kernel<IO, CT, 128, false, 3> : paged_append_chunks_kernel<IO, CT, 256, false, 3>;
-    if (D == 64)
-      k = many ? paged_append_chunks_kernel<IO, CT, 64, true, 4> : paged_append_chunks_kernel<IO, CT, 64, true, 3>;
-    if (D == 128)
-      k = many ? paged_append_chunks_kernel<IO, CT, 128, true, 4> : paged_append_chunks_kernel<IO, CT, 128, true, 3>;
-    return launch_pdl(k, static_cast<unsigned>(grid), kPageThreads, 0, stream, p, static_cast<const IO*>(qkv), offsets, rows, static_cast<IO*>(query_out), static_cast<int>(parts),
-                      part_heads, static_cast<int>(blocks), page_heads);
-  }
+  if (by_rows(P))
+    return p.a.rotary == p.a.D && p.a.pair_count >= p.a.rotary / 2
+               ? append_by_rows<IO, CT, true>(P, p, qkv, offsets, rows, query_out, stream)
+               : append_by_rows<IO, CT, false>(P, p, qkv, offsets, rows, query_out, stream);
   const size_t smem = row_smem(P);
   auto k = paged_append_kernel<IO, CT>;
   cudaError_t e = cudaSuccess;
@@ -732,7 +746,7 @@ cudaError_t append_t(const tla_paged* P, const PagedArgs& p, const void* qkv, co
   if (e != cudaSuccess) return e;
   e = launch_pdl(k, rows, kThreads, smem, stream, p, static_cast<const IO*>(qkv), offsets, rows,
                  static_cast<IO*>(query_out));
-  if (e != cudaSuccess || !by_pages) return e;
+  if (e != cudaSuccess || !p.bounds || !offsets) return e;
   return launch_pdl(paged_bounds_kernel<CT>, rows, kThreads, 0, stream, p, offsets, rows);
 }
 
