@@ -350,7 +350,8 @@ typedef struct tla_page_pool {
   void* value;             /* kv_head*head_stride + slot*slot_stride + d, strides in elements      */
   void* bounds;            /* device [page_count][kv_head_count][2][head_dim] in the pages' type, 16-byte
                               aligned, or NULL: per page the smallest and the largest key of every
-                              dimension over the slots appended so far */
+                              dimension over the slots appended so far (NaN keys are left out; a dimension that
+                              has no others has no meaning) */
   int64_t page_stride, head_stride, slot_stride;
   int32_t page_count;
   int32_t page_size;       /* tokens per page: a power of two up to 1024 */
@@ -410,7 +411,8 @@ int tla_paged_decode(tla_paged* layer, const void* query, const int32_t* positio
  * heads and over d of q_d * high_d where q_d > 0 and q_d * low_d where q_d < 0,
  * low and high being its bounds: an upper bound on the summed dot products
  * with any of its keys. It is summed in 64 bits and rounded to 32; ties go to
- * the lower page. Needs a pool with bounds and a positive attn_scale.
+ * the lower page. (Bounds of 16 bits that are not finite count as numbers of the
+ * next exponent, an infinity as 65536 in float16 and 2^128 in bfloat16.) Needs a pool with bounds and a positive attn_scale.
  *   pages_out device int32 [batch][kv_head_count][page_count], rising, then -1 */
 int tla_paged_select(tla_paged* layer, const void* query, const int32_t* positions, const int32_t* page_table,
                      int32_t table_width, int32_t first_pages, int32_t last_pages, int32_t* pages_out,

@@ -35,6 +35,41 @@ def test_decode_reports_what_follows_a_full_list(pkg, cuda, page, wide):
         assert (out.float() - exp.float()).abs().max() <= 4 * 2.0 ** -10
 
 
+@pytest.mark.parametrize("d,io,kept", [(64, "fp16", "fp16"), (128, "bf16", "bf16"), (96, "fp32", "fp16"), (256, "fp32", "fp32"),
+                                       (100, "fp16", "fp16"), (100, "fp32", "fp32"), (64, "fp32", "bf16")])
+@pytest.mark.parametrize("chunks", [[1, 1, 1], [40, 1, 33], None])
+def test_append_bounds_leave_out_what_is_no_number(pkg, cuda, d, io, kept, chunks):
+    """NaN keys are stored but not counted, first and last slots among them, however the tokens were appended."""
+    hk, page, n = 2, 16, 48
+    w = World([0, 0, 0], hk, d, page, kept, room=n)
+    layer, k, v, bd = make(pkg, cuda, w, hk, hk, d, io, rotaryDim=0)
+    x = w.normal(3, n, 3 * hk * d, dtype=TYPES[io])
+    keys = x.view(3, n, 3, hk, d)[:, :, 1]
+    keys[torch.rand(keys.shape, generator=w.g) < 0.3] = float("nan")
+    keys[:, 0::16, :, 1] = float("nan")
+    keys[:, 15::16, :, 2] = float("nan")
+    keys[:, 3::16, :] = w.normal(*keys[:, 3::16].shape, dtype=TYPES[io])  # one number at least
+    table = w.device_table(cuda)
+    at = [0, 0, 0]
+    while min(at) < n:  # to 48 tokens each, from the start
+        new = [min(c, n - a) for c, a in zip(chunks or [n, n, n], at)]
+        rows = torch.cat([x[b, a:a + c] for b, (a, c) in enumerate(zip(at, new))]).to(cuda)
+        offsets = None
+        if new != [1, 1, 1] or chunks != [1, 1, 1]:
+            offsets = ints([0, new[0], new[0] + new[1], sum(new)], cuda)
+        layer.append(rows, ints(at, cuda), table, row_offsets=offsets)
+        at = [a + c for a, c in zip(at, new)]
+        if chunks == [40, 1, 33]:
+            chunks = [5, 20, 1]
+    assert layer.context.error() == 0
+    stored = keys.to(w.kept).float().view(3, n // page, page, hk, d)
+    low, high = stored.nan_to_num(nan=float("inf")).amin(2), stored.nan_to_num(nan=float("-inf")).amax(2)
+    for b in range(3):
+        for i in range(n // page):
+            p = w.table[b][i]
+            assert torch.equal(bd[p, :, 0].float().cpu(), low[b, i]) and torch.equal(bd[p, :, 1].float().cpu(), high[b, i])
+
+
 # ---------------------------------------------------------------- select: tables next to the 48 KB default
 SELECT_TABLES = """
 import sys

@@ -57,13 +57,16 @@ __device__ __forceinline__ int sequence_of_warp(const int32_t* offsets, int batc
   return lo < batch && offsets[lo] <= row && row < offsets[lo + 1] ? lo : -1;
 }
 
+// The smaller and the larger of two; what is no number gives way to a number.
 template <typename CT>
 __device__ __forceinline__ CT low_of(CT a, CT b) {
-  return to_f32(b) < to_f32(a) ? b : a;
+  const float x = to_f32(a), y = to_f32(b);
+  return y < x || x != x ? b : a;
 }
 template <typename CT>
 __device__ __forceinline__ CT high_of(CT a, CT b) {
-  return to_f32(b) > to_f32(a) ? b : a;
+  const float x = to_f32(a), y = to_f32(b);
+  return y > x || x != x ? b : a;
 }
 
 // A block per row.
@@ -202,7 +205,7 @@ __device__ __forceinline__ void put_same(T* p, Raw4<U> v) {
   store4(p, floats(v));
 }
 
-// The smaller and the larger of two, element by element (a NaN gives way to a number).
+// The same of pairs and of four.
 template <typename P>
 __device__ __forceinline__ uint32_t low_pair(uint32_t a, uint32_t b) {
   const P v = __hmin2(*reinterpret_cast<P*>(&a), *reinterpret_cast<P*>(&b));
@@ -604,10 +607,7 @@ __device__ __forceinline__ void append_page(const PagedArgs& p, const IO* __rest
       v = (is_low ? u < v : u > v) ? u : v;
     }
     CT* to = static_cast<CT*>(p.bounds) + bounds_row(p, page, head, hd) + at;
-    if (begin > 0) {
-      const float u = to_f32(to[0]);
-      v = (is_low ? v < u : v > u) ? v : u;
-    }
+    if (begin > 0) v = is_low ? low_of(to_f32(to[0]), v) : high_of(to_f32(to[0]), v);
     to[0] = from_f32<CT>(v);
   }
 }
