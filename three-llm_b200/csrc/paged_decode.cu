@@ -1021,19 +1021,27 @@ long long most_tiles(const PagedArgs& p, int count) {
 // CTAs per pair when a cluster takes it, 0 when the pairs' tiles are cut into
 // shares. A cluster joins its triples itself: one launch, no workspace, only
 // its own sequence's position to wait for. It gets a CTA per four tiles, up to
-// 16 and up to two CTAs per SM in all. Shares balance unequal lengths and fill
-// every SM; they win where a CTA of a cluster would get many tiles. Measured
-// (shares / cluster, us; head_dim 64, 4 query heads for each of 8 kv heads):
-// 1 x 1025 tokens 6.9 / 5.9, 8 x 4097 18.0 / 16.6, 64 x 1025 35.0 / 29.6; of
-// lengths from a sixteenth up: 64 x 2049 30.7 / 28.5 (65 tiles per CTA), 16 x
-// 2049 12.6 / 13.5 (33), 64 x 4097 45.5 / 48.3; 1 x 8193 8.9 / 9.4 (17, on 128
-// CTAs only).
+// 16 (8 above head_dim 128) and up to two CTAs per SM in all. Shares balance
+// unequal lengths and fill every SM; they win where a CTA of a cluster would get
+// many tiles. Measured (shares / cluster, us; 4 query heads for each of 8 kv
+// heads; * what the rule takes):
+//   head_dim 64:  1 x 1025 tokens 7.0 / 5.7*, 1 x 8193 8.6* / 9.4, 8 x 4097 17.8 / 16.5*,
+//                 64 x 1025 35.1 / 29.4*
+//   head_dim 128: 1 x 1025 8.6 / 7.0*, 1 x 8193 12.6* / 12.8, 8 x 2049 17.7 / 16.5*,
+//                 8 x 4097 27.7* / 25.8, 64 x 1025 53.1* / 47.2
+//   head_dim 256: 1 x 1025 9.5 / 9.0*, 1 x 2049 9.8 / 11.0*, 1 x 4097 13.3* / 15.5, 8 x 4097 48.9* / 46.4
+// and of lengths from a sixteenth up:
+//   head_dim 64:  16 x 2049 12.6 / 13.1*, 64 x 2049 30.8* / 28.1, 64 x 4097 45.4* / 47.6
+//   head_dim 128: 16 x 2049 16.3* / 19.5, 64 x 2049 45.6* / 44.8, 64 x 4097 75.2* / 80.1
+// Above head_dim 128 an SM holds one CTA, and clusters of 16 leave a GPC's other
+// SMs idle: 1 x 1025, 2049 and 4097 took 15.2, 17.3 and 22.0 us in them.
 int cluster_size(const tla_paged* P, const PagedArgs& p, int count) {
   const long long tiles = most_tiles(p, count), pairs = static_cast<long long>(p.batch) * p.a.Hk * subgroups(P);
   const int sms = P->base.ctx->sm_count;
   const int per_sm = p.a.D > 128 ? 1 : kCtasPerSm;
+  const int most = p.a.D > 128 && P->decode_cluster > 8 ? 8 : P->decode_cluster;
   int n = 1;
-  while (n < P->decode_cluster && tiles > 4 * n && pairs * n * 2 <= per_sm * sms) n *= 2;
+  while (n < most && tiles > 4 * n && pairs * n * 2 <= per_sm * sms) n *= 2;
   return tiles <= (pairs * n > sms ? 40 : 20) * n ? n : 0;
 }
 
