@@ -716,9 +716,14 @@ cudaError_t append_by_rows(const tla_paged* P, const PagedArgs& p, const void* q
          pages * ((p.a.Hk + page_heads - 1) / page_heads) > 2 * P->base.ctx->sm_count)
     page_heads *= 2;
   const long long blocks = pages * ((p.a.Hk + page_heads - 1) / page_heads);
-  // Long chunks run at four blocks per SM (64 registers): more reads in
-  // flight, 96 us against 104 for 20,000 rows of 48 heads of 128; short ones
-  // at three, 7.2 us against 8.9 for 2048 rows of 18 heads of 64.
+  // Many blocks run four on an SM (64 registers): more reads in flight; few
+  // three, which spares the spills. Measured (three / four, us; * what the rule
+  // takes), 32 + 8 + 8 heads of 128: 1 chunk of 2048 rows 17.1* / 15.2, of 8192
+  // 41.8 / 37.6*, 16 of up to 256 16.5* / 17.2, of up to 1024 41.2 / 43.0*, of
+  // up to 2047 95 / 88* (with QK-norm, token-major bfloat16 pages 104 / 93*);
+  // the same heads of 64: 1 of 2048 10.2* / 8.9, 16 of up to 256 8.9* / 9.5, of
+  // up to 2047 56 / 50*; 14 + 2 + 2 heads of 64: 1 of 2048 7.3* / 8.4. Widths
+  // between and above have the three only.
   const int warps = kPageThreads / 32;
   const long long grid = blocks + (rows * parts + warps - 1) / warps;
   const bool many = grid > 6LL * P->base.ctx->sm_count;

@@ -473,11 +473,15 @@ cudaError_t select_t(const tla_paged* P, const PagedArgs& p, const void* query, 
     // while another picks. A cluster's blocks share the scores out, up to eight,
     // at least two pages per warp, as long as all blocks run at once (five per
     // SM of 128 threads, two of 256, one of 512; the longest ones up to 1.6
-    // times that). Measured (threads x blocks per pair, us): 512 pairs of 64
-    // pages 128 x 1 7.5, x 2 13.2; 160 of 1250 (128 wide) 128 x 4 36.7, 256 x 1
-    // 53, 512 x 2 52; 256 of 4000 256 x 1 91, 128 x 2 109, 512 x 2 111; 64 of 500
-    // (128 wide) 256 x 4 9.3, x 8 15.2; 114 of up to 5562 512 x 2 46, x 8 60; 32
-    // of 1875 512 x 4 13.8, x 8 22.2.
+    // times that). Measured (threads x blocks per pair, us; * what the rule
+    // takes): 512 pairs of 64 pages 128 x 1 7.3*, x 2 13.0; 160 of 1250 (128
+    // wide) 128 x 4 36.7*, 256 x 1 53, 512 x 2 52; 256 of 256 (128 wide) 128 x 1
+    // 20.6, x 2 16.6*, x 4 19.1, 256 x 1 14.6, of ragged lengths up to that 128 x
+    // 1 14.5, x 2 12.5*, x 4 11.8, 256 x 1 12.0; 256 of 4000 256 x 1 91*, 128 x 2
+    // 109, 512 x 2 111; 128 of 256 (128 wide) 128 x 4 10.1*, 256 x 2 8.9; 64 of
+    // 500 (128 wide) 256 x 4 9.3*, x 8 15.2; 32 of 1024 (128 wide) 256 x 8 13.5*,
+    // x 4 11.5, 512 x 2 12.8; 114 of up to 5562 512 x 2 46*, x 8 60; 32 of 1875
+    // 512 x 4 13.8*, x 8 22.2; 8 of 2048 (128 wide) 512 x 8 9.9*, x 2 20.
     // (Clusters of 16 leave a GPC's other SMs idle: 8 of them with 512 threads
     // each ran in two waves, 28 us for a sparse step at 131072 tokens.)
     const int sms = P->base.ctx->sm_count;
