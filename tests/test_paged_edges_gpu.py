@@ -223,6 +223,61 @@ def test_decode_gives_a_constant_back(pkg, cuda, io, kept, wide, low):
     assert (out - c).abs().max() <= (2.0 ** -17 * c if io == "fp32" else 0.0)
 
 
+@pytest.mark.parametrize("io,kept", [("fp32", "fp16"), ("fp16", "fp16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("wide", [1, WIDE])
+@pytest.mark.parametrize("d,hq", [(64, 4), (64, 16), (128, 7), (256, 8)])
+def test_decode_rounds_nothing_but_its_output(pkg, cuda, io, kept, wide, d, hq):
+    """Two weights, one of them as far from the 16-bit type as they come, whose shares of the output nearly cancel: what
+    the weights were rounded to would be most of what is left."""
+    n, page = 700, 16
+    w = World([n], 1, d, page, kept, extra_width=wide)
+    p, s = places(w, n)
+    gap = worst_gap(w.kept, 0.5, 1.0)
+    w.keys[p, 0, s] = 0
+    w.keys[p[::2], 0, s[::2], 0] = gap
+    w.values[p[::2], 0, s[::2]] = 1
+    w.values[p[1::2], 0, s[1::2]] = -2.0 ** gap
+    layer, *_ = make(pkg, cuda, w, hq, 1, d, io, attnScale=math.log(2.0))
+    q = torch.zeros(1, hq, d, dtype=TYPES[io])
+    q[..., 0] = 1
+    out = layer.decode(q.view(1, -1).to(cuda), ints([n - 1], cuda), w.device_table(cuda))
+    weight = torch.softmax(w.keys[p, 0, s, 0].double() * math.log(2.0), 0)
+    v = w.values[p, 0, s].double()
+    exp, size = weight @ v, weight @ v.abs()
+    # a score of at most one power of two, its roundings and the exponential's 2^-22; 700 / 16 steps over four warps and
+    # 24 joins, 2^-22 each; a weight's two parts, 21 bits or 15
+    share = 2 * 2.0 ** -22 + (700 / 16 / 4 + 24) * 2.0 ** -22 + (2.0 ** -15 if kept == "bf16" else 2.0 ** -21)
+    tol = share * size + ref.half_step(TYPES[io]) * exp.abs() + ref.smallest(TYPES[io])
+    for h in range(hq):
+        close(out[0].view(hq, d)[h], exp, tol, f"head {h}")
+
+
+FORMS = [(64, "fp16", "fp16", 16), (128, "bf16", "bf16", 16), (64, "fp32", "fp16", 32), (256, "fp32", "fp16", 16),
+         (64, "fp32", "fp32", 16), (128, "fp32", "bf16", 16), (64, "bf16", "bf16", 4), (100, "fp16", "fp16", 16)]
+
+
+@pytest.mark.parametrize("d,io,kept,page", FORMS)
+@pytest.mark.parametrize("wide", [1, WIDE])
+def test_decode_infinite_values(pkg, cuda, d, io, kept, page, wide):
+    """An infinite value that takes part is one in its dimension of the output, whatever its weight is made of, and
+    nowhere else."""
+    n, hq, inf = 400, 6, float("inf")
+    w = World([n] * 2, 2, d, page, kept, extra_width=wide)
+    w.values[w.table[0][0], 0, 0, 3] = inf
+    w.values[w.table[1][33 // page], 1, 33 % page, d - 1] = -inf
+    layer, *_ = make(pkg, cuda, w, hq, 2, d, io)
+    q = w.normal(2, hq, d, dtype=TYPES[io])
+    q[0, 0], q[0, 2], q[1, 3], q[1, 5] = 0, 0, 0, 0  # (equal scores: weights that the type holds without a rest)
+    out = layer.decode(q.view(2, -1).to(cuda), ints([n - 1] * 2, cuda), w.device_table(cuda)).view(2, hq, d).cpu()
+    for b in range(2):
+        exp, tol = ref.attend(q[b], w.keys, w.values, w.table[b], n - 1, page, d ** -0.5, out_type=TYPES[io], kept=w.kept)
+        assert int((~exp.isfinite()).sum()) == hq // 2
+        for h in range(hq):
+            fine = exp[h].isfinite()
+            assert torch.equal(out[b, h][~fine].float(), exp[h][~fine].float())
+            close(out[b, h][fine], exp[h][fine], tol[h][fine], f"sequence {b}, head {h}")
+
+
 # ---------------------------------------------------------------- append: scaled and partial rotations
 YARN = {"type": "yarn", "factor": 4.0, "original_context_length": 256.0, "beta_fast": 32.0, "beta_slow": 1.0}
 ROTATIONS = [
