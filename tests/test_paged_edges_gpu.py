@@ -12,7 +12,7 @@ import torch
 
 from oracle import oracle
 from tests import paged_ref as ref
-from tests.test_paged_gpu import PAIRS, TYPES, WIDE, World, close, ints, make
+from tests.test_paged_gpu import PAIRS, TYPES, WIDE, World, by_head, close, ints, make
 
 pytestmark = pytest.mark.gpu
 
@@ -276,6 +276,29 @@ def test_decode_infinite_values(pkg, cuda, d, io, kept, page, wide):
             fine = exp[h].isfinite()
             assert torch.equal(out[b, h][~fine].float(), exp[h][~fine].float())
             close(out[b, h][fine], exp[h][fine], tol[h][fine], f"sequence {b}, head {h}")
+
+
+@pytest.mark.parametrize("d,io,kept,page", FORMS)
+@pytest.mark.parametrize("wide", [1, WIDE])
+def test_decode_infinite_scores(pkg, cuda, d, io, kept, page, wide):
+    """A key whose score is minus infinity takes no part; one whose score is infinity leaves no number."""
+    n, hq, inf = 400, 6, float("inf")
+    w = World([n] * 2, 2, d, page, kept, extra_width=wide)
+    at = [(w.table[b][t // page], t % page) for b, t in ((0, n - 1), (1, 100))]
+    layer, k, *_ = make(pkg, cuda, w, hq, 2, d, io)
+    for (p, s), value in zip(at, (-inf, inf)):
+        by_head(k, w.layout)[p, 0, s, 1] = value
+    q = w.normal(2, hq, d, dtype=TYPES[io])
+    q[:, :, 1] = 0.5  # the infinity's sign is the score's, and the type holds it without a rest
+    out = layer.decode(q.view(2, -1).to(cuda), ints([n - 1] * 2, cuda), w.device_table(cuda)).view(2, hq, d)
+    assert out[1, :3].isnan().all()
+    exp, tol = ref.attend(q[1], w.keys, w.values, w.table[1], n - 1, page, d ** -0.5, out_type=TYPES[io], kept=w.kept)
+    close(out[1, 3:], exp[3:], tol[3:])
+    # sequence 0: the first kv head as if it ended one token earlier, the other with all tokens
+    exp, tol = ref.attend(q[0], w.keys, w.values, w.table[0], n - 1, page, d ** -0.5, out_type=TYPES[io], kept=w.kept)
+    close(out[0, 3:], exp[3:], tol[3:])
+    exp, tol = ref.attend(q[0], w.keys, w.values, w.table[0], n - 2, page, d ** -0.5, out_type=TYPES[io], kept=w.kept)
+    close(out[0, :3], exp[:3], tol[:3])
 
 
 # ---------------------------------------------------------------- append: scaled and partial rotations

@@ -44,7 +44,7 @@
 // heads per kv head (8 x 4097 19.6 us for 18.7).
 //
 // float32 activations over float16 pages: each query row is scaled by a power
-// of two and split into two float16 parts, so that the scores carry 22 bits, and
+// of two and split the same way, so that the scores carry 21 bits as well, and
 // the output keeps float32's use for its caller. K and V are exact as stored.
 #include <cooperative_groups.h>
 #include <math.h>
@@ -529,16 +529,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // largest element to [1, 2); a row of zeros or of values without an exponent stays
+        // largest element to [2^13, 2^14); a row of zeros or of values without an exponent stays
         int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-        if (ex < -100 || ex > 120) ex = top == 0.f ? 0 : max(-100, min(ex, 120));
+        if (ex < -100 || ex > 127) ex = top == 0.f ? 0 : max(-100, min(ex, 127));
+        ex -= 13;
         const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
 #pragma unroll
         for (int e = 0; e < D / 32; ++e) {
           const float v = x[e] * down;
-          const __half hi = __float2half_rn(v);
+          const __half hi = __float2half_rz(v);  // (parts as pack2_cut and pack2_rest form them)
           q_s[r * (C::kQPitch / 2) + lane + 32 * e] = hi;
-          q_s[(16 + r) * (C::kQPitch / 2) + lane + 32 * e] = __float2half_rn(v - __half2float(hi));
+          q_s[(16 + r) * (C::kQPitch / 2) + lane + 32 * e] = __float2half_rn(fmaf(v, kUp, -__half2float(hi)));
         }
         if (lane == 0)  // (the row's padding)
           *reinterpret_cast<float*>(q_s + r * (C::kQPitch / 2) + D) = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
@@ -568,7 +569,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       for (int e = 0; e < 2; ++e) {
         scale[nt][e] = p.a.attn_scale * kLog2e;
         if constexpr (SPLIT)
-          scale[nt][e] *= *reinterpret_cast<const float*>(q_s + (nt * 8 + 2 * t4 + e) * (C::kQPitch / 2) + D);
+          scale[nt][e] *= (1.f - 0x1p-23f) *  // (of the parts' kUp)
+                          *reinterpret_cast<const float*>(q_s + (nt * 8 + 2 * t4 + e) * (C::kQPitch / 2) + D);
       }
     }
 
