@@ -364,6 +364,29 @@ def test_append_scaled_and_partial_rotations(pkg, cuda, options, form, d, io, ke
             at += 1
 
 
+@pytest.mark.parametrize("d,kept", [(64, "fp32"), (128, "bf16"), (256, "fp32"), (100, "fp32")])
+def test_append_chunks_at_far_positions(pkg, cuda, d, kept):
+    """Angles of far positions are reduced in 64 bits, in the table of a page's slots too."""
+    hq, hk, page, n, theta = 4, 2, 64, 150, 1e6
+    start = (1 << 24) + 21
+    first = start // page
+    k, v = (torch.zeros(4, hk, page, d, dtype=TYPES[kept], device=cuda) for _ in range(2))
+    bounds = torch.zeros(4, hk, 2, d, dtype=TYPES[kept], device=cuda)
+    table = torch.full((1, first + 4), -1, dtype=torch.int32, device=cuda)
+    table[0, first:] = ints([2, 0, 3, 1], cuda)
+    layer = pkg.PagedAttention(hq * d, hq, 1 << 25, k, v, {"headDim": d, "kvHeadCount": hk, "ropeTheta": theta,
+                                                           "dtype": torch.float32}, key_bounds=bounds)
+    g = torch.Generator().manual_seed(0)
+    qkv = torch.randn(n, (hq + 2 * hk) * d, generator=g)
+    query = layer.append(qkv.to(cuda), ints([start], cuda), table, row_offsets=ints([0, n], cuda)).cpu()
+    assert layer.context.error() == 0
+    got = k.cpu()
+    for i in range(n):
+        q, kk, _ = ref.form_row(qkv[i], start + i, hq, hk, d, theta=theta)
+        close(query[i], q, ref.row_error(q, torch.float32, d))
+        close(got[(2, 0, 3, 1)[(start + i) // page - first], :, (start + i) % page], kk, ref.row_error(kk, TYPES[kept], d))
+
+
 @pytest.mark.parametrize("options", [{"rotaryDim": 0}, {"rotaryDim": 16}, {"ropePairCount": 5}, {"rotaryDim": 24, "ropePairCount": 0}],
                          ids=str)
 @pytest.mark.parametrize("form", ["one", "chunks", "chunks without bounds"])

@@ -716,8 +716,8 @@ cudaError_t append_by_rows(const tla_paged* P, const PagedArgs& p, const void* q
          pages * ((p.a.Hk + page_heads - 1) / page_heads) > 2 * P->base.ctx->sm_count)
     page_heads *= 2;
   const long long blocks = pages * ((p.a.Hk + page_heads - 1) / page_heads);
-  // Many blocks run four on an SM (64 registers): more reads in flight; few
-  // three, which spares the spills. Measured (three / four, us; * what the rule
+  // Many blocks run four on an SM (64 registers each thread): more reads in
+  // flight; few run three (84). Measured (three / four, us; * what the rule
   // takes), 32 + 8 + 8 heads of 128: 1 chunk of 2048 rows 17.1* / 15.2, of 8192
   // 41.8 / 37.6*, 16 of up to 256 16.5* / 17.2, of up to 1024 41.2 / 43.0*, of
   // up to 2047 95 / 88* (with QK-norm, token-major bfloat16 pages 104 / 93*);
