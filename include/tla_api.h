@@ -411,8 +411,9 @@ int tla_paged_decode(tla_paged* layer, const void* query, const int32_t* positio
  * heads and over d of q_d * high_d where q_d > 0 and q_d * low_d where q_d < 0,
  * low and high being its bounds: an upper bound on the summed dot products
  * with any of its keys. It is summed in 64 bits and rounded to 32; ties go to
- * the lower page. (Bounds of 16 bits that are not finite count as numbers of the
- * next exponent, an infinity as 65536 in float16 and 2^128 in bfloat16.) Needs a pool with bounds and a positive attn_scale.
+ * the lower page. (Bounds of 16 bits that are not finite count as numbers of
+ * the next exponent, an infinity as 65536 in float16 and 2^128 in bfloat16.)
+ * Needs a pool with bounds and a positive attn_scale.
  *   pages_out device int32 [batch][kv_head_count][page_count], rising, then -1 */
 int tla_paged_select(tla_paged* layer, const void* query, const int32_t* positions, const int32_t* page_table,
                      int32_t table_width, int32_t first_pages, int32_t last_pages, int32_t* pages_out,

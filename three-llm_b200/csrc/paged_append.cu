@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 5)
   griddep_wait();
   griddep_launch_dependents();
   append_rows<IO, CT, D, EXACT, TURNED>(p, qkv, offsets, rows, query_out, parts, part_heads, true,
-                                static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5));
+                                        static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5));
 }
 
 // Chunks into a pool with bounds: the first blocks take the touched pages'
@@ -634,8 +634,9 @@ __global__ void __launch_bounds__(kPageThreads, kBlocks)
   if (static_cast<int>(blockIdx.x) < page_blocks)
     append_page<IO, CT, D, EXACT, TURNED>(p, qkv, offsets, rows, page_heads, blockIdx.x);
   else
-    append_rows<IO, CT, D, EXACT, TURNED>(p, qkv, offsets, rows, query_out, parts, part_heads, false,
-                                          static_cast<int64_t>(blockIdx.x - page_blocks) * (kPageThreads / 32) + (threadIdx.x >> 5));
+    append_rows<IO, CT, D, EXACT, TURNED>(
+        p, qkv, offsets, rows, query_out, parts, part_heads, false,
+        static_cast<int64_t>(blockIdx.x - page_blocks) * (kPageThreads / 32) + (threadIdx.x >> 5));
 }
 
 // Bounds of the pages that a chunk touched, any shape: the block of a page's
@@ -730,11 +731,14 @@ cudaError_t append_by_rows(const tla_paged* P, const PagedArgs& p, const void* q
   auto k = D < 128 ? paged_append_chunks_kernel<IO, CT, 128, false, 3, TURNED>
                    : paged_append_chunks_kernel<IO, CT, 256, false, 3, TURNED>;
   if (D == 64)
-    k = many ? paged_append_chunks_kernel<IO, CT, 64, true, 4, TURNED> : paged_append_chunks_kernel<IO, CT, 64, true, 3, TURNED>;
+    k = many ? paged_append_chunks_kernel<IO, CT, 64, true, 4, TURNED>
+             : paged_append_chunks_kernel<IO, CT, 64, true, 3, TURNED>;
   if (D == 128)
-    k = many ? paged_append_chunks_kernel<IO, CT, 128, true, 4, TURNED> : paged_append_chunks_kernel<IO, CT, 128, true, 3, TURNED>;
-  return launch_pdl(k, static_cast<unsigned>(grid), kPageThreads, 0, stream, p, static_cast<const IO*>(qkv), offsets, rows,
-                    static_cast<IO*>(query_out), static_cast<int>(parts), part_heads, static_cast<int>(blocks), page_heads);
+    k = many ? paged_append_chunks_kernel<IO, CT, 128, true, 4, TURNED>
+             : paged_append_chunks_kernel<IO, CT, 128, true, 3, TURNED>;
+  return launch_pdl(k, static_cast<unsigned>(grid), kPageThreads, 0, stream, p, static_cast<const IO*>(qkv), offsets,
+                    rows, static_cast<IO*>(query_out), static_cast<int>(parts), part_heads, static_cast<int>(blocks),
+                    page_heads);
 }
 
 template <typename IO, typename CT>

@@ -53,8 +53,7 @@ __device__ __forceinline__ void store_out(IO* out, const IO* gate, int64_t i, fl
 // workspace, or where one block has all the tokens to the call's output.
 template <typename IO>
 __device__ __forceinline__ void join_warps(const float* red, int D, int heads, int64_t first_row, int share, int shares,
-                                           const IO* gate, IO* out,
-                                           float* __restrict__ partial) {
+                                           const IO* gate, IO* out, float* __restrict__ partial) {
   for (int i = threadIdx.x; i < heads * D; i += kThreads) {
     const int h = i / D, d = i - h * D;
     float top = -INFINITY, sum = 0.f, acc = 0.f;
@@ -432,8 +431,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 // Joins the shares' triples; a block per output row.
 template <typename IO>
 __global__ void __launch_bounds__(kThreads)
-    paged_join_kernel(const float* __restrict__ partial, int shares, int D, const IO* gate,
-                      IO* out) {
+    paged_join_kernel(const float* __restrict__ partial, int shares, int D, const IO* gate, IO* out) {
   griddep_wait();
   griddep_launch_dependents();
   const int64_t row = blockIdx.x;
